@@ -305,6 +305,109 @@ typedef struct lb_layer_rows_args {
 lb_status lb_layer_rows(const lb_layer_rows_args *args, void *stream);
 
 /*
+ * A KV cache in 8 bits (the reference's cache is fp16 only: KV Select, torch_npu_smollm.py:325-329).  Each sequence
+ * and KV head holds blocks of LB_KV_BLOCK slots; a full block is held as 8-bit codes with one scale for its keys and
+ * one for its values, a being the largest magnitude of the block's LB_KV_BLOCK x head_dim values:
+ *   LB_KV_INT8   scale = a / 127 (fp32),  code = rint(127 x / a), to even
+ *   LB_KV_FP8    scale = a / 448,         code = e4m3(448 x / a), to even (OCP e4m3fn)
+ * and a code stands for code * scale.  A block is quantised once, when its last row arrives; until then, and until
+ * the block after it is full too, its rows are held in fp16 in a ring of two blocks (slot mod 128).  So nothing is
+ * ever quantised twice, the held values do not depend on how the rows were split into calls, and positions may be taken
+ * back (drafted tokens that were rejected) as far as the start of the block before the one that is open.
+ * A row with a key or value that is not finite gets a key of NaNs, and a block with one NaN scales: the rows that
+ * attend to it are NaN, others are not.
+ * Layouts, per sequence and KV head (row-major; D = head_dim, blocks = capacity / 64):
+ *   key_codes    [blocks][64 slots][D]          key_tail    fp16 [2][64 slots][D]
+ *   value_codes  [blocks][D][64 places]         value_tail  fp16 [2][D][64 places]
+ * slot 16 s + 4 g + r of a block lying at place 16 g + 4 s + r (the order in which the matrix instructions take a
+ * value row), and the block of slots 64 i .. 64 i + 63 in half i mod 2 of the tails.
+ * The program keeps each sequence's length; the calls read it from the device, so they can be captured.
+ */
+#define LB_KV_BLOCK 64
+
+typedef enum lb_kv_format { LB_KV_INT8 = 0, LB_KV_FP8 = 1 } lb_kv_format;
+
+typedef struct lb_kv_cache {
+  uint32_t format;             /* lb_kv_format */
+  uint32_t head_dim;           /* 64 or 128 */
+  int64_t batch, kv_heads;     /* 1..65535 each */
+  int64_t capacity;            /* slots per sequence, a multiple of 64 up to 2^28 */
+  void *key_codes, *value_codes;    /* [batch, kv_heads, capacity * head_dim] bytes, 16-byte aligned */
+  float *key_scales, *value_scales; /* [batch, kv_heads, capacity / 64], 16-byte aligned */
+  void *key_tail, *value_tail;      /* fp16 [batch, kv_heads, 128 * head_dim], 16-byte aligned */
+} lb_kv_cache;
+
+/* Strides in elements of fp16 rows of head_dim contiguous values (16-byte aligned: multiples of 8, >= 0). */
+typedef struct lb_kv_rows {
+  const void *data;
+  int64_t batch_stride, row_stride, head_stride;
+} lb_kv_rows;
+
+typedef struct lb_kv_append_args {
+  uint32_t struct_size;        /* sizeof(lb_kv_append_args) */
+  uint32_t reserved;
+  lb_kv_cache cache;
+  int64_t seq;                 /* rows of k and v per sequence */
+  lb_kv_rows k, v;             /* [batch, seq, kv_heads] rows */
+  const int64_t *position;     /* device [batch]: the slot of a sequence's first row (the slots it holds) */
+  const int64_t *rows;         /* device [batch], 0..seq, or NULL: how many of its rows are appended (a padded batch) */
+  const void *cos, *sin;       /* fp16 [capacity, head_dim] RoPE tables, or NULL: k is appended as it is */
+} lb_kv_append_args;
+
+/*
+ * Appends rows[b] (NULL: seq) rows to every sequence, at slots position[b] ..: with tables each key is rotated first,
+ * fp16(fp16(k cos) + fp16(rotate_half(k) sin)) (torch_npu_smollm.py:262-303).  A sequence whose rows would lie outside
+ * 0 .. capacity - 1 is left alone, as is everything behind the appended rows.  One launch.
+ */
+lb_status lb_kv_append(const lb_kv_append_args *args, void *stream);
+
+typedef struct lb_kv_read_args {
+  uint32_t struct_size;        /* sizeof(lb_kv_read_args) */
+  uint32_t reserved;
+  lb_kv_cache cache;
+  const int64_t *length;       /* device [batch]: the slots that each sequence holds */
+  int64_t start, count;        /* slots start .. start + count - 1 of every sequence, within the capacity */
+  lb_kv_rows keys, values;     /* written: row i of [batch, count, kv_heads] rows is slot start + i */
+} lb_kv_read_args;
+
+/*
+ * fp16(fp32(code * scale)) of full blocks, and the fp16 rows of the open block.  Rows at or past a sequence's length are
+ * left as they are; a length outside 0..capacity gives NaN rows.  One launch.
+ */
+lb_status lb_kv_read(const lb_kv_read_args *args, void *stream);
+
+typedef struct lb_kv_attention_args {
+  uint32_t struct_size;        /* sizeof(lb_kv_attention_args) */
+  uint32_t reserved;
+  lb_kv_cache cache;
+  int64_t seq, heads;          /* heads a multiple of kv_heads: query head h uses KV head h / (heads / kv_heads) */
+  lb_kv_rows q, out;           /* [batch, seq, heads] rows; out is written */
+  const int64_t *position;     /* device [batch]: the slot of a sequence's first query row */
+  const int64_t *rows;         /* device [batch], 0..seq, or NULL: its query rows (out rows behind them stay as they are) */
+  const void *cos, *sin;       /* fp16 [capacity, head_dim], or NULL: rotates q (and k) as lb_kv_append does */
+  lb_kv_rows k, v;             /* data NULL: the rows are in the cache already; else appended first, as lb_kv_append */
+  float scale;                 /* score scale, finite and >= 0 (usually 1 / sqrt(head_dim)) */
+  uint32_t reserved2;
+  int64_t limit;               /* about how many slots the longest sequence holds, for the split of the work (any value
+                                  gives the same sums in another order); 0: capacity */
+  void *workspace;             /* lb_kv_attention_workspace_bytes, 16-byte aligned, any contents; calls sharing it must
+                                  be ordered (one stream) */
+  size_t workspace_bytes;
+} lb_kv_attention_args;
+
+/* Bytes of workspace lb_kv_attention needs for these arguments (0 when none); host-only. */
+lb_status lb_kv_attention_workspace_bytes(const lb_kv_attention_args *args, size_t *bytes);
+
+/*
+ * Causal grouped-query attention over the held values: the row at slot p attends over slots 0 .. p of its sequence
+ * (which holds position + rows slots, the query rows' own among them), scores, softmax and sums in fp32, the
+ * probabilities rounded to fp16 for the product with V, the output to fp16.  Replaces the attention of the reference's
+ * decode and prefill graphs (torch_npu_smollm.py:174-182, :195-340) over a cache that those did not have.  A sequence
+ * whose rows lie outside the capacity gives NaN rows.
+ */
+lb_status lb_kv_attention(const lb_kv_attention_args *args, void *stream);
+
+/*
  * Greedy step: t = first index of the largest logit (NaN logits are never chosen);
  * token[0] = t; if 0 <= position[0] < limit: tokens[position[0]] = t and position[0] += 1;
  * h_next = embedding[t] (fp16 [hidden]).  Replaces the host argmax and the next step's embedding

@@ -1,0 +1,313 @@
+// lb_kv_append, lb_kv_read and lb_kv_attention: the KV cache in 8 bits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+
+#include "../../include/lowbit_decode_hip.h"
+#include "abi_util.h"
+#include "lb_kv.h"
+
+using namespace lb;
+using namespace lb::abi;
+
+namespace {
+
+constexpr int64_t kMaxCapacity = (int64_t)1 << 28, kMaxStride = (int64_t)1 << 40, kMaxRows = (int64_t)1 << 28;
+
+KvCache cache_params(const lb_kv_cache &c) {
+  KvCache p{};
+  p.kc = static_cast<uint8_t *>(c.key_codes);
+  p.vc = static_cast<uint8_t *>(c.value_codes);
+  p.ks = c.key_scales;
+  p.vs = c.value_scales;
+  p.kt = static_cast<f16 *>(c.key_tail);
+  p.vt = static_cast<f16 *>(c.value_tail);
+  p.kv_heads = (int)c.kv_heads;
+  p.capacity = (int)c.capacity;
+  p.blocks = (int)(c.capacity / kKvBlock);
+  return p;
+}
+
+KvRows rows_params(const lb_kv_rows &r) {
+  return {static_cast<f16 *>(const_cast<void *>(r.data)), (long long)r.batch_stride, (long long)r.row_stride, (long long)r.head_stride};
+}
+
+// The cache's buffers, and whether they are sound.
+lb_status check_cache(const char *what, const lb_kv_cache &c, Range (&r)[6]) {
+  if (c.format > LB_KV_FP8) return fail(LB_INVALID_ARGUMENT, "%s: unknown cache format %u", what, c.format);
+  if (c.head_dim != 64 && c.head_dim != 128) return fail(LB_UNSUPPORTED, "%s: head_dim %u (64 and 128 are supported)", what, c.head_dim);
+  if (c.batch < 1 || c.batch > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.capacity < kKvBlock || c.capacity > kMaxCapacity ||
+      c.capacity % kKvBlock != 0)
+    return fail(LB_INVALID_ARGUMENT, "%s: batch and kv_heads 1..65535, capacity a multiple of %d up to 2^28 required", what, kKvBlock);
+  const size_t heads = (size_t)c.batch * c.kv_heads, codes = heads * c.capacity * c.head_dim, scales = heads * (c.capacity / kKvBlock) * 4,
+               tail = heads * (2 * kKvBlock) * c.head_dim * 2;   // (below 2^32 * 2^35 bytes)
+  r[0] = range_of(c.key_codes, codes, "key_codes");
+  r[1] = range_of(c.value_codes, codes, "value_codes");
+  r[2] = range_of(c.key_scales, scales, "key_scales");
+  r[3] = range_of(c.value_scales, scales, "value_scales");
+  r[4] = range_of(c.key_tail, tail, "key_tail");
+  r[5] = range_of(c.value_tail, tail, "value_tail");
+  for (int i = 0; i < 6; ++i) {
+    if (!r[i].lo || r[i].lo % 16 != 0) return fail(LB_INVALID_ARGUMENT, "%s: %s must be non-NULL with 16-byte alignment", what, r[i].name);
+    if (r[i].hi < r[i].lo) return fail(LB_INVALID_ARGUMENT, "%s: %s does not fit the address space", what, r[i].name);
+    for (int k = 0; k < i; ++k)
+      if (overlaps(r[i], r[k])) return fail(LB_INVALID_ARGUMENT, "%s: %s overlaps %s", what, r[k].name, r[i].name);
+  }
+  return LB_OK;
+}
+
+// fp16 rows [batch, seq, heads] of dim values; written ones may not share memory with one another.
+lb_status check_rows(const char *what, const char *name, const lb_kv_rows &v, int64_t batch, int64_t seq, int64_t heads, int64_t dim,
+                     bool written, Range &range) {
+  if (!v.data || !aligned(v.data, 16)) return fail(LB_INVALID_ARGUMENT, "%s: %s must be non-NULL with 16-byte alignment", what, name);
+  struct Axis { int64_t size, stride; } axes[3] = {{batch, v.batch_stride}, {seq, v.row_stride}, {heads, v.head_stride}};
+  int64_t span = dim;
+  for (Axis &a : axes) {
+    if (a.size == 1) a.stride = 0;
+    if (a.stride < 0 || a.stride > kMaxStride || a.stride % 8 != 0)
+      return fail(LB_INVALID_ARGUMENT, "%s: strides of %s must be multiples of 8, 0 to 2^40 elements", what, name);
+    span += (a.size - 1) * a.stride;   // (below 2^28 * 2^40 * 3)
+  }
+  if (span > INT64_MAX / 4) return fail(LB_INVALID_ARGUMENT, "%s: %s is past the address space", what, name);
+  if (written) {
+    std::sort(axes, axes + 3, [](const Axis &a, const Axis &b) { return a.stride < b.stride; });
+    int64_t extent = dim;
+    for (const Axis &a : axes) {
+      if (a.size == 1) continue;
+      if (a.stride < extent) return fail(LB_INVALID_ARGUMENT, "%s: rows of %s overlap one another", what, name);
+      extent += (a.size - 1) * a.stride;
+    }
+  }
+  range = range_of(v.data, (size_t)span * 2, name);
+  return range.hi < range.lo ? fail(LB_INVALID_ARGUMENT, "%s: %s does not fit the address space", what, name) : LB_OK;
+}
+
+lb_status check_counts(const char *what, const char *name, const int64_t *p, int64_t batch, bool needed, Range &range) {
+  if (!p && !needed) {
+    range = Range{};
+    return LB_OK;
+  }
+  if (!p || !aligned(p, 8)) return fail(LB_INVALID_ARGUMENT, "%s: %s must be a non-NULL device array of 64-bit integers", what, name);
+  range = range_of(p, (size_t)batch * 8, name);
+  return LB_OK;
+}
+
+lb_status check_tables(const char *what, const void *cos, const void *sin, const lb_kv_cache &c, Range (&r)[2]) {
+  r[0] = r[1] = Range{};
+  if (!cos && !sin) return LB_OK;
+  if (!cos || !sin || !aligned(cos, 16) || !aligned(sin, 16))
+    return fail(LB_INVALID_ARGUMENT, "%s: cos and sin go together, with 16-byte alignment", what);
+  r[0] = range_of(cos, (size_t)c.capacity * c.head_dim * 2, "cos");
+  r[1] = range_of(sin, (size_t)c.capacity * c.head_dim * 2, "sin");
+  return LB_OK;
+}
+
+lb_status check_apart(const char *what, const Range *written, int nw, const Range *read, int nr) {
+  for (int i = 0; i < nw; ++i)
+    for (int k = 0; k < nr; ++k)
+      if (overlaps(written[i], read[k])) return fail(LB_INVALID_ARGUMENT, "%s: %s overlaps %s", what, written[i].name, read[k].name);
+  return LB_OK;
+}
+
+// Calls f with the kernels' format and head size as constants.
+template <class F>
+void with_kind(const lb_kv_cache &c, F &&f) {
+  if (c.format == LB_KV_INT8) {
+    c.head_dim == 64 ? f(std::integral_constant<int, KV_INT8>{}, std::integral_constant<int, 64>{})
+                     : f(std::integral_constant<int, KV_INT8>{}, std::integral_constant<int, 128>{});
+  } else {
+    c.head_dim == 64 ? f(std::integral_constant<int, KV_FP8>{}, std::integral_constant<int, 64>{})
+                     : f(std::integral_constant<int, KV_FP8>{}, std::integral_constant<int, 128>{});
+  }
+}
+
+lb_status check_append(const char *what, const lb_kv_cache &c, int64_t seq, const lb_kv_rows &k, const lb_kv_rows &v,
+                       const int64_t *position, const int64_t *rows, const void *cos, const void *sin, Range (&cache)[6], Range (&ins)[6]) {
+  if (const lb_status st = check_cache(what, c, cache); st != LB_OK) return st;
+  if (seq < 1 || seq > kMaxRows) return fail(LB_INVALID_ARGUMENT, "%s: seq 1 to 2^28 required", what);
+  Range tables[2];
+  if (const lb_status st = check_rows(what, "k", k, c.batch, seq, c.kv_heads, c.head_dim, false, ins[0]); st != LB_OK) return st;
+  if (const lb_status st = check_rows(what, "v", v, c.batch, seq, c.kv_heads, c.head_dim, false, ins[1]); st != LB_OK) return st;
+  if (const lb_status st = check_counts(what, "position", position, c.batch, true, ins[2]); st != LB_OK) return st;
+  if (const lb_status st = check_counts(what, "rows", rows, c.batch, false, ins[3]); st != LB_OK) return st;
+  if (const lb_status st = check_tables(what, cos, sin, c, tables); st != LB_OK) return st;
+  ins[4] = tables[0];
+  ins[5] = tables[1];
+  return check_apart(what, cache, 6, ins, 6);
+}
+
+void launch_append(const lb_kv_cache &c, int64_t seq, const lb_kv_rows &k, const lb_kv_rows &v, const int64_t *position,
+                   const int64_t *rows, const void *cos, const void *sin, hipStream_t s) {
+  KvAppendParams p{};
+  p.c = cache_params(c);
+  p.k = rows_params(k);
+  p.v = rows_params(v);
+  p.position = position;
+  p.rows = rows;
+  p.cos = static_cast<const f16 *>(cos);
+  p.sin = static_cast<const f16 *>(sin);
+  p.seq = (int)seq;
+  // Blocks that seq consecutive slots can fall into, wherever the first lies.
+  const int64_t blocks = std::min((seq + 2 * kKvBlock - 2) / kKvBlock, c.capacity / kKvBlock);
+  with_kind(c, [&](auto fmt, auto dim) {
+    hipLaunchKernelGGL((kv_append_kernel<fmt(), dim()>), dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(2 * dim()), 0, s, p);
+  });
+}
+
+// Tiles of query rows, and the parts that the slots are taken in.
+struct AttendPlan {
+  int qt, tiles, splits, chunk;
+  size_t sums, bytes;   // floats of the partial sums, bytes of workspace
+};
+
+AttendPlan attend_plan(const lb_kv_attention_args *a) {
+  AttendPlan plan{};
+  const lb_kv_cache &c = a->cache;
+  const int64_t rows = a->seq * (a->heads / c.kv_heads);
+  plan.qt = rows > 16 ? 2 : 1;
+  plan.tiles = (int)((rows + 16 * plan.qt - 1) / (16 * plan.qt));
+  const int64_t units = c.batch * c.kv_heads * plan.tiles;
+  const int64_t held = a->limit > 0 ? std::min(a->limit, c.capacity) : c.capacity, blocks = (held + kKvBlock - 1) / kKvBlock;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(1024 / units, blocks / 4));
+  plan.chunk = (int)((blocks + want - 1) / want + 3) / 4 * 4;
+  plan.splits = (int)((blocks + plan.chunk - 1) / plan.chunk);
+  if (plan.splits > 1) {
+    const size_t parts = (size_t)units * plan.splits * 16 * plan.qt;
+    plan.sums = parts * c.head_dim;
+    plan.bytes = (plan.sums + parts * 2) * sizeof(float);
+  }
+  return plan;
+}
+
+lb_status check_shape(const char *what, const lb_kv_attention_args *a) {
+  const lb_kv_cache &c = a->cache;
+  if (a->seq < 1 || a->seq > kMaxRows || a->heads < 1 || a->heads > 65535 || a->heads % c.kv_heads != 0 ||
+      a->seq * (a->heads / c.kv_heads) > kMaxRows)
+    return fail(LB_INVALID_ARGUMENT, "%s: heads a multiple of kv_heads up to 65535, and 1 to 2^28 rows of a KV head required", what);
+  if (c.kv_heads * ((a->seq * (a->heads / c.kv_heads) + 15) / 16) > INT32_MAX / 1024)
+    return fail(LB_UNSUPPORTED, "%s: too many rows for one launch", what);
+  if (!(a->scale >= 0.0f) || !std::isfinite(a->scale)) return fail(LB_INVALID_ARGUMENT, "%s: scale must be finite and >= 0", what);
+  if (a->limit < 0) return fail(LB_INVALID_ARGUMENT, "%s: limit must be >= 0", what);
+  return LB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+lb_status lb_kv_append(const lb_kv_append_args *a, void *stream) {
+  const char *what = "lb_kv_append";
+  if (const lb_status bad = refuse_if_failed(what); bad != LB_OK) return bad;
+  if (!a) return fail(LB_INVALID_ARGUMENT, "%s: args is NULL", what);
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  Range cache[6], ins[6];
+  if (const lb_status st = check_append(what, a->cache, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, cache, ins); st != LB_OK)
+    return st;
+  launch_append(a->cache, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, static_cast<hipStream_t>(stream));
+  return launch_status(what);
+}
+
+lb_status lb_kv_read(const lb_kv_read_args *a, void *stream) {
+  const char *what = "lb_kv_read";
+  if (const lb_status bad = refuse_if_failed(what); bad != LB_OK) return bad;
+  if (!a) return fail(LB_INVALID_ARGUMENT, "%s: args is NULL", what);
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  const lb_kv_cache &c = a->cache;
+  Range cache[6], outs[2], length;
+  if (const lb_status st = check_cache(what, c, cache); st != LB_OK) return st;
+  if (a->start < 0 || a->count < 1 || a->count > c.capacity || a->start > c.capacity - a->count)
+    return fail(LB_INVALID_ARGUMENT, "%s: start >= 0, count >= 1 and start + count <= capacity required", what);
+  if (const lb_status st = check_counts(what, "length", a->length, c.batch, true, length); st != LB_OK) return st;
+  if (const lb_status st = check_rows(what, "keys", a->keys, c.batch, a->count, c.kv_heads, c.head_dim, true, outs[0]); st != LB_OK) return st;
+  if (const lb_status st = check_rows(what, "values", a->values, c.batch, a->count, c.kv_heads, c.head_dim, true, outs[1]); st != LB_OK) return st;
+  if (const lb_status st = check_apart(what, outs, 2, cache, 6); st != LB_OK) return st;
+  if (const lb_status st = check_apart(what, outs, 2, &length, 1); st != LB_OK) return st;
+  if (overlaps(outs[0], outs[1])) return fail(LB_INVALID_ARGUMENT, "%s: keys overlaps values", what);
+  KvReadParams p{};
+  p.c = cache_params(c);
+  p.length = a->length;
+  p.keys = rows_params(a->keys);
+  p.values = rows_params(a->values);
+  p.start = (int)a->start;
+  p.count = (int)a->count;
+  const int64_t blocks = (a->start + a->count - 1) / kKvBlock - a->start / kKvBlock + 1;
+  with_kind(c, [&](auto fmt, auto dim) {
+    hipLaunchKernelGGL((kv_read_kernel<fmt(), dim()>), dim3((unsigned)blocks, (unsigned)c.kv_heads, (unsigned)c.batch), dim3(2 * dim()), 0,
+                       static_cast<hipStream_t>(stream), p);
+  });
+  return launch_status(what);
+}
+
+lb_status lb_kv_attention_workspace_bytes(const lb_kv_attention_args *a, size_t *bytes) {
+  const char *what = "lb_kv_attention_workspace_bytes";
+  if (!a || !bytes) return fail(LB_INVALID_ARGUMENT, "%s: args and bytes must be non-NULL", what);
+  *bytes = 0;
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  Range cache[6];
+  if (const lb_status st = check_cache(what, a->cache, cache); st != LB_OK) return st;
+  if (const lb_status st = check_shape(what, a); st != LB_OK) return st;
+  *bytes = attend_plan(a).bytes;
+  return ok();
+}
+
+lb_status lb_kv_attention(const lb_kv_attention_args *a, void *stream) {
+  const char *what = "lb_kv_attention";
+  if (const lb_status bad = refuse_if_failed(what); bad != LB_OK) return bad;
+  if (!a) return fail(LB_INVALID_ARGUMENT, "%s: args is NULL", what);
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  const lb_kv_cache &c = a->cache;
+  const bool appends = a->k.data || a->v.data;
+  Range cache[6], ins[6], q, out, counts[2], tables[2];
+  if (const lb_status st = check_cache(what, c, cache); st != LB_OK) return st;
+  if (const lb_status st = check_shape(what, a); st != LB_OK) return st;
+  if (appends)
+    if (const lb_status st = check_append(what, c, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, cache, ins); st != LB_OK) return st;
+  if (const lb_status st = check_rows(what, "q", a->q, c.batch, a->seq, a->heads, c.head_dim, false, q); st != LB_OK) return st;
+  if (const lb_status st = check_rows(what, "out", a->out, c.batch, a->seq, a->heads, c.head_dim, true, out); st != LB_OK) return st;
+  if (const lb_status st = check_counts(what, "position", a->position, c.batch, true, counts[0]); st != LB_OK) return st;
+  if (const lb_status st = check_counts(what, "rows", a->rows, c.batch, false, counts[1]); st != LB_OK) return st;
+  if (const lb_status st = check_tables(what, a->cos, a->sin, c, tables); st != LB_OK) return st;
+  const AttendPlan plan = attend_plan(a);
+  if (plan.bytes && (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < plan.bytes))
+    return fail(LB_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %zu bytes required (got %zu)", what, plan.bytes, a->workspace_bytes);
+  const Range writes[] = {out, plan.bytes ? range_of(a->workspace, plan.bytes, "workspace") : Range{}};
+  const Range reads[] = {q, counts[0], counts[1], tables[0], tables[1], appends ? ins[0] : Range{}, appends ? ins[1] : Range{}};
+  if (const lb_status st = check_apart(what, writes, 2, reads, 7); st != LB_OK) return st;
+  if (const lb_status st = check_apart(what, writes, 2, cache, 6); st != LB_OK) return st;
+  if (appends)
+    if (const lb_status st = check_apart(what, cache, 6, &q, 1); st != LB_OK) return st;
+  if (overlaps(writes[0], writes[1])) return fail(LB_INVALID_ARGUMENT, "%s: out overlaps workspace", what);
+
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (appends) launch_append(c, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, s);
+  KvAttendParams p{};
+  p.c = cache_params(c);
+  p.q = rows_params(a->q);
+  p.out = rows_params(a->out);
+  p.position = a->position;
+  p.rows = a->rows;
+  p.cos = static_cast<const f16 *>(a->cos);
+  p.sin = static_cast<const f16 *>(a->sin);
+  p.partial = static_cast<float *>(a->workspace);
+  p.seq = (int)a->seq;
+  p.heads = (int)a->heads;
+  p.group = (int)(a->heads / c.kv_heads);
+  p.tiles = plan.tiles;
+  p.splits = plan.splits;
+  p.chunk = plan.chunk;
+  p.scale = a->scale * 1.44269504088896340736f;
+  const int64_t units = c.kv_heads * plan.tiles;
+  with_kind(c, [&](auto fmt, auto dim) {
+    auto run = [&](auto qt) {
+      hipLaunchKernelGGL((kv_attend_kernel<fmt(), dim(), qt()>), dim3((unsigned)(units * plan.splits), (unsigned)c.batch), dim3(256), 0, s, p);
+      if (plan.splits > 1)
+        hipLaunchKernelGGL((kv_join_kernel<dim(), qt()>), dim3((unsigned)(units * 16 * qt() / 4), (unsigned)c.batch), dim3(256), 0, s, p, plan.sums);
+    };
+    plan.qt == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+  });
+  return launch_status(what);
+}
+
+}  // extern "C"

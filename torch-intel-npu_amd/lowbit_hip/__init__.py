@@ -16,7 +16,7 @@ import torch
 
 LIBRARY_PATH = Path(os.environ.get('LOWBIT_HIP_LIBRARY', Path(__file__).resolve().parent.parent / 'liblowbit_hip.so'))
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 OK, INVALID_ARGUMENT, OUT_OF_MEMORY, UNSUPPORTED, DEVICE_FAILED, INTERNAL = 0, 1, 2, 5, 10, 12
 FORMATS = {'int8': 0, 'int4': 1, 'nf4': 2, 'fp16': 3}
 FLAG_FORCE_GEMV, FLAG_FORCE_GEMM, FLAG_FORCE_GENERIC, FLAG_FORCE_STREAM, FLAG_FORCE_WIDE = 0x1, 0x2, 0x4, 0x20, 0x40
@@ -29,9 +29,12 @@ EXPORTS = ('lb_abi_version', 'lb_status_name', 'lb_last_error', 'lb_failed', 'lb
 NOALLOC_SCRATCH_BYTES = 32 << 20   # LB_NOALLOC_SCRATCH_BYTES
 DECODE_EXPORTS = ('lb_fused_linear', 'lb_decode_attention', 'lb_argmax_next', 'lb_head_next', 'lb_decode_layer',
                   'lb_decode_stack_prepare', 'lb_decode_stack', 'lb_decode_stack_release', 'lb_decode_check',
-                  'lb_rms_rows', 'lb_layer_rows')
+                  'lb_rms_rows', 'lb_layer_rows', 'lb_kv_append', 'lb_kv_read', 'lb_kv_attention_workspace_bytes',
+                  'lb_kv_attention')
 PROLOGUES = {'none': 0, 'rmsnorm': 1, 'silu_mul': 2}
 MAX_PROBLEMS, MAX_RANK, MAX_FUSED_K = 3, 32, 1536
+KV_BLOCK = 64                                # LB_KV_BLOCK: slots of a cache block that share a scale
+KV_FORMATS = {'int8': 0, 'fp8': 1}           # lb_kv_format
 def attention_workspace_bytes(heads, capacity):
     """LB_ATTN_WORKSPACE_BYTES: tagged score words [heads][ceil(capacity / 48) * 16], launch count, timeout."""
     return heads * ((capacity + 47) // 48) * 128 + 16
@@ -176,6 +179,45 @@ class LayerRowsArgs(ctypes.Structure):
                 ('workspace', ctypes.c_void_p), ('workspace_bytes', ctypes.c_size_t)]
 
 
+class KVCacheStruct(ctypes.Structure):
+    """Mirror of lb_kv_cache."""
+    _fields_ = [('format', ctypes.c_uint32), ('head_dim', ctypes.c_uint32), ('batch', ctypes.c_int64),
+                ('kv_heads', ctypes.c_int64), ('capacity', ctypes.c_int64),
+                ('key_codes', ctypes.c_void_p), ('value_codes', ctypes.c_void_p),
+                ('key_scales', ctypes.c_void_p), ('value_scales', ctypes.c_void_p),
+                ('key_tail', ctypes.c_void_p), ('value_tail', ctypes.c_void_p)]
+
+
+class KVRows(ctypes.Structure):
+    """Mirror of lb_kv_rows."""
+    _fields_ = [('data', ctypes.c_void_p), ('batch_stride', ctypes.c_int64), ('row_stride', ctypes.c_int64),
+                ('head_stride', ctypes.c_int64)]
+
+
+class KVAppendArgs(ctypes.Structure):
+    """Mirror of lb_kv_append_args."""
+    _fields_ = [('struct_size', ctypes.c_uint32), ('reserved', ctypes.c_uint32), ('cache', KVCacheStruct),
+                ('seq', ctypes.c_int64), ('k', KVRows), ('v', KVRows), ('position', ctypes.c_void_p),
+                ('rows', ctypes.c_void_p), ('cos', ctypes.c_void_p), ('sin', ctypes.c_void_p)]
+
+
+class KVReadArgs(ctypes.Structure):
+    """Mirror of lb_kv_read_args."""
+    _fields_ = [('struct_size', ctypes.c_uint32), ('reserved', ctypes.c_uint32), ('cache', KVCacheStruct),
+                ('length', ctypes.c_void_p), ('start', ctypes.c_int64), ('count', ctypes.c_int64),
+                ('keys', KVRows), ('values', KVRows)]
+
+
+class KVAttentionArgs(ctypes.Structure):
+    """Mirror of lb_kv_attention_args."""
+    _fields_ = [('struct_size', ctypes.c_uint32), ('reserved', ctypes.c_uint32), ('cache', KVCacheStruct),
+                ('seq', ctypes.c_int64), ('heads', ctypes.c_int64), ('q', KVRows), ('out', KVRows),
+                ('position', ctypes.c_void_p), ('rows', ctypes.c_void_p), ('cos', ctypes.c_void_p),
+                ('sin', ctypes.c_void_p), ('k', KVRows), ('v', KVRows), ('scale', ctypes.c_float),
+                ('reserved2', ctypes.c_uint32), ('limit', ctypes.c_int64), ('workspace', ctypes.c_void_p),
+                ('workspace_bytes', ctypes.c_size_t)]
+
+
 _lib = None
 
 
@@ -234,6 +276,11 @@ def library():
                                     ctypes.c_float, ctypes.c_void_p]
         lib.lb_layer_rows.restype = ctypes.c_int
         lib.lb_layer_rows.argtypes = [ctypes.POINTER(LayerRowsArgs), ctypes.c_void_p]
+        for name, args in (('lb_kv_append', KVAppendArgs), ('lb_kv_read', KVReadArgs), ('lb_kv_attention', KVAttentionArgs)):
+            getattr(lib, name).restype = ctypes.c_int
+            getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
+        lib.lb_kv_attention_workspace_bytes.restype = ctypes.c_int
+        lib.lb_kv_attention_workspace_bytes.argtypes = [ctypes.POINTER(KVAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
         if lib.lb_abi_version() != ABI_VERSION:
             raise RuntimeError(f'liblowbit_hip ABI {lib.lb_abi_version()} != expected {ABI_VERSION}')
         _lib = lib
@@ -995,3 +1042,281 @@ class LayerRows:
         if status != OK:
             _check(status, 'lb_layer_rows')
         return out
+
+
+# ---------------------------------------------------------------- the KV cache in 8 bits
+class QuantizedKVCache:
+    """The buffers of a KV cache in 8 bits (lb_kv_cache, include/lowbit_decode_hip.h): batch sequences of up to
+    `capacity` slots.  Full blocks of 64 slots are held as codes with a scale for their keys and one for their values
+    (per KV head), the open block and the one before it in fp16; the calls below fill and read them.  The program keeps
+    the number of slots that each sequence holds, as a device tensor: it is the `position` of the rows appended next.
+
+    key_codes int8 or float8_e4m3fn [batch, kv_heads, blocks, 64, D] (D 64 or 128), value_codes the same by dim
+    [batch, kv_heads, blocks, D, 64], key_scales and value_scales fp32 [batch, kv_heads, blocks], key_tail fp16
+    [batch, kv_heads, 2, 64, D], value_tail fp16 [batch, kv_heads, 2, D, 64].
+    """
+
+    CODES = {'int8': torch.int8, 'fp8': torch.float8_e4m3fn}
+
+    def __init__(self, key_codes, value_codes, key_scales, value_scales, key_tail, value_tail):
+        formats = {dtype: name for name, dtype in self.CODES.items()}
+        if not isinstance(key_codes, torch.Tensor) or key_codes.dtype not in formats or key_codes.ndim != 5:
+            raise ValueError('key_codes must be int8 or float8_e4m3fn [batch, kv_heads, blocks, 64, head_dim]')
+        batch, heads, blocks, slots, dim = key_codes.shape
+        if slots != KV_BLOCK or dim not in (64, 128) or min(batch, heads, blocks) < 1:
+            raise ValueError('key_codes must be [batch, kv_heads, blocks, 64, head_dim] with head_dim 64 or 128')
+        lead = (batch, heads)
+        for name, t, dtype, shape in (
+                ('key_codes', key_codes, key_codes.dtype, (*lead, blocks, slots, dim)),
+                ('value_codes', value_codes, key_codes.dtype, (*lead, blocks, dim, slots)),
+                ('key_scales', key_scales, torch.float32, (*lead, blocks)),
+                ('value_scales', value_scales, torch.float32, (*lead, blocks)),
+                ('key_tail', key_tail, torch.float16, (*lead, 2, slots, dim)),
+                ('value_tail', value_tail, torch.float16, (*lead, 2, dim, slots))):
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+                raise ValueError(f'{name} must be contiguous {dtype} {list(shape)}')
+            if t.device != key_codes.device:
+                raise ValueError(f'{name} must be on {key_codes.device} with key_codes (found {t.device})')
+        if key_codes.device.type != 'cuda':
+            raise ValueError('key_codes must be a ROCm device tensor')
+        self.key_codes, self.value_codes = key_codes, value_codes
+        self.key_scales, self.value_scales = key_scales, value_scales
+        self.key_tail, self.value_tail = key_tail, value_tail
+        self.format, self.device = formats[key_codes.dtype], key_codes.device
+        self.batch, self.kv_heads, self.head_dim, self.capacity = batch, heads, dim, blocks * slots
+
+    @classmethod
+    def empty(cls, batch, kv_heads, capacity, *, head_dim=64, format='int8', device='cuda'):
+        """A cache of no held slots; the capacity is rounded up to whole blocks."""
+        if format not in cls.CODES:
+            raise ValueError(f'unknown cache format {format!r}')
+        for name, value in (('batch', batch), ('kv_heads', kv_heads), ('capacity', capacity)):
+            if isinstance(value, bool) or not hasattr(value, '__index__') or value < 1:
+                raise ValueError(f'{name} must be a positive integer')
+        if head_dim not in (64, 128):
+            raise ValueError('head_dim must be 64 or 128')
+        lead, blocks = (batch, kv_heads), (capacity + KV_BLOCK - 1) // KV_BLOCK
+        zeros = lambda dtype, *shape: torch.zeros((*lead, *shape), dtype=dtype, device=device)
+        codes = lambda *shape: zeros(torch.int8, *shape).view(cls.CODES[format])
+        return cls(codes(blocks, KV_BLOCK, head_dim), codes(blocks, head_dim, KV_BLOCK), zeros(torch.float32, blocks),
+                   zeros(torch.float32, blocks), zeros(torch.float16, 2, KV_BLOCK, head_dim),
+                   zeros(torch.float16, 2, head_dim, KV_BLOCK))
+
+    def tensors(self):
+        """The six buffers, in the order of the constructor."""
+        return (self.key_codes, self.value_codes, self.key_scales, self.value_scales, self.key_tail, self.value_tail)
+
+    def clone(self):
+        """A copy with buffers of its own."""
+        return type(self)(*(t.clone() for t in self.tensors()))
+
+    def nbytes(self):
+        """Bytes of all buffers."""
+        return sum(t.numel() * t.element_size() for t in self.tensors())
+
+    def _struct(self):
+        return KVCacheStruct(KV_FORMATS[self.format], self.head_dim, self.batch, self.kv_heads, self.capacity,
+                             *(t.data_ptr() for t in self.tensors()))
+
+
+def _kv_cache(cache):
+    if not isinstance(cache, QuantizedKVCache):
+        raise ValueError('cache must be a QuantizedKVCache')
+    return cache
+
+
+def _kv_rows(t, name, cache, heads, seq=None):
+    """A [batch, seq, heads, head_dim] fp16 operand on the cache's device."""
+    if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.ndim != 4 or t.shape[0] != cache.batch
+            or t.shape[1] < 1 or t.shape[3] != cache.head_dim or (heads is not None and t.shape[2] != heads)
+            or (seq is not None and t.shape[1] != seq)):
+        raise ValueError(f'{name} must be fp16 [batch, seq, heads, head_dim] = [{cache.batch}, '
+                         f'{"seq" if seq is None else seq}, {"heads" if heads is None else heads}, {cache.head_dim}]')
+    if t.device != cache.device:
+        raise ValueError(f'{name} must be on {cache.device} with the cache (found {t.device})')
+    return t
+
+
+def _kv_ready(t):
+    """Whether the kernels take these rows where they lie: whole 16-byte pieces at 16-byte addresses."""
+    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0
+            and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()[:3])))
+
+
+def _kv_struct(t):
+    return KVRows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _kv_counts(t, name, cache):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.numel() != cache.batch or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous int64 tensor with one value per sequence ({cache.batch})')
+    if t.device != cache.device:
+        raise ValueError(f'{name} must be on {cache.device} with the cache (found {t.device})')
+    return t.data_ptr()
+
+
+def _kv_tables(cos, sin, cache):
+    if cos is None and sin is None:
+        return None, None
+    for t, name in ((cos, 'cos'), (sin, 'sin')):
+        if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.ndim != 2 or t.shape[1] != cache.head_dim
+                or t.shape[0] < cache.capacity or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f'{name} must be contiguous fp16 [>= capacity, head_dim] = [{cache.capacity}, {cache.head_dim}] '
+                             'at a 16-byte address (cos and sin go together)')
+        if t.device != cache.device:
+            raise ValueError(f'{name} must be on {cache.device} with the cache (found {t.device})')
+    return cos.data_ptr(), sin.data_ptr()
+
+
+def _kv_run(fn, args, device, what, stream=None):
+    """The call on the device's current stream (or `stream`), with that device current: its default stream has no handle
+    of its own."""
+    index = device.index
+    if index is not None and index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            status = fn(args, ctypes.c_void_p(_raw_stream(device) if stream is None else stream))
+    else:
+        status = fn(args, ctypes.c_void_p(_raw_stream(device) if stream is None else stream))
+    if status != OK:
+        _check(status, what)
+
+
+class _PreparedKV(_Prepared):
+    def run(self, stream=None):
+        _kv_run(self._fn, self._ref, self._device, self._what, stream)
+
+
+def _kv_append_args(cache, k, v, position, rows, cos, sin):
+    a = KVAppendArgs()
+    a.struct_size = ctypes.sizeof(KVAppendArgs)
+    a.cache, a.seq, a.k, a.v = _kv_cache(cache)._struct(), k.shape[1], _kv_struct(k), _kv_struct(v)
+    a.position = _kv_counts(position, 'position', cache)
+    a.rows = None if rows is None else _kv_counts(rows, 'rows', cache)
+    a.cos, a.sin = _kv_tables(cos, sin, cache)
+    return a
+
+
+def _kv_pair(cache, k, v, seq=None):
+    _kv_rows(k, 'k', _kv_cache(cache), cache.kv_heads, seq)
+    _kv_rows(v, 'v', cache, cache.kv_heads, k.shape[1])
+
+
+def kv_append(cache, k, v, position, *, rows=None, cos=None, sin=None):
+    """lb_kv_append: the first rows[b] (default: all) rows of k and v [batch, seq, kv_heads, head_dim] go to slots
+    position[b] .. of each sequence; blocks that become full are quantised.  position and rows: int64 [batch] on the
+    device.  With cos and sin (fp16 [>= capacity, head_dim]) the keys are rotated first.  A sequence whose rows would not
+    fit is left alone.  k and v may have any strides (a copy is made where rows are not 16-byte pieces)."""
+    _kv_pair(cache, k, v)
+    k, v = (t if _kv_ready(t) else _aligned(t) for t in (k, v))
+    a = _kv_append_args(cache, k, v, position, rows, cos, sin)
+    _kv_run(library().lb_kv_append, ctypes.byref(a), cache.device, 'lb_kv_append')
+
+
+def kv_read(cache, length, *, start=0, count=None, keys=None, values=None):
+    """lb_kv_read: slots start .. start + count - 1 (default: to the capacity) of every sequence as fp16 keys and values
+    [batch, kv_heads, count, head_dim].  length: int64 [batch] on the device, the slots that are held; rows at or past it
+    are left as they are in `keys` and `values` (zero where they are allocated here)."""
+    _kv_cache(cache)
+    count = cache.capacity - start if count is None else count
+    if not 0 <= start < cache.capacity or not 1 <= count <= cache.capacity - start:
+        raise ValueError(f'slots {start} .. {start + count - 1} are not within the capacity {cache.capacity}')
+    shape = (cache.batch, cache.kv_heads, count, cache.head_dim)
+    outs = []
+    for name, t in (('keys', keys), ('values', values)):
+        if t is None:
+            t = torch.zeros(shape, dtype=torch.float16, device=cache.device)
+        elif (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape or not _kv_ready(t)
+              or t.device != cache.device):
+            raise ValueError(f'{name} must be fp16 {list(shape)} on {cache.device}, its rows in 16-byte pieces')
+        outs.append(t)
+    a = KVReadArgs()
+    a.struct_size = ctypes.sizeof(KVReadArgs)
+    a.cache, a.length = cache._struct(), _kv_counts(length, 'length', cache)
+    a.start, a.count = start, count
+    a.keys, a.values = (KVRows(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1)) for t in outs)
+    _kv_run(library().lb_kv_read, ctypes.byref(a), cache.device, 'lb_kv_read')
+    return tuple(outs)
+
+
+def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit):
+    a = KVAttentionArgs()
+    a.struct_size = ctypes.sizeof(KVAttentionArgs)
+    a.cache, a.seq, a.heads, a.q, a.out = cache._struct(), q.shape[1], q.shape[2], _kv_struct(q), _kv_struct(out)
+    a.position = _kv_counts(position, 'position', cache)
+    a.rows = None if rows is None else _kv_counts(rows, 'rows', cache)
+    a.cos, a.sin = _kv_tables(cos, sin, cache)
+    if k is not None:
+        a.k, a.v = _kv_struct(k), _kv_struct(v)
+    a.scale = cache.head_dim ** -0.5 if scale is None else scale
+    a.limit = 0 if limit is None else limit
+    return a
+
+
+def _kv_check_attention(q, cache, out, k, v):
+    _kv_rows(q, 'q', _kv_cache(cache), None)
+    if q.shape[2] % cache.kv_heads or q.shape[2] < 1:
+        raise ValueError(f'the heads of q ({q.shape[2]}) must be a multiple of the kv_heads ({cache.kv_heads})')
+    if out is not None:
+        _kv_rows(out, 'out', cache, q.shape[2], q.shape[1])
+        if not _kv_ready(out):
+            raise ValueError('the rows of out must be 16-byte pieces')
+    if (k is None) != (v is None):
+        raise ValueError('k and v go together')
+    if k is not None:
+        _kv_pair(cache, k, v, q.shape[1])
+
+
+def kv_attention_workspace_bytes(args):
+    size = ctypes.c_size_t(0)
+    _check(library().lb_kv_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(size)), 'lb_kv_attention_workspace_bytes')
+    return size.value
+
+
+def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, scale=None, cos=None, sin=None, limit=None):
+    """lb_kv_attention: causal grouped-query attention of q [batch, seq, heads, head_dim] over the cache.  Row i of
+    sequence b lies at slot position[b] + i and attends over slots 0 .. position[b] + i, which the cache holds already, or
+    gets here where k and v are given (kv_append's arguments).  rows (default: all): a sequence's query rows; out rows
+    behind them are left as they are (zero where out is allocated here).  scale: default head_dim ** -0.5.  cos and sin
+    rotate q (and k).  limit: about how many slots the longest sequence holds (default: the capacity); it decides only
+    how the work is split.  Any strides of q, k and v (a copy is made where rows are not 16-byte pieces)."""
+    _kv_check_attention(q, cache, out, k, v)
+    q, k, v = (t if t is None or _kv_ready(t) else _aligned(t) for t in (q, k, v))
+    if out is None:
+        out = (torch.empty if rows is None else torch.zeros)(q.shape, dtype=torch.float16, device=q.device)
+    a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit)
+    need = kv_attention_workspace_bytes(a)
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    _kv_run(library().lb_kv_attention, ctypes.byref(a), cache.device, 'lb_kv_attention')
+    return out
+
+
+class PreparedKVAppend(_PreparedKV):
+    """A fixed lb_kv_append call for hot loops: kv_append's arguments over buffers that stay (no copies are made, so k and
+    v need rows of 16-byte pieces).  run() enqueues it on the current stream; positions are read on the device."""
+
+    def __init__(self, cache, k, v, position, *, rows=None, cos=None, sin=None):
+        _kv_pair(cache, k, v)
+        if not _kv_ready(k) or not _kv_ready(v):
+            raise ValueError('the rows of k and v must be 16-byte pieces')
+        a = _kv_append_args(cache, k, v, position, rows, cos, sin)
+        self._bind('lb_kv_append', 'lb_kv_append', a, cache.device, [cache, k, v, position, rows, cos, sin])
+
+
+class PreparedKVAttention(_PreparedKV):
+    """A fixed lb_kv_attention call for hot loops: kv_attention's arguments over buffers that stay (q, out, k and v with
+    rows of 16-byte pieces).  Owns its workspace, so calls of one instance must be ordered (one stream)."""
+
+    def __init__(self, q, cache, position, out, *, rows=None, k=None, v=None, scale=None, cos=None, sin=None, limit=None):
+        _kv_check_attention(q, cache, out, k, v)
+        if out is None or not all(t is None or _kv_ready(t) for t in (q, k, v)):
+            raise ValueError('the rows of q, k, v and out must be 16-byte pieces')
+        a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit)
+        keep = [q, cache, position, out, rows, k, v, cos, sin]
+        need = kv_attention_workspace_bytes(a)
+        if need:
+            keep.append(torch.empty(need, dtype=torch.uint8, device=q.device))
+            a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
+        self._bind('lb_kv_attention', 'lb_kv_attention', a, cache.device, keep)
+        self.out = out
