@@ -388,14 +388,13 @@ typedef struct lb_kv_attention_args {
   lb_kv_rows k, v;             /* data NULL: the rows are in the cache already; else appended first, as lb_kv_append */
   float scale;                 /* score scale, finite and >= 0 (usually 1 / sqrt(head_dim)) */
   uint32_t reserved2;
-  int64_t limit;               /* about how many slots the longest sequence holds, for the split of the work (any value
-                                  gives the same sums in another order); 0: capacity */
-  void *workspace;             /* lb_kv_attention_workspace_bytes, 16-byte aligned, any contents; calls sharing it must
-                                  be ordered (one stream) */
+  void *workspace;             /* lb_kv_attention_workspace_bytes, 256-byte aligned.  Its first LB_ZEROED_WORKSPACE_BYTES
+                                  are zero before its first use, and every call leaves them zero again; for any calls,
+                                  which must be ordered (one stream) */
   size_t workspace_bytes;
 } lb_kv_attention_args;
 
-/* Bytes of workspace lb_kv_attention needs for these arguments (0 when none); host-only. */
+/* Bytes of workspace lb_kv_attention needs for these arguments (0 when none); host-only.  A larger one does too. */
 lb_status lb_kv_attention_workspace_bytes(const lb_kv_attention_args *args, size_t *bytes);
 
 /*

@@ -350,15 +350,14 @@ def test_attention_matches_the_definition(device, format, shape):
     cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)   # NaN wherever nothing is held
     lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device), rows=ints([s + seq for s in starts], device))
     scale = dim ** -0.5
-    for limit in (None, 64, 2 * capacity):
-        got = lb.kv_attention(dev(q, device), cache, ints(starts, device), limit=limit)
-        worst = check_attention(got, q, k, v, starts, [seq] * batch, format, scale, kv_heads)
-        print(f'[kv attention] {format} {shape[:4]} limit {limit}: {worst:.2f} of the bound', flush=True)
+    got = lb.kv_attention(dev(q, device), cache, ints(starts, device))
+    worst = check_attention(got, q, k, v, starts, [seq] * batch, format, scale, kv_heads)
+    print(f'[kv attention] {format} {shape[:4]}: {worst:.2f} of the bound', flush=True)
 
 
 @pytest.mark.parametrize('format,dim', [('int8', 64), ('fp8', 128)])
 def test_attention_long(device, format, dim):
-    """Thousands of slots in many parts, against the same call in one part's order and the oracle."""
+    """Thousands of slots in many parts."""
     announce('kv attention long', format, dim)
     starts, heads, kv_heads, seq = [5000, 0, 2111, 4095], 4, 2, 2
     batch, capacity = len(starts), 5120
@@ -366,10 +365,9 @@ def test_attention_long(device, format, dim):
     q = rows_of(32, batch, seq, heads, dim)
     cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)
     lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device), rows=ints([s + seq for s in starts], device))
-    for limit in (None, 300, 64):
-        got = lb.kv_attention(dev(q, device), cache, ints(starts, device), limit=limit)
-        worst = check_attention(got, q, k, v, starts, [seq] * batch, format, dim ** -0.5, kv_heads)
-        print(f'[kv attention] long {format} limit {limit}: {worst:.2f} of the bound', flush=True)
+    got = lb.kv_attention(dev(q, device), cache, ints(starts, device))
+    worst = check_attention(got, q, k, v, starts, [seq] * batch, format, dim ** -0.5, kv_heads)
+    print(f'[kv attention] long {format}: {worst:.2f} of the bound', flush=True)
 
 
 @pytest.mark.parametrize('seq,heads', [(3, 6), (90, 6), (1, 2)])
@@ -500,7 +498,7 @@ def test_a_run_as_it_is_used(device):
     # a step: the token rows at each sequence's position, the call, position + 1
     qs, ks, vs = (torch.zeros((batch, 1, t.shape[2], dim), dtype=torch.float16, device=device) for t in (qd, kd, vd))
     out = torch.zeros_like(qs)
-    call = lb.PreparedKVAttention(qs, cache, position, out, k=ks, v=vs, limit=capacity)
+    call = lb.PreparedKVAttention(qs, cache, position, out, k=ks, v=vs)
     lane = torch.arange(batch, device=device)
 
     def step():
@@ -524,7 +522,7 @@ def test_a_run_as_it_is_used(device):
     for i in range(steps):
         graph.replay()
         at = start + i
-        eager = lb.kv_attention(qd[lane, at][:, None], twin, at, k=kd[lane, at][:, None], v=vd[lane, at][:, None], limit=capacity)
+        eager = lb.kv_attention(qd[lane, at][:, None], twin, at, k=kd[lane, at][:, None], v=vd[lane, at][:, None])
         torch.cuda.synchronize()
         assert torch.equal(out, eager), i
         now = [p + i for p in prompt]
@@ -587,9 +585,10 @@ def test_caches_past_32_bit_offsets(device):
     lb.kv_append(cache, many(k), many(v), ints([0] * batch, device), rows=ints([0, 0, n], device))
     lb.kv_append(alone, k, v, ints([0], device))
     at = ints([0, 0, n - 1], device)
-    got = lb.kv_attention(many(q[:, -1:]), cache, at, rows=ints([0, 0, 1], device), limit=256)
-    want = lb.kv_attention(q[:, -1:], alone, at[2:], limit=256)
-    assert torch.equal(got[2:], want)
+    got = lb.kv_attention(many(q[:, -1:]), cache, at, rows=ints([0, 0, 1], device))
+    want = lb.kv_attention(q[:, -1:], alone, at[2:])
+    check_attention(got[2:], *(t.cpu().numpy() for t in (q[:, -1:], k, v)), [n - 1], [1], 'fp8', dim ** -0.5, kv_heads)
+    check_attention(want, *(t.cpu().numpy() for t in (q[:, -1:], k, v)), [n - 1], [1], 'fp8', dim ** -0.5, kv_heads)
     # far slots of the last sequence: its last block
     far = capacity - 64
     lb.kv_append(cache, many(k[:, :64]), many(v[:, :64]), ints([far] * batch, device), rows=ints([0, 0, 64], device))
@@ -597,3 +596,52 @@ def test_caches_past_32_bit_offsets(device):
     for t, rows in ((a, k), (b, v)):
         for h in (0, kv_heads - 1):
             same(t[2, h].cpu().numpy(), ko.read(rows[0, :64, h].cpu().numpy(), 'fp8'))
+
+
+@pytest.mark.parametrize('format', ['int8', 'fp8'])
+@pytest.mark.parametrize('dim,seq', [(64, 1), (64, 60), (128, 45)])
+def test_attention_over_blocks_of_very_different_scales(device, format, dim, seq):
+    """Values from block to block 1e-6 to 2e3 in size, blocks of zeros first and in between, keys of zeros."""
+    announce('kv attention scales', format, dim, seq)
+    heads, kv_heads, capacity, total = 4, 1, 1024, 1000
+    sizes = [0, 1e-6, 1, 1e-3, 0, 6e2, 50, 1e-5, 2, 9, 0.3, 2e3, 1, 1e-6, 7, 1]
+    k, v = rows_of(100, 3, total, kv_heads, dim), rows_of(101, 3, total, kv_heads, dim).astype(np.float64)
+    for i, size in enumerate(sizes):
+        v[:, 64 * i:64 * i + 64] *= size
+    v[1] = np.abs(v[1, ::-1])
+    k[2, 128:320] = 0
+    v = v.astype(np.float16)
+    assert np.isfinite(v).all()
+    starts = [total - seq, 500, 290]
+    q = rows_of(102, 3, seq, heads, dim)
+    cache = fresh(device, 3, kv_heads, capacity, dim, format, fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * 3, device), rows=ints([s + seq for s in starts], device))
+    got = lb.kv_attention(dev(q, device), cache, ints(starts, device))
+    worst = check_attention(got, q, k, v, starts, [seq] * 3, format, dim ** -0.5, kv_heads)
+    print(f'[kv attention] scales {format} {dim} {seq}: {worst:.2f} of the bound', flush=True)
+
+
+def test_attention_of_many_sequences(device):
+    """More sequences than a workgroup has threads: short ones, some of no rows, some outside the capacity, then long."""
+    announce('kv attention many')
+    batch, heads, kv_heads, dim, capacity = 700, 2, 1, 64, 192
+    rng = np.random.default_rng(110)
+    starts = [int(x) for x in rng.integers(0, capacity, batch)]
+    rows = [int(x) for x in rng.integers(0, 3, batch) > 0]
+    starts[5], starts[300], starts[699], rows[699] = -1, capacity, capacity - 1, 1
+    rows[300] = 1
+    good = [0 <= s and s + r <= capacity for s, r in zip(starts, rows)]
+    k, v = rows_of(111, batch, capacity, kv_heads, dim), rows_of(112, batch, capacity, kv_heads, dim)
+    q = rows_of(113, batch, 1, heads, dim)
+    cache = fresh(device, batch, kv_heads, capacity, dim, 'int8', fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device),
+                 rows=ints([s + r if g else 0 for s, r, g in zip(starts, rows, good)], device))
+    out = torch.full((batch, 1, heads, dim), 3.0, dtype=torch.float16, device=device)
+    lb.kv_attention(dev(q, device), cache, ints(starts, device), rows=ints(rows, device), out=out)
+    for b in range(batch):
+        if not good[b]:
+            assert bool(out[b].isnan().all()), b
+        elif rows[b] == 0:
+            assert bool((out[b] == 3).all()), b
+        else:
+            check_attention(out[b:b + 1], q[b:b + 1], k[b:b + 1], v[b:b + 1], [starts[b]], [1], 'int8', dim ** -0.5, kv_heads)

@@ -49,10 +49,12 @@ def attention(**over):
     a = lb.KVAttentionArgs()
     a.struct_size, a.cache, a.seq, a.heads, a.scale = ctypes.sizeof(a), cache(), 5, 9, 0.125
     a.q, a.out = lb.KVRows(0xA00000, 5 * 576, 576, 64), lb.KVRows(0xB00000, 5 * 576, 576, 64)
-    a.position = 0x700000
+    a.position, a.workspace, a.workspace_bytes = 0x700000, 0xC00000, 4 << 20
     return fill(a, over)
 
 
+FAR = dict(cache__capacity=1 << 20, cache__key_codes=1 << 32, cache__value_codes=2 << 32, cache__key_scales=3 << 32,
+           cache__value_scales=4 << 32, cache__key_tail=5 << 32, cache__value_tail=6 << 32)   # a long cache: needs a workspace
 BAD_CACHE = [
     (dict(cache__format=2), 'format', lb.INVALID_ARGUMENT),
     (dict(cache__head_dim=96), 'head_dim', lb.UNSUPPORTED),
@@ -97,19 +99,22 @@ BAD_ATTENTION = [
     (dict(heads=10), 'kv_heads', lb.INVALID_ARGUMENT),
     (dict(heads=0), 'heads', lb.INVALID_ARGUMENT),
     (dict(seq=2 ** 27), '2^28 rows', lb.INVALID_ARGUMENT),
+    (dict(cache__batch=65535, cache__kv_heads=300, heads=300), 'overlaps', lb.INVALID_ARGUMENT),
     (dict(scale=float('nan')), 'scale', lb.INVALID_ARGUMENT),
     (dict(scale=float('inf')), 'scale', lb.INVALID_ARGUMENT),
     (dict(scale=-1.0), 'scale', lb.INVALID_ARGUMENT),
-    (dict(limit=-1), 'limit', lb.INVALID_ARGUMENT),
     (dict(q__data=0xA00004), 'q must', lb.INVALID_ARGUMENT),
     (dict(out__head_stride=0), 'rows of out overlap', lb.INVALID_ARGUMENT),
     (dict(out__data=0xA00040), 'out overlaps q', lb.INVALID_ARGUMENT),
     (dict(out__data=0x200000), 'out overlaps value_codes', lb.INVALID_ARGUMENT),
+    (dict(FAR, workspace=0xC00080), 'workspace', lb.INVALID_ARGUMENT),
+    (dict(FAR, workspace_bytes=50000), 'workspace', lb.INVALID_ARGUMENT),
+    (dict(FAR, workspace=0xB00000), 'out overlaps workspace', lb.INVALID_ARGUMENT),
+    (dict(FAR, workspace=0xA00000), 'workspace overlaps q', lb.INVALID_ARGUMENT),
     (dict(sin=0x780000), 'cos and sin', lb.INVALID_ARGUMENT),
     (dict(k__data=0x600000), 'v must', lb.INVALID_ARGUMENT),
     (dict(v__data=0x600000), 'k must', lb.INVALID_ARGUMENT),
-    (dict(cache__capacity=1 << 20, cache__key_codes=1 << 32, cache__value_codes=2 << 32, cache__key_scales=3 << 32,
-          cache__value_scales=4 << 32, cache__key_tail=5 << 32, cache__value_tail=6 << 32), 'workspace', lb.INVALID_ARGUMENT),
+    (dict(FAR, workspace=0), 'workspace', lb.INVALID_ARGUMENT),
 ]
 
 
@@ -136,15 +141,11 @@ def test_null_args_and_workspace_query():
     assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.OK and size.value == 0
     a = attention(heads=10)
     assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.INVALID_ARGUMENT
-    # a long cache is taken in parts: sums and statistics of each, whatever the split
-    a = attention(seq=1, cache__capacity=1 << 20, cache__value_codes=1 << 40)
-    assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.INVALID_ARGUMENT  # (overlaps: sizes only differ)
-    a = attention(seq=1, cache__capacity=1 << 20, cache__key_codes=1 << 32, cache__value_codes=2 << 32, cache__key_scales=3 << 32,
-                  cache__value_scales=4 << 32, cache__key_tail=5 << 32, cache__value_tail=6 << 32)
+    a = attention(seq=1, **FAR)     # a long cache: parts with 16 rows of 64 sums and two statistics, behind the zeroed bytes
     assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.OK
-    assert size.value > 0 and size.value % (16 * 66 * 4) == 0
-    a.limit = 64
-    assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.OK and size.value == 0
+    assert size.value == 4096 + 514 * 16 * 66 * 4
+    a = attention(seq=11, cache__capacity=64, cache__batch=200, **{k: v for k, v in FAR.items() if k != 'cache__capacity'})
+    assert lib.lb_kv_attention_workspace_bytes(ctypes.byref(a), ctypes.byref(size)) == lb.OK and size.value == 0   # 600 tiles
 
 
 def test_failed_state_refuses_the_cache_entries():
@@ -253,7 +254,7 @@ def test_struct_sizes_match_the_library():
     assert ctypes.sizeof(lb.KVRows) == 32
     assert ctypes.sizeof(lb.KVAppendArgs) == 8 + 80 + 8 + 64 + 32
     assert ctypes.sizeof(lb.KVReadArgs) == 8 + 80 + 24 + 64
-    assert ctypes.sizeof(lb.KVAttentionArgs) == 8 + 80 + 16 + 64 + 32 + 64 + 8 + 24
+    assert ctypes.sizeof(lb.KVAttentionArgs) == 8 + 80 + 16 + 64 + 32 + 64 + 8 + 16
 
 
 def test_oracle_e4m3_is_the_format():

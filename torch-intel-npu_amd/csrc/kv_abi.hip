@@ -3,7 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <initializer_list>
+#include <type_traits>
 
 #include "../../include/lowbit_decode_hip.h"
 #include "abi_util.h"
@@ -156,28 +156,40 @@ void launch_append(const lb_kv_cache &c, int64_t seq, const lb_kv_rows &k, const
   });
 }
 
-// Tiles of query rows, and the parts that the slots are taken in.
+// Which kernel, its grid and its workspace: LB_ZEROED_WORKSPACE_BYTES of tickets, then the sums of parts.
 struct AttendPlan {
-  int qt, tiles, splits, chunk;
-  size_t sums, bytes;   // floats of the partial sums, bytes of workspace
+  bool prompt;
+  int qt, tiles, splits;
+  int64_t grid;
+  size_t bytes;
 };
+static_assert(kKvTickets * 4 == LB_ZEROED_WORKSPACE_BYTES, "tickets are the workspace's zeroed bytes");
+
+constexpr int kCus = 256;
 
 AttendPlan attend_plan(const lb_kv_attention_args *a) {
   AttendPlan plan{};
   const lb_kv_cache &c = a->cache;
-  const int64_t rows = a->seq * (a->heads / c.kv_heads);
+  const int64_t rows = a->seq * (a->heads / c.kv_heads), pairs = c.batch * c.kv_heads;
+  plan.prompt = rows > 32;
   plan.qt = rows > 16 ? 2 : 1;
-  plan.tiles = (int)((rows + 16 * plan.qt - 1) / (16 * plan.qt));
-  const int64_t units = c.batch * c.kv_heads * plan.tiles;
-  const int64_t held = a->limit > 0 ? std::min(a->limit, c.capacity) : c.capacity, blocks = (held + kKvBlock - 1) / kKvBlock;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(1024 / units, blocks / 4));
-  plan.chunk = (int)((blocks + want - 1) / want + 3) / 4 * 4;
-  plan.splits = (int)((blocks + plan.chunk - 1) / plan.chunk);
-  if (plan.splits > 1) {
-    const size_t parts = (size_t)units * plan.splits * 16 * plan.qt;
-    plan.sums = parts * c.head_dim;
-    plan.bytes = (plan.sums + parts * 2) * sizeof(float);
+  plan.tiles = plan.splits = 1;
+  size_t parts, height = 16 * plan.qt;   // parts of `height` rows that are left in the workspace at the most
+  if (plan.prompt) {
+    height = 128;
+    plan.tiles = (int)((rows + 127) / 128);
+    // Parts only where there are not tiles enough for two workgroups on each CU, of eight blocks at the least.
+    const int64_t units = pairs * plan.tiles;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kCus / units, (c.capacity / kKvBlock + 7) / 8));
+    plan.grid = units * plan.splits;     // (at most 2 * kCus where there are parts: the tickets are enough)
+    parts = plan.splits > 1 ? (size_t)plan.grid : 0;
+  } else {
+    // A workgroup per sequence and KV head, and where they can be long enough as many again as they can be split into.
+    const bool split = c.capacity / kKvBlock > kKvLeast;
+    plan.grid = pairs + (split ? (kKvSplit + c.kv_heads - 1) / c.kv_heads * c.kv_heads : 0);
+    parts = split ? kKvPlaces : 0;
   }
+  plan.bytes = parts ? LB_ZEROED_WORKSPACE_BYTES + parts * height * (c.head_dim + 2) * sizeof(float) : 0;
   return plan;
 }
 
@@ -186,10 +198,9 @@ lb_status check_shape(const char *what, const lb_kv_attention_args *a) {
   if (a->seq < 1 || a->seq > kMaxRows || a->heads < 1 || a->heads > 65535 || a->heads % c.kv_heads != 0 ||
       a->seq * (a->heads / c.kv_heads) > kMaxRows)
     return fail(LB_INVALID_ARGUMENT, "%s: heads a multiple of kv_heads up to 65535, and 1 to 2^28 rows of a KV head required", what);
-  if (c.kv_heads * ((a->seq * (a->heads / c.kv_heads) + 15) / 16) > INT32_MAX / 1024)
-    return fail(LB_UNSUPPORTED, "%s: too many rows for one launch", what);
+  if (c.batch * c.kv_heads > (1 << 24) || c.batch * c.kv_heads * ((a->seq * (a->heads / c.kv_heads) + 127) / 128) > (1 << 24))
+    return fail(LB_UNSUPPORTED, "%s: more than 2^24 tiles of 128 rows of a sequence and KV head", what);
   if (!(a->scale >= 0.0f) || !std::isfinite(a->scale)) return fail(LB_INVALID_ARGUMENT, "%s: scale must be finite and >= 0", what);
-  if (a->limit < 0) return fail(LB_INVALID_ARGUMENT, "%s: limit must be >= 0", what);
   return LB_OK;
 }
 
@@ -270,8 +281,8 @@ lb_status lb_kv_attention(const lb_kv_attention_args *a, void *stream) {
   if (const lb_status st = check_counts(what, "rows", a->rows, c.batch, false, counts[1]); st != LB_OK) return st;
   if (const lb_status st = check_tables(what, a->cos, a->sin, c, tables); st != LB_OK) return st;
   const AttendPlan plan = attend_plan(a);
-  if (plan.bytes && (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < plan.bytes))
-    return fail(LB_INVALID_ARGUMENT, "%s: a 16-byte aligned workspace of %zu bytes required (got %zu)", what, plan.bytes, a->workspace_bytes);
+  if (plan.bytes && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < plan.bytes))
+    return fail(LB_INVALID_ARGUMENT, "%s: a 256-byte aligned workspace of %zu bytes required (got %zu)", what, plan.bytes, a->workspace_bytes);
   const Range writes[] = {out, plan.bytes ? range_of(a->workspace, plan.bytes, "workspace") : Range{}};
   const Range reads[] = {q, counts[0], counts[1], tables[0], tables[1], appends ? ins[0] : Range{}, appends ? ins[1] : Range{}};
   if (const lb_status st = check_apart(what, writes, 2, reads, 7); st != LB_OK) return st;
@@ -281,31 +292,33 @@ lb_status lb_kv_attention(const lb_kv_attention_args *a, void *stream) {
   if (overlaps(writes[0], writes[1])) return fail(LB_INVALID_ARGUMENT, "%s: out overlaps workspace", what);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (appends) launch_append(c, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, s);
+  const bool fused = appends && a->seq == 1 && !plan.prompt;   // one row a sequence: appended by the attention's launch
+  if (appends && !fused) launch_append(c, a->seq, a->k, a->v, a->position, a->rows, a->cos, a->sin, s);
   KvAttendParams p{};
   p.c = cache_params(c);
   p.q = rows_params(a->q);
   p.out = rows_params(a->out);
+  if (fused) {
+    p.k = rows_params(a->k);
+    p.v = rows_params(a->v);
+  }
   p.position = a->position;
   p.rows = a->rows;
   p.cos = static_cast<const f16 *>(a->cos);
   p.sin = static_cast<const f16 *>(a->sin);
-  p.partial = static_cast<float *>(a->workspace);
+  p.tickets = static_cast<uint32_t *>(a->workspace);
+  p.partial = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + LB_ZEROED_WORKSPACE_BYTES);
+  p.batch = (int)c.batch;
   p.seq = (int)a->seq;
-  p.heads = (int)a->heads;
   p.group = (int)(a->heads / c.kv_heads);
   p.tiles = plan.tiles;
   p.splits = plan.splits;
-  p.chunk = plan.chunk;
   p.scale = a->scale * 1.44269504088896340736f;
-  const int64_t units = c.kv_heads * plan.tiles;
+  const dim3 grid((unsigned)plan.grid);
   with_kind(c, [&](auto fmt, auto dim) {
-    auto run = [&](auto qt) {
-      hipLaunchKernelGGL((kv_attend_kernel<fmt(), dim(), qt()>), dim3((unsigned)(units * plan.splits), (unsigned)c.batch), dim3(256), 0, s, p);
-      if (plan.splits > 1)
-        hipLaunchKernelGGL((kv_join_kernel<dim(), qt()>), dim3((unsigned)(units * 16 * qt() / 4), (unsigned)c.batch), dim3(256), 0, s, p, plan.sums);
-    };
-    plan.qt == 1 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{});
+    if (plan.prompt) hipLaunchKernelGGL((kv_prompt_kernel<fmt(), dim()>), grid, dim3(256), 0, s, p);
+    else if (plan.qt == 1) hipLaunchKernelGGL((kv_attend_kernel<fmt(), dim(), 1>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((kv_attend_kernel<fmt(), dim(), 2>), grid, dim3(256), 0, s, p);
   });
   return launch_status(what);
 }

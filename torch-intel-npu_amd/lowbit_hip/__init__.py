@@ -214,7 +214,7 @@ class KVAttentionArgs(ctypes.Structure):
                 ('seq', ctypes.c_int64), ('heads', ctypes.c_int64), ('q', KVRows), ('out', KVRows),
                 ('position', ctypes.c_void_p), ('rows', ctypes.c_void_p), ('cos', ctypes.c_void_p),
                 ('sin', ctypes.c_void_p), ('k', KVRows), ('v', KVRows), ('scale', ctypes.c_float),
-                ('reserved2', ctypes.c_uint32), ('limit', ctypes.c_int64), ('workspace', ctypes.c_void_p),
+                ('reserved2', ctypes.c_uint32), ('workspace', ctypes.c_void_p),
                 ('workspace_bytes', ctypes.c_size_t)]
 
 
@@ -1238,7 +1238,7 @@ def kv_read(cache, length, *, start=0, count=None, keys=None, values=None):
     return tuple(outs)
 
 
-def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit):
+def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin):
     a = KVAttentionArgs()
     a.struct_size = ctypes.sizeof(KVAttentionArgs)
     a.cache, a.seq, a.heads, a.q, a.out = cache._struct(), q.shape[1], q.shape[2], _kv_struct(q), _kv_struct(out)
@@ -1248,7 +1248,6 @@ def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, lim
     if k is not None:
         a.k, a.v = _kv_struct(k), _kv_struct(v)
     a.scale = cache.head_dim ** -0.5 if scale is None else scale
-    a.limit = 0 if limit is None else limit
     return a
 
 
@@ -1272,22 +1271,35 @@ def kv_attention_workspace_bytes(args):
     return size.value
 
 
-def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, scale=None, cos=None, sin=None, limit=None):
+_kv_workspaces = {}   # by device and stream: calls on a stream are ordered, so they can share one
+
+
+def _kv_workspace(need, device):
+    """A workspace of lb_kv_attention for a call on the device's current stream: zero once, its counters zero after every
+    call.  A call that is captured gets one of its own (cleared in the graph): replays may run on any stream."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(need, dtype=torch.uint8, device=device)
+    key = (device, _raw_stream(device))
+    held = _kv_workspaces.get(key)
+    if held is None or held.numel() < need:
+        held = _kv_workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+    return held
+
+
+def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, scale=None, cos=None, sin=None):
     """lb_kv_attention: causal grouped-query attention of q [batch, seq, heads, head_dim] over the cache.  Row i of
     sequence b lies at slot position[b] + i and attends over slots 0 .. position[b] + i, which the cache holds already, or
     gets here where k and v are given (kv_append's arguments).  rows (default: all): a sequence's query rows; out rows
     behind them are left as they are (zero where out is allocated here).  scale: default head_dim ** -0.5.  cos and sin
-    rotate q (and k).  limit: about how many slots the longest sequence holds (default: the capacity); it decides only
-    how the work is split.  Any strides of q, k and v (a copy is made where rows are not 16-byte pieces)."""
+    rotate q (and k).  Any strides of q, k and v (a copy is made where rows are not 16-byte pieces)."""
     _kv_check_attention(q, cache, out, k, v)
     q, k, v = (t if t is None or _kv_ready(t) else _aligned(t) for t in (q, k, v))
     if out is None:
         out = (torch.empty if rows is None else torch.zeros)(q.shape, dtype=torch.float16, device=q.device)
-    a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit)
+    a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin)
     need = kv_attention_workspace_bytes(a)
     if need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+        a.workspace, a.workspace_bytes = _kv_workspace(need, cache.device).data_ptr(), need
     _kv_run(library().lb_kv_attention, ctypes.byref(a), cache.device, 'lb_kv_attention')
     return out
 
@@ -1308,15 +1320,15 @@ class PreparedKVAttention(_PreparedKV):
     """A fixed lb_kv_attention call for hot loops: kv_attention's arguments over buffers that stay (q, out, k and v with
     rows of 16-byte pieces).  Owns its workspace, so calls of one instance must be ordered (one stream)."""
 
-    def __init__(self, q, cache, position, out, *, rows=None, k=None, v=None, scale=None, cos=None, sin=None, limit=None):
+    def __init__(self, q, cache, position, out, *, rows=None, k=None, v=None, scale=None, cos=None, sin=None):
         _kv_check_attention(q, cache, out, k, v)
         if out is None or not all(t is None or _kv_ready(t) for t in (q, k, v)):
             raise ValueError('the rows of q, k, v and out must be 16-byte pieces')
-        a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, limit)
+        a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin)
         keep = [q, cache, position, out, rows, k, v, cos, sin]
         need = kv_attention_workspace_bytes(a)
         if need:
-            keep.append(torch.empty(need, dtype=torch.uint8, device=q.device))
+            keep.append(torch.zeros(need, dtype=torch.uint8, device=q.device))
             a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
         self._bind('lb_kv_attention', 'lb_kv_attention', a, cache.device, keep)
         self.out = out
