@@ -210,6 +210,7 @@ class HostCache(lb.QuantizedKVCache):
             setattr(self, name, t)
         self.format, self.device = 'int8', torch.device('cpu')
         self.batch, self.kv_heads, self.head_dim, self.capacity = 2, 3, 64, 128
+        self._bound()
 
 
 def half(*shape, **options):
@@ -233,19 +234,32 @@ AT = torch.zeros(2, dtype=torch.int64)
     (lambda c: lb.kv_read(c, AT, start=128), 'capacity'),
     (lambda c: lb.kv_read(c, AT, start=100, count=29), 'capacity'),
     (lambda c: lb.kv_read(c, AT, count=5, keys=half(2, 3, 6, 64)), 'keys must be'),
-    (lambda c: lb.kv_read(c, AT, count=5, values=half(2, 3, 64, 5).transpose(2, 3)), 'values must be'),
+    (lambda c: lb.kv_read(c, AT, count=5, values=half(2, 3, 64, 5).transpose(2, 3)), '16-byte'),
     (lambda c: lb.kv_attention(half(2, 1, 4, 64), c, AT), 'multiple of the kv_heads'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 32), c, AT), 'q must be'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, k=half(2, 1, 3, 64)), 'go together'),
+    (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=1e300), 'scale'),
+    (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=float('nan')), 'scale'),
+    (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=-0.1), 'scale'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, k=half(2, 2, 3, 64), v=half(2, 2, 3, 64)), 'k must be'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, out=half(2, 1, 64, 9).transpose(2, 3)), '16-byte'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, out=half(2, 2, 9, 64)), 'out must be'),
     (lambda c: lb.PreparedKVAppend(c, half(2, 1, 64, 3).transpose(2, 3), half(2, 1, 3, 64), AT), '16-byte'),
-    (lambda c: lb.PreparedKVAttention(half(2, 1, 9, 64), c, AT, None), '16-byte'),
+    (lambda c: lb.PreparedKVAttention(half(2, 1, 9, 64), c, AT, None), 'out must be'),
 ])
 def test_wrappers_refuse(call, needle):
     with pytest.raises(ValueError, match=needle):
         call(HostCache())
+
+
+def test_packed_structs_match_their_mirrors():
+    for packed, mirror in ((lb._KV_APPEND, lb.KVAppendArgs), (lb._KV_READ, lb.KVReadArgs), (lb._KV_ATTENTION, lb.KVAttentionArgs)):
+        assert lb._KV_HEAD.size + ctypes.sizeof(lb.KVCacheStruct) + packed.size == ctypes.sizeof(mirror)
+    c = HostCache()
+    a, need = lb._kv_attention_args(half(2, 1, 9, 64), c, AT, half(2, 1, 9, 64), None, None, None, 0.5, None, None, [], True)
+    assert (a.struct_size, a.seq, a.heads, a.scale) == (ctypes.sizeof(a), 1, 9, 0.5)
+    assert a.cache.capacity == 128 and a.cache.value_tail == c.value_tail.data_ptr() and a.q.head_stride == 64
+    assert a.position == AT.data_ptr() and not a.rows and not a.k.data and need == 0
 
 
 def test_struct_sizes_match_the_library():

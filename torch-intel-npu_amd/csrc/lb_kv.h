@@ -967,30 +967,21 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
   const uint8_t *const kc = p.c.kc + bh * p.c.capacity * D, *const vc = p.c.vc + bh * p.c.capacity * D;
   const float *const ks = p.c.ks + bh * p.c.blocks, *const vs = p.c.vs + bh * p.c.blocks;
 
-  // A block on its way: 16-byte pieces of its codes, or of its fp16 rows (twice as many).
-  u4 raw[4 * RAW];
+  // A block of codes on its way, in 16-byte pieces.
+  u4 raw[2 * RAW];
   auto fetch = [&](int block) {
-    if (block >= stop) return;
-    if (block < closed) {
-      const size_t at = (size_t)block * (kKvBlock * D);
+    if (block >= stop || block >= closed) return;
+    const size_t at = (size_t)block * (kKvBlock * D);
 #pragma unroll
-      for (int u = 0; u < RAW; ++u) {
-        raw[u] = *reinterpret_cast<const u4 *>(kc + at + 16 * (tid + 256 * u));
-        raw[RAW + u] = *reinterpret_cast<const u4 *>(vc + at + 16 * (tid + 256 * u));
-      }
-    } else {
-      const size_t half = (2 * bh + (block & 1)) * (kKvBlock * D);
-#pragma unroll
-      for (int u = 0; u < 2 * RAW; ++u) {
-        raw[u] = *reinterpret_cast<const u4 *>(p.c.kt + half + 8 * (tid + 256 * u));
-        raw[2 * RAW + u] = *reinterpret_cast<const u4 *>(p.c.vt + half + 8 * (tid + 256 * u));
-      }
+    for (int u = 0; u < RAW; ++u) {
+      raw[u] = *reinterpret_cast<const u4 *>(kc + at + 16 * (tid + 256 * u));
+      raw[RAW + u] = *reinterpret_cast<const u4 *>(vc + at + 16 * (tid + 256 * u));
     }
   };
   // Keys: rows of D, 8 dims a piece.  Values: rows of 64 slots by dim, piece 2 s + f holding what lane half f takes in K
   // step s: slots 16 s + 4 f .. + 3 and 16 s + 8 + 4 f .. + 3.
-  auto key_at = [&](int slot, int piece) { return slot * (2 * D) + (piece ^ (D == 64 ? slot >> 1 & 7 : slot & 15)) * 16; };
-  auto value_at = [&](int dim, int piece) { return KBYTES + dim * (2 * kKvBlock) + (piece ^ (dim >> 1 & 7)) * 16; };
+  auto key_at = [&](int slot, int piece) { return slot * (2 * D) + (piece ^ (slot & (D == 64 ? 7 : 15))) * 16; };
+  auto value_at = [&](int dim, int piece) { return KBYTES + dim * (2 * kKvBlock) + (piece ^ (dim & 7)) * 16; };
   auto stage = [&](int block) {
     if (block >= stop) return;
     uint8_t *const to = mem + (block & 1) * BYTES;
@@ -1009,15 +1000,16 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
           *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + 2 + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
         }
       }
-    } else {                              // (values as in kv_attend_kernel: finite, whatever lies there)
+    } else {                              // fp16 rows (values as in kv_attend_kernel: finite, whatever lies there)
+      const size_t half = (2 * bh + (block & 1)) * (kKvBlock * D);
       const f16 most = (f16)65504.0f;
       const h8 hi = {most, most, most, most, most, most, most, most};
 #pragma unroll
       for (int u = 0; u < 2 * RAW; ++u) {
         const int at = tid + 256 * u;
-        *reinterpret_cast<h8 *>(to + key_at(at / (D / 8), at % (D / 8))) = kv_order8<FMT>(__builtin_bit_cast(h8, raw[u]));
+        *reinterpret_cast<h8 *>(to + key_at(at / (D / 8), at % (D / 8))) = kv_order8<FMT>(*reinterpret_cast<const h8 *>(p.c.kt + half + 8 * at));
         const int dim = at / 8, f = at / 2 % 4, e = at % 2;
-        const h8 x = __builtin_bit_cast(h8, raw[2 * RAW + u]);
+        const h8 x = *reinterpret_cast<const h8 *>(p.c.vt + half + 8 * at);
         const h8 v = kv_order8<FMT>(__builtin_elementwise_min(__builtin_elementwise_max(x, -hi), hi));
         *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
         *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + 2 + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
@@ -1059,18 +1051,25 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
       const uint8_t *const from = mem + (block & 1) * BYTES;
       const bool open = block >= closed;
       const float kscale = open ? p.scale : p.scale * ks[block], vscale = open ? 1.0f : vs[block];
+      // Eight operands of each product are read ahead: a read is 100 cycles and more from its use, a product 32.
       f16x s[2];
 #pragma unroll
-      for (int a = 0; a < 2; ++a) {
+      for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[a][e] = 0.0f;
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int a = 0; a < 2; ++a)
           s[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + key_at(32 * a + j, 2 * k + g)), q[k], s[a], 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
+      __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
       float shift = 0.0f, part = 1.0f;    // log2 of vs / unit, which the probabilities carry, and unit / vs
       if (vscale > 0.0f) {                // (a block of zeros adds nothing in any unit)
-        const float ratio = unit > 0.0f ? vscale / unit : 0.0f;
+        const float ratio = unit > 0.0f ? vscale * __builtin_amdgcn_rcpf(unit) : 0.0f;
         if (ratio > 4.0f || ratio < 0.25f) {
           if (unit > 0.0f) {
             const float turn = unit / vscale;
@@ -1080,14 +1079,13 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
           unit = vscale;
         } else {
           shift = __builtin_amdgcn_logf(ratio);
-          part = unit / vscale;
+          part = unit * __builtin_amdgcn_rcpf(vscale);   // (to 2^-23, as the logarithm)
         }
       } else if (!(vscale == 0.0f) && base <= pos) {
         shift = part = vscale;            // NaN, for the rows that see some of the block
       }
-      float most = -INFINITY;
-      const bool whole = base + kKvBlock - 1 <= low;
-      if (whole) {
+      float most = -INFINITY, factor = kscale;
+      if (base + kKvBlock - 1 <= low) {
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -1102,6 +1100,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
             s[a][e] = slot <= pos ? s[a][e] * kscale : -INFINITY;
             most = fmaxf(most, s[a][e]);
           }
+        factor = 1.0f;
       }
       if (__any(most > top + kKvSlack)) {
         const float raised = fmaxf(top, fmaxf(most, __shfl_xor(most, 32)));
@@ -1112,27 +1111,30 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
         for (int d = 0; d < DT; ++d) acc[d] *= shrink;
       }
       const float bias = kKvLift - 1.0f + shift - top;   // (at most 2^15 with the ratio's 2^2)
-      h8 pf[4];
       float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         h8 x;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float t = s[k / 2][8 * (k % 2) + e];
-          x[e] = (f16)__builtin_amdgcn_exp2f(whole ? __builtin_fmaf(t, kscale, bias) : t + bias);
-        }
+        for (int e = 0; e < 8; ++e) x[e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[k / 2][8 * (k % 2) + e], factor, bias));
         const h2 one = {(f16)1.0f, (f16)1.0f};
 #pragma unroll
         for (int e = 0; e < 8; e += 2) sum = __builtin_amdgcn_fdot2(h2{x[e], x[e + 1]}, one, sum, false);
-        pf[k] = kv_order8<FMT>(x);
+        const h8 pf = kv_order8<FMT>(x);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + value_at(32 * d + j, 2 * k + g)), pf, acc[d], 0, 0, 0);
       }
       total = __builtin_fmaf(sum, part, total);
+      // The next step's exponentials stand between a step's products.
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * DT, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 24, 0);
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + value_at(32 * d + j, 2 * k + g)), pf[k], acc[d], 0, 0, 0);
+      for (int i = 0; i < 4 * DT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i < 3 * DT) __builtin_amdgcn_sched_group_barrier(0x002, 24 / DT, 0);
+        if (i < 2 * DT) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
     __syncthreads();
   }

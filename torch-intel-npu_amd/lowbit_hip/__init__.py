@@ -9,7 +9,9 @@ torch_intel_npu.py:516-521): contract violations raise ValueError before any
 launch, native failures raise RuntimeError carrying lb_last_error().
 """
 import ctypes
+import operator
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -1084,6 +1086,23 @@ class QuantizedKVCache:
         self.key_tail, self.value_tail = key_tail, value_tail
         self.format, self.device = formats[key_codes.dtype], key_codes.device
         self.batch, self.kv_heads, self.head_dim, self.capacity = batch, heads, dim, blocks * slots
+        self._bound()
+
+    def _bound(self):
+        """What every call's argument struct begins with, and the workspaces that attention calls need by their rows."""
+        cache = KVCacheStruct(KV_FORMATS[self.format], self.head_dim, self.batch, self.kv_heads, self.capacity,
+                              *(t.data_ptr() for t in self.tensors()))
+        self._heads = {args: _KV_HEAD.pack(ctypes.sizeof(args), 0) + bytes(cache) for args in (KVAppendArgs, KVReadArgs, KVAttentionArgs)}
+        self._needs = {}
+
+    def __getstate__(self):
+        """Copies and pickles have buffers of their own."""
+        return {name: value for name, value in self.__dict__.items() if name not in ('_heads', '_needs')}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self.key_codes.device
+        self._bound()
 
     @classmethod
     def empty(cls, batch, kv_heads, capacity, *, head_dim=64, format='int8', device='cuda'):
@@ -1114,9 +1133,14 @@ class QuantizedKVCache:
         """Bytes of all buffers."""
         return sum(t.numel() * t.element_size() for t in self.tensors())
 
-    def _struct(self):
-        return KVCacheStruct(KV_FORMATS[self.format], self.head_dim, self.batch, self.kv_heads, self.capacity,
-                             *(t.data_ptr() for t in self.tensors()))
+
+# The argument structs behind their cache, packed in one go (nested ctypes fields cost a call 4 us of 12).
+_KV_HEAD = struct.Struct('=II')
+_KV_APPEND = struct.Struct('=q8q4Q')                # seq; k, v; position, rows, cos, sin
+_KV_READ = struct.Struct('=Qqq8q')                  # length, start, count; keys, values
+_KV_ATTENTION = struct.Struct('=qq8q4Q8qfIQQ')      # seq, heads; q, out; position, rows, cos, sin; k, v; scale, 0; workspace, bytes
+_NO_ROWS = (0, 0, 0, 0)
+_MAX_FLOAT = (2 - 2 ** -23) * 2.0 ** 127
 
 
 def _kv_cache(cache):
@@ -1125,26 +1149,30 @@ def _kv_cache(cache):
     return cache
 
 
-def _kv_rows(t, name, cache, heads, seq=None):
-    """A [batch, seq, heads, head_dim] fp16 operand on the cache's device."""
-    if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.ndim != 4 or t.shape[0] != cache.batch
-            or t.shape[1] < 1 or t.shape[3] != cache.head_dim or (heads is not None and t.shape[2] != heads)
-            or (seq is not None and t.shape[1] != seq)):
+def _kv_rows(t, name, cache, heads, seq, keep, copy):
+    """(address, batch, row and head strides, seq, heads) of a [batch, seq, heads, head_dim] fp16 operand on the cache's
+    device.  Where its rows are not whole 16-byte pieces at 16-byte addresses, of a copy (added to `keep`) if `copy`."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.ndim != 4:
+        shape = None
+    else:
+        shape = t.shape
+    if (shape is None or shape[0] != cache.batch or shape[1] < 1 or shape[3] != cache.head_dim
+            or (heads is not None and shape[2] != heads) or (seq is not None and shape[1] != seq)):
         raise ValueError(f'{name} must be fp16 [batch, seq, heads, head_dim] = [{cache.batch}, '
                          f'{"seq" if seq is None else seq}, {"heads" if heads is None else heads}, {cache.head_dim}]')
     if t.device != cache.device:
         raise ValueError(f'{name} must be on {cache.device} with the cache (found {t.device})')
-    return t
-
-
-def _kv_ready(t):
-    """Whether the kernels take these rows where they lie: whole 16-byte pieces at 16-byte addresses."""
-    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or s % 8 == 0 for n, s in zip(t.shape[:3], t.stride()[:3])))
-
-
-def _kv_struct(t):
-    return KVRows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    b, i, h, d = t.stride()
+    at = t.data_ptr()
+    if d != 1 or at % 16 or (b | i | h) % 8:
+        if d != 1 or at % 16 or any(s % 8 and n > 1 for s, n in zip((b, i, h), shape)):
+            if not copy:
+                raise ValueError(f'the rows of {name} must be 16-byte pieces')
+            t = _aligned(t)
+            keep.append(t)
+            b, i, h, _ = t.stride()
+            at = t.data_ptr()
+    return (at, b, i, h), shape[1], shape[2]
 
 
 def _kv_counts(t, name, cache):
@@ -1157,7 +1185,7 @@ def _kv_counts(t, name, cache):
 
 def _kv_tables(cos, sin, cache):
     if cos is None and sin is None:
-        return None, None
+        return 0, 0
     for t, name in ((cos, 'cos'), (sin, 'sin')):
         if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.ndim != 2 or t.shape[1] != cache.head_dim
                 or t.shape[0] < cache.capacity or not t.is_contiguous() or t.data_ptr() % 16):
@@ -1186,19 +1214,12 @@ class _PreparedKV(_Prepared):
         _kv_run(self._fn, self._ref, self._device, self._what, stream)
 
 
-def _kv_append_args(cache, k, v, position, rows, cos, sin):
-    a = KVAppendArgs()
-    a.struct_size = ctypes.sizeof(KVAppendArgs)
-    a.cache, a.seq, a.k, a.v = _kv_cache(cache)._struct(), k.shape[1], _kv_struct(k), _kv_struct(v)
-    a.position = _kv_counts(position, 'position', cache)
-    a.rows = None if rows is None else _kv_counts(rows, 'rows', cache)
-    a.cos, a.sin = _kv_tables(cos, sin, cache)
-    return a
-
-
-def _kv_pair(cache, k, v, seq=None):
-    _kv_rows(k, 'k', _kv_cache(cache), cache.kv_heads, seq)
-    _kv_rows(v, 'v', cache, cache.kv_heads, k.shape[1])
+def _kv_append_args(cache, k, v, position, rows, cos, sin, keep, copy):
+    k, seq, _ = _kv_rows(k, 'k', _kv_cache(cache), cache.kv_heads, None, keep, copy)
+    v, _, _ = _kv_rows(v, 'v', cache, cache.kv_heads, seq, keep, copy)
+    return KVAppendArgs.from_buffer_copy(cache._heads[KVAppendArgs] + _KV_APPEND.pack(
+        seq, *k, *v, _kv_counts(position, 'position', cache), 0 if rows is None else _kv_counts(rows, 'rows', cache),
+        *_kv_tables(cos, sin, cache)))
 
 
 def kv_append(cache, k, v, position, *, rows=None, cos=None, sin=None):
@@ -1206,10 +1227,9 @@ def kv_append(cache, k, v, position, *, rows=None, cos=None, sin=None):
     position[b] .. of each sequence; blocks that become full are quantised.  position and rows: int64 [batch] on the
     device.  With cos and sin (fp16 [>= capacity, head_dim]) the keys are rotated first.  A sequence whose rows would not
     fit is left alone.  k and v may have any strides (a copy is made where rows are not 16-byte pieces)."""
-    _kv_pair(cache, k, v)
-    k, v = (t if _kv_ready(t) else _aligned(t) for t in (k, v))
-    a = _kv_append_args(cache, k, v, position, rows, cos, sin)
-    _kv_run(library().lb_kv_append, ctypes.byref(a), cache.device, 'lb_kv_append')
+    keep = []
+    a = _kv_append_args(cache, k, v, position, rows, cos, sin, keep, True)
+    _kv_run(library().lb_kv_append, a, cache.device, 'lb_kv_append')
 
 
 def kv_read(cache, length, *, start=0, count=None, keys=None, values=None):
@@ -1217,58 +1237,55 @@ def kv_read(cache, length, *, start=0, count=None, keys=None, values=None):
     [batch, kv_heads, count, head_dim].  length: int64 [batch] on the device, the slots that are held; rows at or past it
     are left as they are in `keys` and `values` (zero where they are allocated here)."""
     _kv_cache(cache)
-    count = cache.capacity - start if count is None else count
+    start = operator.index(start)
+    count = cache.capacity - start if count is None else operator.index(count)
     if not 0 <= start < cache.capacity or not 1 <= count <= cache.capacity - start:
         raise ValueError(f'slots {start} .. {start + count - 1} are not within the capacity {cache.capacity}')
     shape = (cache.batch, cache.kv_heads, count, cache.head_dim)
-    outs = []
+    outs, rows = [], []
     for name, t in (('keys', keys), ('values', values)):
         if t is None:
             t = torch.zeros(shape, dtype=torch.float16, device=cache.device)
-        elif (not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape or not _kv_ready(t)
-              or t.device != cache.device):
-            raise ValueError(f'{name} must be fp16 {list(shape)} on {cache.device}, its rows in 16-byte pieces')
+        elif not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape or t.device != cache.device:
+            raise ValueError(f'{name} must be fp16 {list(shape)} on {cache.device}')
+        b, h, i, d = t.stride()
+        at = t.data_ptr()
+        if d != 1 or at % 16 or any(s % 8 and n > 1 for s, n in zip((b, h, i), shape)):
+            raise ValueError(f'the rows of {name} must be 16-byte pieces')
         outs.append(t)
-    a = KVReadArgs()
-    a.struct_size = ctypes.sizeof(KVReadArgs)
-    a.cache, a.length = cache._struct(), _kv_counts(length, 'length', cache)
-    a.start, a.count = start, count
-    a.keys, a.values = (KVRows(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1)) for t in outs)
-    _kv_run(library().lb_kv_read, ctypes.byref(a), cache.device, 'lb_kv_read')
+        rows += (at, b, i, h)
+    a = KVReadArgs.from_buffer_copy(cache._heads[KVReadArgs] + _KV_READ.pack(
+        _kv_counts(length, 'length', cache), start, count, *rows))
+    _kv_run(library().lb_kv_read, a, cache.device, 'lb_kv_read')
     return tuple(outs)
-
-
-def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin):
-    a = KVAttentionArgs()
-    a.struct_size = ctypes.sizeof(KVAttentionArgs)
-    a.cache, a.seq, a.heads, a.q, a.out = cache._struct(), q.shape[1], q.shape[2], _kv_struct(q), _kv_struct(out)
-    a.position = _kv_counts(position, 'position', cache)
-    a.rows = None if rows is None else _kv_counts(rows, 'rows', cache)
-    a.cos, a.sin = _kv_tables(cos, sin, cache)
-    if k is not None:
-        a.k, a.v = _kv_struct(k), _kv_struct(v)
-    a.scale = cache.head_dim ** -0.5 if scale is None else scale
-    return a
-
-
-def _kv_check_attention(q, cache, out, k, v):
-    _kv_rows(q, 'q', _kv_cache(cache), None)
-    if q.shape[2] % cache.kv_heads or q.shape[2] < 1:
-        raise ValueError(f'the heads of q ({q.shape[2]}) must be a multiple of the kv_heads ({cache.kv_heads})')
-    if out is not None:
-        _kv_rows(out, 'out', cache, q.shape[2], q.shape[1])
-        if not _kv_ready(out):
-            raise ValueError('the rows of out must be 16-byte pieces')
-    if (k is None) != (v is None):
-        raise ValueError('k and v go together')
-    if k is not None:
-        _kv_pair(cache, k, v, q.shape[1])
 
 
 def kv_attention_workspace_bytes(args):
     size = ctypes.c_size_t(0)
     _check(library().lb_kv_attention_workspace_bytes(ctypes.byref(args), ctypes.byref(size)), 'lb_kv_attention_workspace_bytes')
     return size.value
+
+
+def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, keep, copy):
+    """The argument struct without its workspace, and the bytes that it needs of one."""
+    q, seq, heads = _kv_rows(q, 'q', _kv_cache(cache), None, None, keep, copy)
+    if heads % cache.kv_heads or heads < 1:
+        raise ValueError(f'the heads of q ({heads}) must be a multiple of the kv_heads ({cache.kv_heads})')
+    out, _, _ = _kv_rows(out, 'out', cache, heads, seq, keep, False)
+    if (k is None) != (v is None):
+        raise ValueError('k and v go together')
+    scale = cache.head_dim ** -0.5 if scale is None else float(scale)
+    if not 0 <= scale <= _MAX_FLOAT:
+        raise ValueError('scale must be finite (fp32) and >= 0')
+    k = _NO_ROWS if k is None else _kv_rows(k, 'k', cache, cache.kv_heads, seq, keep, copy)[0]
+    v = _NO_ROWS if v is None else _kv_rows(v, 'v', cache, cache.kv_heads, seq, keep, copy)[0]
+    a = KVAttentionArgs.from_buffer_copy(cache._heads[KVAttentionArgs] + _KV_ATTENTION.pack(
+        seq, heads, *q, *out, _kv_counts(position, 'position', cache), 0 if rows is None else _kv_counts(rows, 'rows', cache),
+        *_kv_tables(cos, sin, cache), *k, *v, scale, 0, 0, 0))
+    need = cache._needs.get((seq, heads))
+    if need is None:
+        need = cache._needs[seq, heads] = kv_attention_workspace_bytes(a)
+    return a, need
 
 
 _kv_workspaces = {}   # by device and stream: calls on a stream are ordered, so they can share one
@@ -1292,15 +1309,13 @@ def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, sca
     gets here where k and v are given (kv_append's arguments).  rows (default: all): a sequence's query rows; out rows
     behind them are left as they are (zero where out is allocated here).  scale: default head_dim ** -0.5.  cos and sin
     rotate q (and k).  Any strides of q, k and v (a copy is made where rows are not 16-byte pieces)."""
-    _kv_check_attention(q, cache, out, k, v)
-    q, k, v = (t if t is None or _kv_ready(t) else _aligned(t) for t in (q, k, v))
-    if out is None:
+    if out is None and isinstance(q, torch.Tensor):   # (what is not right with q is said below)
         out = (torch.empty if rows is None else torch.zeros)(q.shape, dtype=torch.float16, device=q.device)
-    a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin)
-    need = kv_attention_workspace_bytes(a)
+    keep = []
+    a, need = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, keep, True)
     if need:
         a.workspace, a.workspace_bytes = _kv_workspace(need, cache.device).data_ptr(), need
-    _kv_run(library().lb_kv_attention, ctypes.byref(a), cache.device, 'lb_kv_attention')
+    _kv_run(library().lb_kv_attention, a, cache.device, 'lb_kv_attention')
     return out
 
 
@@ -1309,10 +1324,7 @@ class PreparedKVAppend(_PreparedKV):
     v need rows of 16-byte pieces).  run() enqueues it on the current stream; positions are read on the device."""
 
     def __init__(self, cache, k, v, position, *, rows=None, cos=None, sin=None):
-        _kv_pair(cache, k, v)
-        if not _kv_ready(k) or not _kv_ready(v):
-            raise ValueError('the rows of k and v must be 16-byte pieces')
-        a = _kv_append_args(cache, k, v, position, rows, cos, sin)
+        a = _kv_append_args(cache, k, v, position, rows, cos, sin, None, False)
         self._bind('lb_kv_append', 'lb_kv_append', a, cache.device, [cache, k, v, position, rows, cos, sin])
 
 
@@ -1321,14 +1333,10 @@ class PreparedKVAttention(_PreparedKV):
     rows of 16-byte pieces).  Owns its workspace, so calls of one instance must be ordered (one stream)."""
 
     def __init__(self, q, cache, position, out, *, rows=None, k=None, v=None, scale=None, cos=None, sin=None):
-        _kv_check_attention(q, cache, out, k, v)
-        if out is None or not all(t is None or _kv_ready(t) for t in (q, k, v)):
-            raise ValueError('the rows of q, k, v and out must be 16-byte pieces')
-        a = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin)
+        a, need = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, None, False)
         keep = [q, cache, position, out, rows, k, v, cos, sin]
-        need = kv_attention_workspace_bytes(a)
         if need:
-            keep.append(torch.zeros(need, dtype=torch.uint8, device=q.device))
+            keep.append(torch.zeros(need, dtype=torch.uint8, device=cache.device))
             a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
         self._bind('lb_kv_attention', 'lb_kv_attention', a, cache.device, keep)
         self.out = out
