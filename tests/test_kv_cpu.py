@@ -282,3 +282,19 @@ def test_oracle_e4m3_is_the_format():
     assert np.array_equal(ko.e4m3(mid), even)
     x = np.random.default_rng(0).standard_normal(20000) * np.exp2(np.random.default_rng(1).integers(-12, 7, 20000))
     assert np.array_equal(ko.e4m3(x.astype(np.float32)), torch.from_numpy(x.astype(np.float32)).to(torch.float8_e4m3fn).double().numpy())
+
+
+def test_layer_cache_formats():
+    import smollm_random
+    from torch_npu_smollm import FrozenSmolLayer, FrozenSmolStack, _SHAPES
+    config = smollm_random.config(theta=10000.0, layers=1)
+    weights = {n: torch.zeros(s) if len(s) == 1 else torch.eye(*s) for n, s in _SHAPES.items()}
+    with pytest.raises(ValueError, match='cache must be'):
+        FrozenSmolLayer(config, weights, cache='int4')
+    layers = [FrozenSmolLayer(config, weights, mode='fp16', cache=c) for c in ('fp16', 'fp8')]
+    assert [layer.cache for layer in layers] == ['fp16', 'fp8'] and layers[1]._kv_capacity() == 64
+    with pytest.raises(ValueError, match='cache format'):
+        FrozenSmolStack.from_layers(layers)
+    state = layers[0].__dict__
+    del state['_cache_format']               # as a layer pickled before there was a choice
+    assert layers[0].cache == 'fp16'

@@ -18,6 +18,11 @@ Deviations (the reference limits come from its NPU graph and are lifted):
 KV snapshots keep the reference contract (decode never changes an earlier snapshot's
 valid positions): snapshots of one sequence share storage and append in place; decoding
 from a snapshot that is no longer the newest copies the storage first.
+
+cache='int8' or 'fp8' holds the KV cache in 8 bits (lowbit_hip.QuantizedKVCache; the reference has fp16 only): prefill
+and decode then attend over the held values with kv_attention, for any capacity and length, at half the memory and
+without a score matrix.  forward keeps no cache and stays as it is.  A snapshot more than 64 positions behind the newest
+one of its sequence goes on from the 8-bit values of its last, incomplete block of 64.
 """
 from dataclasses import dataclass, replace
 import json
@@ -105,14 +110,71 @@ class SmolKVCache:
     _storage: object = None
 
 
+class _QuantizedStorage:
+    """An 8-bit cache shared by the snapshots of one sequence; `high` is the written length."""
+
+    def __init__(self, cache, high):
+        self.cache, self.high = cache, high
+
+    def read(self, length, start=0, count=None):
+        """fp16 keys and values [B, 3, count, 64] of the first `length` slots; zeros behind them."""
+        cache, block = self.cache, lowbit_hip.KV_BLOCK
+        count = cache.capacity - start if count is None else count
+        # Past the ring of fp16 rows the last block is read as it was closed since.
+        held = length if length // block >= self.high // block - 1 else (length + block - 1) // block * block
+        rows = lowbit_hip.kv_read(cache, torch.full((cache.batch,), held, dtype=torch.int64, device=cache.device), start=start,
+                                  count=count)
+        if held > length:
+            for t in rows:
+                t[:, :, max(0, length - start):] = 0
+        return rows
+
+    def branch(self, length):
+        """A copy that goes on from `length` slots."""
+        copy, block = _QuantizedStorage(self.cache.clone(), length), lowbit_hip.KV_BLOCK
+        if length // block < self.high // block - 1 and length % block:   # its open block's fp16 rows are gone
+            start = length // block * block
+            k, v = (t.transpose(1, 2) for t in self.read(length, start, length - start))
+            lowbit_hip.kv_append(copy.cache, k, v, torch.full((k.shape[0],), start, dtype=torch.int64, device=k.device))
+        return copy
+
+
+@dataclass(frozen=True, eq=False)
+class SmolQuantizedKVCache:
+    """KV snapshot of a layer with an 8-bit cache: positions [0, length) of `cache` are valid."""
+    _owner: object
+    _sequence: object
+    cache: object
+    length: int
+    _position: torch.Tensor
+    _storage: object
+    _capacity: int
+
+    def read(self):
+        """fp16 keys and values [B,3,capacity,64] as the cache holds them, zeros past the length."""
+        return self._storage.read(self.length, 0, self._capacity)
+
+    @property
+    def keys(self):
+        return self.read()[0]
+
+    @property
+    def values(self):
+        return self.read()[1]
+
+
 class FrozenSmolLayer(torch.nn.Module):
-    """One frozen SmolLM2-135M decoder layer (reference :66-544)."""
+    """One frozen SmolLM2-135M decoder layer (reference :66-544).  cache: the KV cache's format, fp16, int8 or fp8."""
+
+    _cache_format = 'fp16'   # (of layers pickled before there was a choice)
 
     def __init__(self, config, weights, *, mode='w8a16', packed_weights=None, fp16_projections=(), corrections=None,
-                 capacity=64):
+                 capacity=64, cache='fp16'):
         super().__init__()
         if mode not in _WEIGHT_FORMATS:
             raise ValueError('Requires fp16, w8a16, w4a16 or nf4a16')
+        if cache != 'fp16' and cache not in lowbit_hip.KV_FORMATS:
+            raise ValueError('cache must be fp16, int8 or fp8')
         fmt = _WEIGHT_FORMATS[mode]
         self._fp16_projections = _projection_policy(mode, fp16_projections)
         theta = config.get('rope_theta') if isinstance(config, dict) else None
@@ -142,6 +204,7 @@ class FrozenSmolLayer(torch.nn.Module):
         self._mode = mode
         self._theta = float(theta)
         self._capacity = capacity
+        self._cache_format = cache
         self._corrections = {} if corrections is None else dict(corrections)
         self._weights = {name: _half(weights[name], shape) for name, shape in _SHAPES.items()}
         self._packed = {}
@@ -159,7 +222,7 @@ class FrozenSmolLayer(torch.nn.Module):
 
     @classmethod
     def from_checkpoint(cls, directory, *, layer_index=0, mode='w8a16', packed_weights=None, fp16_projections=(),
-                        corrections=None, capacity=64):
+                        corrections=None, capacity=64, cache='fp16'):
         from safetensors import safe_open
         _projection_policy(mode, fp16_projections)
         directory = Path(directory)
@@ -170,7 +233,7 @@ class FrozenSmolLayer(torch.nn.Module):
         with safe_open(directory / 'model.safetensors', framework='pt', device='cpu') as file:
             weights = {n[len(prefix):]: file.get_tensor(n) for n in file.keys() if n.startswith(prefix)}
         return cls(config, weights, mode=mode, packed_weights=packed_weights, fp16_projections=fp16_projections,
-                   corrections=corrections, capacity=capacity)
+                   corrections=corrections, capacity=capacity, cache=cache)
 
     def __getstate__(self):
         """Copies and pickles place their own device state (it holds raw pointers to this layer's weights)."""
@@ -187,6 +250,10 @@ class FrozenSmolLayer(torch.nn.Module):
     @property
     def capacity(self):
         return self._capacity
+
+    @property
+    def cache(self):
+        return self._cache_format
 
     def _shape(self, shape, limit=None):
         limit = self._capacity if limit is None else limit
@@ -298,8 +365,13 @@ class FrozenSmolLayer(torch.nn.Module):
                 state['rows'] = lowbit_hip.LayerRows(projections, hidden=HIDDEN, intermediate=1536, norm1=state['norm1'],
                                                      norm2=state['norm2'], eps=1e-5, heads=HEADS, kv_heads=KV_HEADS,
                                                      cos=state['cos'], sin=state['sin'])
+            if self._cache_format != 'fp16':   # (an 8-bit cache holds whole blocks)
+                state['kv_tables'] = tuple(t.to(device) for t in _rope_tables(self._theta, self._kv_capacity()))
             self._device[key] = state
         return self._device[key]
+
+    def _kv_capacity(self):
+        return (self._capacity + lowbit_hip.KV_BLOCK - 1) // lowbit_hip.KV_BLOCK * lowbit_hip.KV_BLOCK
 
     @staticmethod
     def _linear(state, x2d, name, out=None):
@@ -374,19 +446,44 @@ class FrozenSmolLayer(torch.nn.Module):
         self._validate_input(x)
         return self._full(x, None)
 
+    def _over_quantized(self, x, cache, position):
+        """The layer over new rows x at slots position .. of an 8-bit cache, which they are appended to."""
+        state = self._dev(x.device)
+        b, s, d = x.shape
+        n1 = lowbit_hip.rms_rows(x, state['norm1']).view(b * s, d)
+        q = self._linear(state, n1, 'self_attn.q_proj.weight').view(b, s, HEADS, HEAD_DIM)
+        k = self._linear(state, n1, 'self_attn.k_proj.weight').view(b, s, KV_HEADS, HEAD_DIM)
+        v = self._linear(state, n1, 'self_attn.v_proj.weight').view(b, s, KV_HEADS, HEAD_DIM)
+        cos, sin = state['kv_tables']
+        att = lowbit_hip.kv_attention(q, cache, position, k=k, v=v, cos=cos, sin=sin, scale=0.125)
+        delta = self._linear(state, att.view(b * s, d), 'self_attn.o_proj.weight').view(b, s, d)
+        return self._mlp(state, (x + delta).half())
+
     def prefill(self, x):
         """Full prefix; returns the output and a KV snapshot (reference :506-523)."""
         b, s, _ = self._validate_input(x)
+        if self._cache_format != 'fp16':
+            cache = lowbit_hip.QuantizedKVCache.empty(b, KV_HEADS, self._kv_capacity(), head_dim=HEAD_DIM,
+                                                      format=self._cache_format, device=x.device)
+            position = torch.zeros(b, dtype=torch.int64, device=x.device)
+            out = self._over_quantized(x, cache, position)
+            return out, SmolQuantizedKVCache(self._cache_owner, object(), cache, s, position + s, _QuantizedStorage(cache, s),
+                                             self._capacity)
         storage = _KVStorage(torch.zeros((2, b, KV_HEADS, self._capacity, HEAD_DIM), dtype=torch.float16, device=x.device), s)
         out = self._full(x, storage.both)
         position = torch.full((1,), s, dtype=torch.int32, device=x.device)
         return out, SmolKVCache(self._cache_owner, object(), storage.keys, storage.values, s, position, storage)
 
     def _validate_cache(self, x, cache):
-        if x.shape[1] != 1 or type(cache) is not SmolKVCache or cache._owner is not self._cache_owner:
+        kind = SmolKVCache if self._cache_format == 'fp16' else SmolQuantizedKVCache
+        if x.shape[1] != 1 or type(cache) is not kind or cache._owner is not self._cache_owner:
             raise ValueError("Decode requires one token and this layer's own KV cache")
         if type(cache.length) is not int or not 1 <= cache.length < self._capacity:
             raise ValueError(f'KV cache is full or has an invalid length; total tokens must be <= {self._capacity}')
+        if kind is SmolQuantizedKVCache:
+            if cache.cache.batch != x.shape[0] or cache.cache.device != x.device:
+                raise ValueError('KV cache has the wrong batch, layout or device')
+            return
         if (tuple(cache.keys.shape) != (x.shape[0], KV_HEADS, self._capacity, HEAD_DIM)
                 or cache.keys.dtype != torch.float16 or cache.keys.device != x.device):
             raise ValueError('KV cache has the wrong batch, layout or device')
@@ -395,6 +492,12 @@ class FrozenSmolLayer(torch.nn.Module):
         """Append exactly one token; earlier snapshots keep their valid positions (reference :529-544)."""
         self._validate_input(x)
         self._validate_cache(x, cache)
+        if self._cache_format != 'fp16':
+            storage = cache._storage if cache._storage.high == cache.length else cache._storage.branch(cache.length)
+            out = self._over_quantized(x, storage.cache, cache._position)
+            storage.high = cache.length + 1
+            return out, SmolQuantizedKVCache(self._cache_owner, cache._sequence, storage.cache, cache.length + 1,
+                                             cache._position + 1, storage, self._capacity)
         state = self._dev(x.device)
         storage = cache._storage
         if storage.high != cache.length:  # decoding from an older snapshot: copy on write
@@ -429,7 +532,7 @@ class FrozenSmolStack(torch.nn.Module):
     """Contiguous frozen decoder layers (reference :558-657)."""
 
     def __init__(self, directory, *, start_layer=0, num_layers=2, mode='w8a16', packed_weights=None,
-                 fp16_projections=(), corrections=None, capacity=64):
+                 fp16_projections=(), corrections=None, capacity=64, cache='fp16'):
         super().__init__()
         from safetensors import safe_open
         _projection_policy(mode, fp16_projections)
@@ -444,7 +547,7 @@ class FrozenSmolStack(torch.nn.Module):
                 prefix = f'model.layers.{index}.'
                 weights = {n[len(prefix):]: file.get_tensor(n) for n in names if n.startswith(prefix)}
                 layers.append(FrozenSmolLayer(
-                    config, weights, mode=mode, fp16_projections=fp16_projections, capacity=capacity,
+                    config, weights, mode=mode, fp16_projections=fp16_projections, capacity=capacity, cache=cache,
                     packed_weights=None if packed_weights is None else packed_weights[index],
                     corrections=None if corrections is None else corrections[index]))
         self._init_layers(layers, start_layer, mode, fp16_projections)
@@ -483,8 +586,8 @@ class FrozenSmolStack(torch.nn.Module):
         """Stack already-built FrozenSmolLayer objects (e.g. random-init weights without a checkpoint)."""
         if not layers or any(not isinstance(layer, FrozenSmolLayer) for layer in layers):
             raise ValueError('Requires a nonempty list of FrozenSmolLayer')
-        if len({(layer.mode, layer.fp16_projections, layer.capacity) for layer in layers}) != 1:
-            raise ValueError('Layers must share mode, protection policy and capacity')
+        if len({(layer.mode, layer.fp16_projections, layer.capacity, layer.cache) for layer in layers}) != 1:
+            raise ValueError('Layers must share mode, protection policy, capacity and cache format')
         stack = cls.__new__(cls)
         torch.nn.Module.__init__(stack)
         stack._init_layers(list(layers), start_layer, layers[0].mode, tuple(sorted(layers[0].fp16_projections)))
@@ -871,20 +974,22 @@ class GraphDecoder:
 
     # ---------------------------------------------------------------- common
     def load(self, caches, next_token):
-        """Start from a prefill snapshot: copy its K/V, set the position and the next input token."""
+        """Start from a prefill snapshot: copy its K/V (an 8-bit one read back: the decoder's own cache is fp16), set the
+        position and the next input token."""
         length = caches[0].length
         if not 1 <= length < self.capacity:
             raise ValueError('the snapshot leaves no free KV slot')
-        targets, sources = self.keys + self.values, [c.keys for c in caches] + [c.values for c in caches]
+        rows = [c.read() if isinstance(c, SmolQuantizedKVCache) else (c.keys, c.values) for c in caches]
+        targets, sources = self.keys + self.values, [k for k, _ in rows] + [v for _, v in rows]
         if self.fused and len(targets) == len(sources) and all(t.shape == s.shape for t, s in zip(targets, sources)):
             # Whole buffers, contiguous: all layers' copies share launches (60 strided copies took 0.5 ms of a
             # 16-token generation).  What a later continuation wrote past `length` comes along: the fused kernels'
             # buffers end at the position, so they read no slot before its own token has written it.
             torch._foreach_copy_(targets, sources)
         else:
-            for dst_k, dst_v, cache in zip(self.keys, self.values, caches):
-                dst_k[:, :, :length].copy_(cache.keys[:, :, :length])
-                dst_v[:, :, :length].copy_(cache.values[:, :, :length])
+            for dst_k, dst_v, (keys, values) in zip(self.keys, self.values, rows):
+                dst_k[:, :, :length].copy_(keys[:, :, :length])
+                dst_v[:, :, :length].copy_(values[:, :, :length])
             if not self.fused:  # the staged attention multiplies every slot, by masked scores and zero probabilities
                 for dst in self.keys + self.values:
                     dst[:, :, length:].zero_()
