@@ -645,3 +645,27 @@ def test_attention_of_many_sequences(device):
             assert bool((out[b] == 3).all()), b
         else:
             check_attention(out[b:b + 1], q[b:b + 1], k[b:b + 1], v[b:b + 1], [starts[b]], [1], 'int8', dim ** -0.5, kv_heads)
+
+
+@pytest.mark.parametrize('batch', [2, 33, 64, 65])
+def test_attention_of_unequal_lengths(device, batch):
+    """Batches on both sides of what one wave ranks, from one slot to thousands, some without rows: every sequence is
+    found once, whole, whichever workgroups share it."""
+    announce('kv attention unequal', batch)
+    heads, kv_heads, dim, capacity = 3, 1, 64, 2560
+    rng = np.random.default_rng(120 + batch)
+    starts = [int(x) for x in rng.choice([0, 63, 64, 200, 700, 1500, 2500], batch)]
+    rows = [int(x) for x in rng.integers(0, 5, batch) > 0]
+    starts[-1], rows[-1], starts[0], rows[0] = 2559, 1, 0, 1
+    k, v = rows_of(121, batch, capacity, kv_heads, dim), rows_of(122, batch, capacity, kv_heads, dim, spread=.3)
+    q = rows_of(123, batch, 1, heads, dim)
+    cache = fresh(device, batch, kv_heads, capacity, dim, 'fp8', fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device),
+                 rows=ints([s + r for s, r in zip(starts, rows)], device))
+    out = torch.full((batch, 1, heads, dim), 3.0, dtype=torch.float16, device=device)
+    lb.kv_attention(dev(q, device), cache, ints(starts, device), rows=ints(rows, device), out=out)
+    some = [b for b in range(batch) if rows[b]]
+    assert bool((out[[b for b in range(batch) if not rows[b]]] == 3).all())
+    worst = check_attention(out[some], q[some], k[some], v[some], [starts[b] for b in some], [1] * len(some), 'fp8',
+                            dim ** -0.5, kv_heads)
+    print(f'[kv attention] unequal {batch}: {worst:.2f} of the bound', flush=True)

@@ -438,6 +438,17 @@ constexpr int kKvTickets = 1024;      // (LB_ZEROED_WORKSPACE_BYTES)
 // themselves (the CUs); blocks of a part at the least (one a wave); and places for the sums of parts.
 constexpr int kKvSplit = 256, kKvLeast = 4, kKvPlaces = 2 * kKvSplit + 2;
 
+// Inclusive prefix sum over the wave's lanes, in data-parallel shifts of rows of 16 and broadcasts of their ends.
+__device__ __forceinline__ uint32_t kv_scan(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, true);   // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false);  // row_bcast 15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false);  // row_bcast 31 into rows 2 and 3
+  return x;
+}
+
 // The largest over the four lanes that hold a query.
 __device__ __forceinline__ float kv_max_across(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -532,8 +543,9 @@ __device__ __forceinline__ void kv_join(__amdgpu_buffer_rsrc_t po, __amdgpu_buff
 //     of 128: parts of 4, 16 and 64 blocks take 8.5, 12.8 and 27.9 us; eight waves a workgroup 9.3, 13.5 and 26.6).
 //   - A workgroup takes one part: going on with another costs a whole chain of waits, 4 us (64 sequences of 1 to 8192
 //     slots, 8 heads of 128, equal shares cut across sequences: 128 us).
-//   - Longest sequences first, and every other 256 workgroups backwards, so that the two that share a CU have together what
-//     others have: the same 64 sequences 100 us (5.4 TB/s) against 118 in the batch's order.
+//   - Longer sequences first, and every other 256 workgroups backwards, so that the two that share a CU have together what
+//     others have: the same 64 sequences 100 us (5.4 TB/s) against 118 in the batch's order.  (Up to 64 sequences, by
+//     prefix sums in registers; sorting them outright took 50 ns a sequence.)
 //
 // Scores are K.Q^T and outputs V^T.P^T, so that a lane holds one query throughout (column lane % 16): its maximum,
 // total and rescaling are the lane's own, and the probabilities that it computes are the B operand of the second product
@@ -551,8 +563,8 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
     float sums[W][R][PITCH];
     float tops[W][R], totals[W][R];
   };
-  __shared__ union { __align__(16) Sums w; uint32_t blocks[2][NT]; } mem;
-  __shared__ uint32_t found[8], tops[W];
+  __shared__ __align__(16) Sums mem;
+  __shared__ uint32_t found[8], tops[W], sum_of[2][W];
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -566,7 +578,7 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
     const bool fine = kv_span(p.position, p.rows, b, p.seq, p.c.capacity, first, count);
     return blocks_of(fine, first, count);
   };
-  // Workgroups in the order of what they take: the longest sequences first, their parts and heads side by side; every
+  // Workgroups in the order of what they take: longer sequences first, their parts and heads side by side; every
   // other 256 of them backwards, since the two that are 256 apart share a CU.
   const uint32_t heads = p.c.kv_heads, turned = blockIdx.x & 256 && (blockIdx.x | 255) < gridDim.x ? blockIdx.x ^ 255 : blockIdx.x;
   const uint32_t h = turned % heads, ticket = turned / heads;
@@ -580,24 +592,28 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
     most = part_of(blocks_of(fine, first, count));
   } else if (p.batch <= 64) {             // a lane per sequence, in every wave by itself
     if (lane < p.batch) fine = kv_span(p.position, p.rows, lane, p.seq, p.c.capacity, first, count);
-    const uint32_t n = blocks_of(fine, first, count);
-    uint32_t all = n;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d);
-    most = part_of(__builtin_amdgcn_readfirstlane(all));
+    const uint32_t n = lane < p.batch ? blocks_of(fine, first, count) : 0, upto = kv_scan(n);
+    const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+    most = part_of(all);
     const uint32_t parts = (n + most - 1) / most;
-    uint32_t before = 0, longer = 0;
-    for (int i = 0; i < p.batch; ++i) {
-      const uint32_t other = __builtin_amdgcn_readlane(n, i), its = __builtin_amdgcn_readlane(parts, i);
-      const bool ahead = other > n || (other == n && i < lane);
-      before += ahead ? its : 0;
-      longer += ahead ? other : 0;
+    // Nine classes of length, in quarters of the mean; within one the batch's order.  Three classes' sums share a
+    // register, ten bits each: the parts of up to 64 sequences are at most 64 + kKvSplit together.
+    static_assert(64 + kKvSplit < 1024, "kv_attend: sums of parts in ten bits");
+    const uint32_t mine = 8 - min(8u, (uint32_t)((float)n * (4.0f * p.batch) * __builtin_amdgcn_rcpf((float)max(all, 1u))));
+    const uint32_t three = mine / 3, at = (mine - 3 * three) * 10;
+    uint32_t before = 0, base = 0;
+#pragma unroll
+    for (uint32_t c = 0; c < 3; ++c) {
+      const uint32_t its = three == c ? parts << at : 0, sum = kv_scan(its), ends = __builtin_amdgcn_readlane(sum, 63);
+      const uint32_t e0 = ends & 1023, e1 = ends >> 10 & 1023, e2 = ends >> 20;
+      if (three == c) before = base + (at == 0 ? 0 : at == 10 ? e0 : e0 + e1) + (sum >> at & 1023) - parts;
+      base += e0 + e1 + e2;
     }
     const uint64_t it = __ballot(ticket >= before && ticket - before < parts);
     if (it == 0) return;
     b = __builtin_ctzll(it);
     part = ticket - __builtin_amdgcn_readlane(before, b);
-    ahead = __builtin_amdgcn_readlane(longer, b);
+    ahead = __builtin_amdgcn_readlane(upto - n, b);
     first = __builtin_amdgcn_readlane(first, b);
     count = __builtin_amdgcn_readlane(count, b);
     fine = __builtin_amdgcn_readlane((int)fine, b);
@@ -605,38 +621,40 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
     // Larger batches in their own order: a sum over all sequences, then NT sequences at a time.
     uint32_t sum = 0;
     for (int i = tid; i < p.batch; i += NT) sum += blocks_at(i);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
-    if (lane == 0) tops[wave] = sum;
+    sum = kv_scan(sum);
+    if (lane == 63) sum_of[0][wave] = sum;
     if (tid == 0) found[0] = ~0u;
     __syncthreads();
     uint32_t all = 0;
-    for (int w = 0; w < W; ++w) all += tops[w];
+    for (int w = 0; w < W; ++w) all += sum_of[0][w];
     most = part_of(all);
-    uint32_t parts_before = 0, blocks_before = 0;
+    uint32_t parts_before = 0, blocks_before = 0;   // of the chunks before this one
     for (int c = 0; c < p.batch; c += NT) {
       const uint32_t n = c + tid < p.batch ? blocks_at(c + tid) : 0, parts = (n + most - 1) / most;
-      mem.blocks[0][tid] = n;
-      mem.blocks[1][tid] = parts;
+      const uint32_t upto = kv_scan(n), parts_upto = kv_scan(parts);
       __syncthreads();
-      uint32_t before = parts_before, longer = blocks_before;
-      for (int i = 0; i < NT; ++i) {
-        const uint32_t other = mem.blocks[0][i], its = mem.blocks[1][i];
-        if (i < tid) {
-          before += its;
-          longer += other;
+      if (lane == 63) {
+        sum_of[0][wave] = upto;
+        sum_of[1][wave] = parts_upto;
+      }
+      __syncthreads();
+      uint32_t before = parts_before + parts_upto - parts, longer = blocks_before + upto - n;
+      for (int w = 0; w < W; ++w) {
+        if (w < wave) {
+          longer += sum_of[0][w];
+          before += sum_of[1][w];
         }
-        parts_before += its;
-        blocks_before += other;
+        blocks_before += sum_of[0][w];
+        parts_before += sum_of[1][w];
       }
       if (ticket >= before && ticket - before < parts) {
         found[0] = c + tid;
         found[1] = ticket - before;
         found[2] = longer;
       }
-      __syncthreads();
       if (ticket < parts_before) break;
     }
+    __syncthreads();
     b = __builtin_amdgcn_readfirstlane(found[0]);
     if (b == ~0u) return;
     part = __builtin_amdgcn_readfirstlane(found[1]);
@@ -875,12 +893,12 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
   for (int t = 0; t < QT; ++t) {
     const int r = 16 * t + j;
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *reinterpret_cast<f4 *>(&mem.w.sums[wave][r][16 * d + 4 * g]) = acc[t][d];
+    for (int d = 0; d < DT; ++d) *reinterpret_cast<f4 *>(&mem.sums[wave][r][16 * d + 4 * g]) = acc[t][d];
     total[t] += __shfl_xor(total[t], 16);
     total[t] += __shfl_xor(total[t], 32);
     if (g == 0) {
-      mem.w.tops[wave][r] = top[t];
-      mem.w.totals[wave][r] = total[t];
+      mem.tops[wave][r] = top[t];
+      mem.totals[wave][r] = total[t];
     }
   }
   __syncthreads();
@@ -896,15 +914,15 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
   const int slot = 2 * unit + part;
   for (int i = tid; i < rows * DQ; i += NT) {
     const int r = i / DQ, d = i % DQ * 4;
-    float top = mem.w.tops[0][r], sum = 0.0f;
+    float top = mem.tops[0][r], sum = 0.0f;
 #pragma unroll
-    for (int w = 1; w < W; ++w) top = fmaxf(top, mem.w.tops[w][r]);
+    for (int w = 1; w < W; ++w) top = fmaxf(top, mem.tops[w][r]);
     f4 o = zero;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = __builtin_amdgcn_exp2f(mem.w.tops[w][r] - top);
-      sum += f * mem.w.totals[w][r];
-      o += f * *reinterpret_cast<const f4 *>(&mem.w.sums[w][r][d]);
+      const float f = __builtin_amdgcn_exp2f(mem.tops[w][r] - top);
+      sum += f * mem.totals[w][r];
+      o += f * *reinterpret_cast<const f4 *>(&mem.sums[w][r][d]);
     }
     if (parts == 1) {
       store(r, d, o, sum);
@@ -917,7 +935,7 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
     }
   }
   if (parts > 1 && kv_last_part(p.tickets + unit, parts, &found[6]))
-    kv_join<R, D, NT>(po, pm, rows, parts, [&](uint32_t k) { return 2 * unit + k; }, reinterpret_cast<f4 *>(&mem.w.sums), store);
+    kv_join<R, D, NT>(po, pm, rows, parts, [&](uint32_t k) { return 2 * unit + k; }, reinterpret_cast<f4 *>(&mem.sums), store);
 }
 
 // Attention of more query rows: a KV head's rows (row i of the call and query head g of the group: row i group + g) in
