@@ -386,7 +386,7 @@ typedef struct lb_kv_attention_args {
   const int64_t *rows;         /* device [batch], 0..seq, or NULL: its query rows (out rows behind them stay as they are) */
   const void *cos, *sin;       /* fp16 [capacity, head_dim], or NULL: rotates q (and k) as lb_kv_append does */
   lb_kv_rows k, v;             /* data NULL: the rows are in the cache already; else appended first, as lb_kv_append */
-  float scale;                 /* score scale, finite and >= 0 (usually 1 / sqrt(head_dim)) */
+  float scale;                 /* score scale, 0 to 2^16 (usually 1 / sqrt(head_dim)) */
   uint32_t reserved2;
   void *workspace;             /* lb_kv_attention_workspace_bytes, 256-byte aligned.  Its first LB_ZEROED_WORKSPACE_BYTES
                                   are zero before its first use, and every call leaves them zero again; for any calls,

@@ -669,3 +669,36 @@ def test_attention_of_unequal_lengths(device, batch):
     worst = check_attention(out[some], q[some], k[some], v[some], [starts[b] for b in some], [1] * len(some), 'fp8',
                             dim ** -0.5, kv_heads)
     print(f'[kv attention] unequal {batch}: {worst:.2f} of the bound', flush=True)
+
+
+def test_two_graphs_of_plain_calls(device):
+    """kv_attention and kv_append captured as they are, twice; replays of both graphs at once and eager calls between
+    them give what the eager calls gave."""
+    announce('kv two graphs')
+    heads, kv_heads, dim, n = 4, 2, 64, 4000
+    made, graphs = [], []
+    for i in range(2):
+        k, v = rows_of(130 + i, 2, n, kv_heads, dim), rows_of(132 + i, 2, n, kv_heads, dim)
+        cache = lb.QuantizedKVCache.empty(2, kv_heads, n + 64, head_dim=dim, device=device)
+        at = ints([n - 65, 100], device)
+        lb.kv_append(cache, dev(k[:, :n - 65], device), dev(v[:, :n - 65], device), ints([0, 0], device), rows=at)
+        q = dev(rows_of(134 + i, 2, 1, heads, dim), device).expand(2, 3, heads, dim)[:, :1]
+        made.append((cache, q, at, dev(k[:, n - 65:n - 64], device), dev(v[:, n - 65:n - 64], device)))
+    call = lambda c, q, at, k, v: (lb.kv_append(c, k, v, at), lb.kv_attention(q, c, at, k=k, v=v))[1]
+    want = [call(*m) for m in made]
+    torch.cuda.synchronize()
+    for m in made:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(*m)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream(device) for _ in range(2)]
+    for _ in range(4):
+        for (graph, out), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), m, w in zip(graphs, made, want):
+            assert torch.equal(out, w) and torch.equal(call(*m), w)
+        torch.cuda.synchronize()

@@ -103,6 +103,7 @@ BAD_ATTENTION = [
     (dict(scale=float('nan')), 'scale', lb.INVALID_ARGUMENT),
     (dict(scale=float('inf')), 'scale', lb.INVALID_ARGUMENT),
     (dict(scale=-1.0), 'scale', lb.INVALID_ARGUMENT),
+    (dict(scale=65537.0), 'scale', lb.INVALID_ARGUMENT),
     (dict(q__data=0xA00004), 'q must', lb.INVALID_ARGUMENT),
     (dict(out__head_stride=0), 'rows of out overlap', lb.INVALID_ARGUMENT),
     (dict(out__data=0xA00040), 'out overlaps q', lb.INVALID_ARGUMENT),
@@ -241,6 +242,7 @@ AT = torch.zeros(2, dtype=torch.int64)
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=1e300), 'scale'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=float('nan')), 'scale'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=-0.1), 'scale'),
+    (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, scale=1e6), 'scale'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, k=half(2, 2, 3, 64), v=half(2, 2, 3, 64)), 'k must be'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, out=half(2, 1, 64, 9).transpose(2, 3)), '16-byte'),
     (lambda c: lb.kv_attention(half(2, 1, 9, 64), c, AT, out=half(2, 2, 9, 64)), 'out must be'),
@@ -298,3 +300,17 @@ def test_layer_cache_formats():
     state = layers[0].__dict__
     del state['_cache_format']               # as a layer pickled before there was a choice
     assert layers[0].cache == 'fp16'
+
+
+def test_the_buffers_are_fixed():
+    """What calls are given was packed once: another tensor in place of a buffer is refused, copies have their own."""
+    import copy
+    import pickle
+    cache = HostCache()
+    with pytest.raises(AttributeError, match='fixed'):
+        cache.key_codes = torch.zeros_like(cache.key_codes)
+    for twin in (copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))):
+        assert twin.key_codes.data_ptr() != cache.key_codes.data_ptr()
+        packed = bytes(twin._heads[lb.KVReadArgs])
+        assert twin.key_codes.data_ptr().to_bytes(8, 'little') in packed
+        assert cache.key_codes.data_ptr().to_bytes(8, 'little') not in packed

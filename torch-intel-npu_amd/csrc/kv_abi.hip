@@ -2,7 +2,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <type_traits>
 
 #include "../../include/lowbit_decode_hip.h"
@@ -15,6 +14,7 @@ using namespace lb::abi;
 namespace {
 
 constexpr int64_t kMaxCapacity = (int64_t)1 << 28, kMaxStride = (int64_t)1 << 40, kMaxRows = (int64_t)1 << 28;
+constexpr float kMaxScale = 65536.0f;   // |q| and |k| are below 2^16, so scores stay within 2^56
 
 KvCache cache_params(const lb_kv_cache &c) {
   KvCache p{};
@@ -198,9 +198,9 @@ lb_status check_shape(const char *what, const lb_kv_attention_args *a) {
   if (a->seq < 1 || a->seq > kMaxRows || a->heads < 1 || a->heads > 65535 || a->heads % c.kv_heads != 0 ||
       a->seq * (a->heads / c.kv_heads) > kMaxRows)
     return fail(LB_INVALID_ARGUMENT, "%s: heads a multiple of kv_heads up to 65535, and 1 to 2^28 rows of a KV head required", what);
-  if (c.batch * c.kv_heads > (1 << 24) || c.batch * c.kv_heads * ((a->seq * (a->heads / c.kv_heads) + 127) / 128) > (1 << 24))
-    return fail(LB_UNSUPPORTED, "%s: more than 2^24 tiles of 128 rows of a sequence and KV head", what);
-  if (!(a->scale >= 0.0f) || !std::isfinite(a->scale)) return fail(LB_INVALID_ARGUMENT, "%s: scale must be finite and >= 0", what);
+  if (c.batch * c.kv_heads > (1 << 23) || c.batch * c.kv_heads * ((a->seq * (a->heads / c.kv_heads) + 127) / 128) > (1 << 23))   // 2^32 threads a launch
+    return fail(LB_UNSUPPORTED, "%s: more than 2^23 tiles of 128 rows of a sequence and KV head", what);
+  if (!(a->scale >= 0.0f && a->scale <= kMaxScale)) return fail(LB_INVALID_ARGUMENT, "%s: scale must be 0 to 2^16", what);
   return LB_OK;
 }
 

@@ -429,7 +429,7 @@ struct KvAttendParams {
   float scale;            // score scale * log2(e)
 };
 
-constexpr float kKvLowest = -1e30f;   // a running maximum below every score (scores are under 1e14 in magnitude)
+constexpr float kKvLowest = -1e30f;   // a running maximum below every score (scores are under 1e17 in magnitude)
 // Probabilities are 2^kKvLift above 1 at a row's running maximum, which is raised where a score exceeds it by more than
 // kKvSlack (in units of log2): fp16 then has them in [2^-24, 2^14], of which the smallest are 2^-34 of the largest.
 constexpr float kKvLift = 10.0f, kKvSlack = 4.0f;

@@ -1092,8 +1092,14 @@ class QuantizedKVCache:
         """What every call's argument struct begins with, and the workspaces that attention calls need by their rows."""
         cache = KVCacheStruct(KV_FORMATS[self.format], self.head_dim, self.batch, self.kv_heads, self.capacity,
                               *(t.data_ptr() for t in self.tensors()))
-        self._heads = {args: _KV_HEAD.pack(ctypes.sizeof(args), 0) + bytes(cache) for args in (KVAppendArgs, KVReadArgs, KVAttentionArgs)}
-        self._needs = {}
+        heads = {args: _KV_HEAD.pack(ctypes.sizeof(args), 0) + bytes(cache) for args in (KVAppendArgs, KVReadArgs, KVAttentionArgs)}
+        self.__dict__.update(_heads=heads, _needs={})
+
+    def __setattr__(self, name, value):
+        """The buffers are fixed: their addresses are in what calls are given."""
+        if '_heads' in self.__dict__:
+            raise AttributeError(f'{name}: the buffers of a QuantizedKVCache are fixed; make another of other tensors')
+        super().__setattr__(name, value)
 
     def __getstate__(self):
         """Copies and pickles have buffers of their own."""
@@ -1140,7 +1146,7 @@ _KV_APPEND = struct.Struct('=q8q4Q')                # seq; k, v; position, rows,
 _KV_READ = struct.Struct('=Qqq8q')                  # length, start, count; keys, values
 _KV_ATTENTION = struct.Struct('=qq8q4Q8qfIQQ')      # seq, heads; q, out; position, rows, cos, sin; k, v; scale, 0; workspace, bytes
 _NO_ROWS = (0, 0, 0, 0)
-_MAX_FLOAT = (2 - 2 ** -23) * 2.0 ** 127
+_KV_MAX_SCALE = 65536.0
 
 
 def _kv_cache(cache):
@@ -1275,8 +1281,8 @@ def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, kee
     if (k is None) != (v is None):
         raise ValueError('k and v go together')
     scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-    if not 0 <= scale <= _MAX_FLOAT:
-        raise ValueError('scale must be finite (fp32) and >= 0')
+    if not 0 <= scale <= _KV_MAX_SCALE:
+        raise ValueError('scale must be 0 to 2^16')
     k = _NO_ROWS if k is None else _kv_rows(k, 'k', cache, cache.kv_heads, seq, keep, copy)[0]
     v = _NO_ROWS if v is None else _kv_rows(v, 'v', cache, cache.kv_heads, seq, keep, copy)[0]
     a = KVAttentionArgs.from_buffer_copy(cache._heads[KVAttentionArgs] + _KV_ATTENTION.pack(
@@ -1314,7 +1320,8 @@ def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, sca
     keep = []
     a, need = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, keep, True)
     if need:
-        a.workspace, a.workspace_bytes = _kv_workspace(need, cache.device).data_ptr(), need
+        workspace = _kv_workspace(need, cache.device)   # (held until the call is enqueued, whoever replaces it)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
     _kv_run(library().lb_kv_attention, a, cache.device, 'lb_kv_attention')
     return out
 
