@@ -996,10 +996,18 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
       raw[RAW + u] = *reinterpret_cast<const u4 *>(vc + at + 16 * (tid + 256 * u));
     }
   };
-  // Keys: rows of D, 8 dims a piece.  Values: rows of 64 slots by dim, piece 2 s + f holding what lane half f takes in K
-  // step s: slots 16 s + 4 f .. + 3 and 16 s + 8 + 4 f .. + 3.
-  auto key_at = [&](int slot, int piece) { return slot * (2 * D) + (piece ^ (slot & (D == 64 ? 7 : 15))) * 16; };
-  auto value_at = [&](int dim, int piece) { return KBYTES + dim * (2 * kKvBlock) + (piece ^ (dim & 7)) * 16; };
+  // Keys: rows of D, 8 dims a piece; row m of the 32 that a product takes is slot 16 (m / 8) + m % 8, and 8 more in the
+  // second product: the 8 probabilities that a lane then has for K step s are those of 8 consecutive codes of a value row.
+  // Values: rows of 64 slots by dim, piece 2 s + g for lane half g.  LDS moves 16 lanes' pieces a cycle where they lie in
+  // 16 different columns of its 256 bytes: pieces are swizzled so that consecutive lanes' are, written and read.
+  auto key_at = [&](int slot, int piece) {
+    const int turn = D == 64 ? ((slot >> 1 & 3) | (slot >> 2 & 4)) ^ (slot & 1) : piece >> 3 ^ (slot & 7) ^ (slot >> 1 & 8);
+    return slot * (2 * D) + (piece ^ turn) * 16;
+  };
+  auto value_at = [&](int dim, int piece) {
+    const int turn = ((dim & 2) | (dim >> 2 & 1) | (dim >> 1 & 4)) ^ (dim & 1) << 1;
+    return KBYTES + dim * (2 * kKvBlock) + (piece ^ turn) * 16;
+  };
   auto stage = [&](int block) {
     if (block >= stop) return;
     uint8_t *const to = mem + (block & 1) * BYTES;
@@ -1010,13 +1018,10 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           *reinterpret_cast<h8 *>(to + key_at(slot, piece + e)) = kv_decode8<FMT>(raw[u][2 * e], raw[u][2 * e + 1]);
-        const int dim = at / 4, f = at % 4;    // places 16 f ..: slots 16 s + 4 f ..
+        const int dim = at / 4, f = at % 4;    // places 16 f ..: slots 16 i + 4 f ..
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const h8 v = kv_decode8<FMT>(raw[RAW + u][2 * e], raw[RAW + u][2 * e + 1]);
-          *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-          *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + 2 + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
-        }
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<h8 *>(to + value_at(dim, 4 * (f >> 1) + 2 * e + (f & 1))) = kv_decode8<FMT>(raw[RAW + u][2 * e], raw[RAW + u][2 * e + 1]);
       }
     } else {                              // fp16 rows (values as in kv_attend_kernel: finite, whatever lies there)
       const size_t half = (2 * bh + (block & 1)) * (kKvBlock * D);
@@ -1028,9 +1033,8 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
         *reinterpret_cast<h8 *>(to + key_at(at / (D / 8), at % (D / 8))) = kv_order8<FMT>(*reinterpret_cast<const h8 *>(p.c.kt + half + 8 * at));
         const int dim = at / 8, f = at / 2 % 4, e = at % 2;
         const h8 x = *reinterpret_cast<const h8 *>(p.c.vt + half + 8 * at);
-        const h8 v = kv_order8<FMT>(__builtin_elementwise_min(__builtin_elementwise_max(x, -hi), hi));
-        *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 0, 1, 2, 3);
-        *reinterpret_cast<h4 *>(to + value_at(dim, 4 * e + 2 + (f & 1)) + 8 * (f >> 1)) = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        *reinterpret_cast<h8 *>(to + value_at(dim, 4 * (f >> 1) + 2 * e + (f & 1))) =
+            kv_order8<FMT>(__builtin_elementwise_min(__builtin_elementwise_max(x, -hi), hi));
       }
     }
   };
@@ -1077,7 +1081,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int a = 0; a < 2; ++a)
-          s[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + key_at(32 * a + j, 2 * k + g)), q[k], s[a], 0, 0, 0);
+          s[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + key_at(16 * (j >> 3) + 8 * a + (j & 7), 2 * k + g)), q[k], s[a], 0, 0, 0);
       __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -1085,6 +1089,14 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       }
       __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
+      // Where the values' operands lie, settled before the block of the second product (in it the compiler puts these
+      // operations, and with them the reads, behind the exponentials).
+      uint32_t value_from[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        value_from[k] = (block & 1) * BYTES + value_at(j, 2 * k + g);
+        asm volatile("" : "+v"(value_from[k]));
+      }
       float shift = 0.0f, part = 1.0f;    // log2 of vs / unit, which the probabilities carry, and unit / vs
       if (vscale > 0.0f) {                // (a block of zeros adds nothing in any unit)
         const float ratio = unit > 0.0f ? vscale * __builtin_amdgcn_rcpf(unit) : 0.0f;
@@ -1114,7 +1126,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
         for (int a = 0; a < 2; ++a)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const int slot = base + 32 * a + 8 * (e / 4) + 4 * g + e % 4;
+            const int slot = base + 16 * (e / 4) + 8 * a + 4 * g + e % 4;
             s[a][e] = slot <= pos ? s[a][e] * kscale : -INFINITY;
             most = fmaxf(most, s[a][e]);
           }
@@ -1141,7 +1153,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
         const h8 pf = kv_order8<FMT>(x);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(from + value_at(32 * d + j, 2 * k + g)), pf, acc[d], 0, 0, 0);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8 *>(mem + value_from[k] + d * (64 * kKvBlock)), pf, acc[d], 0, 0, 0);
       }
       total = __builtin_fmaf(sum, part, total);
       // The next step's exponentials stand between a step's products.
