@@ -449,6 +449,11 @@ __device__ __forceinline__ uint32_t kv_scan(uint32_t x) {
   return x;
 }
 
+// A value that is the same in every lane, as one.
+__device__ __forceinline__ float kv_uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
+
 // The largest over the four lanes that hold a query.
 __device__ __forceinline__ float kv_max_across(float x) {
   x = fmaxf(x, __shfl_xor(x, 16));
@@ -1062,17 +1067,28 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.0f;
   float top = kKvLowest, total = 0.0f, unit = 0.0f;
 
+  // A block's scales are requested ahead of the codes of the block behind it: loads come back in order, so that they
+  // are there once those codes are (asked for when they are used, they wait for every code on its way).
+  float ksn = 1.0f, vsn = 1.0f;
+  auto fetch_scales = [&](int block) {
+    const int at = min(block, p.c.blocks - 1);
+    ksn = ks[at];
+    vsn = vs[at];
+  };
   stage(begin);
+  fetch_scales(begin);
   fetch(begin + 1);
   __syncthreads();
   for (int block = begin; block < stop; ++block) {
     stage(block + 1);
+    const float ksb = kv_uniform(ksn), vsb = kv_uniform(vsn);
+    fetch_scales(block + 1);
     fetch(block + 2);
     const int base = block * kKvBlock;
     if (base <= high && mine < rows) {
       const uint8_t *const from = mem + (block & 1) * BYTES;
       const bool open = block >= closed;
-      const float kscale = open ? p.scale : p.scale * ks[block], vscale = open ? 1.0f : vs[block];
+      const float kscale = open ? p.scale : p.scale * ksb, vscale = open ? 1.0f : vsb;
       // Eight operands of each product are read ahead: a read is 100 cycles and more from its use, a product 32.
       f16x s[2];
 #pragma unroll
