@@ -269,7 +269,10 @@ struct KvAppendParams {
 
 // One workgroup of 2 D threads per block of 64 slots that new rows fall into, KV head and sequence.  A block that
 // becomes full takes its older rows from the tails; rows of the last block and of the one before it go to the tails.
-// Bound by memory for prompts, by its launch and one chain of loads for single tokens.
+// Each thread holds 8 dims of 4 slots, so that a block is read once, in 16-byte pieces, and a value's 4 slots are one
+// dword of the turned codes.  Bound by memory for prompts (4 x 4100 rows, 8 heads of 128, fp8: 101 MB in 18.0 us,
+// 5.6 TB/s), by its launch and one chain of loads for single tokens (64 sequences, 3 heads of 64: 4.8 us, 6.0 where
+// blocks become full).
 template <int FMT, int D>
 __global__ __launch_bounds__(2 * D) void kv_append_kernel(KvAppendParams p) {
   __shared__ KvTurn<D> turn;
@@ -342,7 +345,7 @@ struct KvReadParams {
 
 // One workgroup of 2 D threads per block, KV head and sequence.  Keys are decoded where they lie, 8 dims of 4 slots a
 // thread; value codes are fetched 16 bytes at a time and turned into rows by slot through LDS.  Bound by memory: of
-// 3 bytes moved per value, two are written.
+// 3 bytes moved per value, two are written (131000 slots, 8 heads of 128, int8: 805 MB in 140 us, 5.7 TB/s).
 template <int FMT, int D>
 __global__ __launch_bounds__(2 * D) void kv_read_kernel(KvReadParams p) {
   constexpr int CH = D / 8, PITCH = 20;
@@ -551,6 +554,8 @@ __device__ __forceinline__ void kv_join(__amdgpu_buffer_rsrc_t po, __amdgpu_buff
 //   - Longer sequences first, and every other 256 workgroups backwards, so that the two that share a CU have together what
 //     others have: the same 64 sequences 100 us (5.4 TB/s) against 118 in the batch's order.  (Up to 64 sequences, by
 //     prefix sums in registers; sorting them outright took 50 ns a sequence.)
+//   - At 5 TB/s and more the loads in flight are what HBM takes; short ones are bound by the chain of position, codes, two
+//     products and the join: 4.1 us for one sequence of 150 slots and 3 heads of 64, 12.5 for 32 of 1984 with the append.
 //
 // Scores are K.Q^T and outputs V^T.P^T, so that a lane holds one query throughout (column lane % 16): its maximum,
 // total and rescaling are the lane's own, and the probabilities that it computes are the B operand of the second product
@@ -954,8 +959,15 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
 // query (column lane % 32) and its probabilities are the B operand as they are.  The block's value scale would cost an
 // operation per output and block as a factor of the fp32 sums; instead the sums are kept in units of `unit`, a recent
 // block's scale, and the ratio vs / unit enters the exponent of the probabilities, whose total is divided by it once per
-// block.  A block whose ratio is past 4 either way sets the unit anew.  What bounds it: per 64 slots and wave D / 2 MFMA (32 cycles each at peak) against 32 exponentials and about 100
-// other vector operations a lane.
+// block.  A block whose ratio is past 4 either way sets the unit anew.
+//
+// What bounds it: of the cycles of a CU the matrix cores are busy 46% and the vector units 54% (per 64 slots and wave
+// D / 4 products of 32 cycles and, a lane, 32 exponentials at a quarter of the rate and some 150 other operations), which
+// two waves a SIMD overlap little.  8192 rows of 32 query and 8 KV heads of 128, fp8:
+// 575 us, 957 TFLOP/s; 509 rows over 32768 more slots 321 us; 8 x 500 rows, 9 and 3 heads of 64: 13.4 us.  Measured on
+// the way: bank conflicts on a fifth of the cycles before the pieces' layout (620 us), scales asked for where they are
+// used (598 against 588).  Not kept: the next block's scores beside this one's exponentials (721 against 620, for want of
+// registers), 256 rows a workgroup (606 against 615, but 64 rows 45 us against 36).
 template <int FMT, int D>
 __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
   constexpr int R = 128, KS = D / 16, DT = D / 32, RAW = D / 64, DQ = D / 4;
