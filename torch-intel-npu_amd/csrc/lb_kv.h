@@ -270,8 +270,8 @@ struct KvAppendParams {
 // One workgroup of 2 D threads per block of 64 slots that new rows fall into, KV head and sequence.  A block that
 // becomes full takes its older rows from the tails; rows of the last block and of the one before it go to the tails.
 // Each thread holds 8 dims of 4 slots, so that a block is read once, in 16-byte pieces, and a value's 4 slots are one
-// dword of the turned codes.  Bound by memory for prompts (4 x 4100 rows, 8 heads of 128, fp8: 101 MB in 18.0 us,
-// 5.6 TB/s), by its launch and one chain of loads for single tokens (64 sequences, 3 heads of 64: 4.8 us, 6.0 where
+// dword of the turned codes.  Bound by memory for prompts (four prompts of up to 4100 rows, 8 heads of 128, fp8: 69 MB
+// in 18.0 us, 3.8 TB/s), by its launch and one chain of loads for single tokens (64 sequences, 3 heads of 64: 4.8 us, 6.0 where
 // blocks become full).
 template <int FMT, int D>
 __global__ __launch_bounds__(2 * D) void kv_append_kernel(KvAppendParams p) {
