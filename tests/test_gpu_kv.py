@@ -702,3 +702,46 @@ def test_two_graphs_of_plain_calls(device):
         for (_, out), m, w in zip(graphs, made, want):
             assert torch.equal(out, w) and torch.equal(call(*m), w)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize('format', ['int8', 'fp8'])
+@pytest.mark.parametrize('heads,kv_heads,dim,seq', [(8, 2, 128, 1), (20, 1, 128, 1), (20, 1, 64, 1), (32, 1, 128, 1), (4, 1, 128, 5),
+                                                    (8, 1, 128, 4), (10, 2, 128, 6), (16, 2, 64, 4)])
+def test_attention_of_wide_groups_appends(device, format, heads, kv_heads, dim, seq):
+    """Up to 32 rows of a KV head, either head size, rows that fill a block in the same call, short and split sequences."""
+    announce('kv attention wide groups', format, heads, kv_heads, dim, seq)
+    starts, capacity = [63, 0, 130, 2879, 255, 64 - seq], 2944
+    batch, total = len(starts), capacity
+    k, v = rows_of(140, batch, total, kv_heads, dim), rows_of(141, batch, total, kv_heads, dim, spread=.3)
+    q = rows_of(142, batch, seq, heads, dim)
+    cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device), rows=ints(starts, device))
+    new = [dev(np.stack([x[b, s:s + seq] for b, s in enumerate(starts)]), device) for x in (k, v)]
+    twin = cache.clone()
+    out = lb.kv_attention(dev(q, device), cache, ints(starts, device), k=new[0], v=new[1])
+    lb.kv_append(twin, new[0], new[1], ints(starts, device))
+    assert torch.equal(out, lb.kv_attention(dev(q, device), twin, ints(starts, device)))
+    for a, b in zip(cache.tensors(), twin.tensors()):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    worst = check_attention(out, q, k, v, starts, [seq] * batch, format, dim ** -0.5, kv_heads)
+    print(f'[kv attention] wide groups {format} {heads}/{kv_heads} {dim} {seq}: {worst:.2f} of the bound', flush=True)
+
+
+@pytest.mark.parametrize('format', ['int8', 'fp8'])
+@pytest.mark.parametrize('heads,kv_heads,dim,seq', [(3, 1, 64, 70), (2, 1, 128, 133), (33, 1, 128, 1), (8, 2, 64, 40)])
+def test_attention_of_chunks_in_parts(device, format, heads, kv_heads, dim, seq):
+    """Chunks of a prompt behind thousands of slots beside short ones and a padded one: a tile's slots in many parts."""
+    announce('kv attention chunks', format, heads, kv_heads, dim, seq)
+    starts, capacity = [2500, 0, 1090], 2688
+    rows = [seq, seq, max(1, seq // 2)]
+    batch = len(starts)
+    k, v = rows_of(150, batch, capacity, kv_heads, dim), rows_of(151, batch, capacity, kv_heads, dim, spread=.3)
+    q = rows_of(152, batch, seq, heads, dim)
+    cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device),
+                 rows=ints([s + r for s, r in zip(starts, rows)], device))
+    out = torch.full((batch, seq, heads, dim), 3.0, dtype=torch.float16, device=device)
+    lb.kv_attention(dev(q, device), cache, ints(starts, device), rows=ints(rows, device), out=out)
+    assert bool((out[2, rows[2]:] == 3).all())
+    worst = check_attention(out, q, k, v, starts, rows, format, dim ** -0.5, kv_heads)
+    print(f'[kv attention] chunks {format} {heads}/{kv_heads} {dim} {seq}: {worst:.2f} of the bound', flush=True)
