@@ -1252,11 +1252,11 @@ def kv_read(cache, length, *, start=0, count=None, keys=None, values=None):
     for name, t in (('keys', keys), ('values', values)):
         if t is None:
             t = torch.zeros(shape, dtype=torch.float16, device=cache.device)
-        elif not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or tuple(t.shape) != shape or t.device != cache.device:
+        elif not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.shape != shape or t.device != cache.device:
             raise ValueError(f'{name} must be fp16 {list(shape)} on {cache.device}')
         b, h, i, d = t.stride()
         at = t.data_ptr()
-        if d != 1 or at % 16 or any(s % 8 and n > 1 for s, n in zip((b, h, i), shape)):
+        if d != 1 or at % 16 or ((b | h | i) % 8 and any(s % 8 and n > 1 for s, n in zip((b, h, i), shape))):
             raise ValueError(f'the rows of {name} must be 16-byte pieces')
         outs.append(t)
         rows += (at, b, i, h)
