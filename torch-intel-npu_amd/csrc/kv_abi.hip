@@ -165,7 +165,7 @@ struct AttendPlan {
 };
 static_assert(kKvTickets * 4 == LB_ZEROED_WORKSPACE_BYTES, "tickets are the workspace's zeroed bytes");
 
-constexpr int kCus = 256;
+constexpr int kCus = 256, kKvAlone = 6;   // the CUs; parts of a tile from which they are held to one a CU
 
 AttendPlan attend_plan(const lb_kv_attention_args *a) {
   AttendPlan plan{};
@@ -178,10 +178,15 @@ AttendPlan attend_plan(const lb_kv_attention_args *a) {
   if (plan.prompt) {
     height = 128;
     plan.tiles = (int)((rows + 127) / 128);
-    // Parts only where there are not tiles enough for two workgroups on each CU, of eight blocks at the least.
-    const int64_t units = pairs * plan.tiles;
-    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * kCus / units, (c.capacity / kKvBlock + 7) / 8));
-    plan.grid = units * plan.splits;     // (at most 2 * kCus where there are parts: the tickets are enough)
+    // Parts only where there are not tiles enough for the workgroups that fit on the CUs, of kKvChunk blocks at the least
+    // (4096 rows, 9 and 3 heads of 64: 52 us for three a CU, 74 for two; 509 rows over 32768 slots, 32 and 8 heads of 128,
+    // of which two fit: 327 us, 350 for three).  Where one a CU makes kKvAlone parts of a tile there are no more: a part
+    // costs the workgroup that adds them as much as a block or two, and CUs that have two set the pace (64 rows over 30000
+    // slots, 32 and 8 heads of 128: 16 parts 82 us, 18 to 21 parts 111, 32 parts 122; 4 x 100 rows over 8000, 9 and 3 heads
+    // of 64: 7 parts 33 us, 21 parts 46; but 256 rows over 30000: 4 parts 208 us, 8 parts 182).
+    const int64_t units = pairs * plan.tiles, fit = (c.head_dim == 64 ? 3 : 2) * kCus, alone = kCus / units;
+    plan.splits = (int)std::max<int64_t>(1, std::min<int64_t>(alone >= kKvAlone ? alone : fit / units, (c.capacity / kKvBlock + kKvChunk - 1) / kKvChunk));
+    plan.grid = units * plan.splits;     // (at most 3 * kCus where there are parts: the tickets are enough)
     parts = plan.splits > 1 ? (size_t)plan.grid : 0;
   } else {
     // A workgroup per sequence and KV head, and where they can be long enough as many again as they can be split into.

@@ -437,6 +437,7 @@ constexpr float kKvLowest = -1e30f;   // a running maximum below every score (sc
 // kKvSlack (in units of log2): fp16 then has them in [2^-24, 2^14], of which the smallest are 2^-34 of the largest.
 constexpr float kKvLift = 10.0f, kKvSlack = 4.0f;
 constexpr int kKvTickets = 1024;      // (LB_ZEROED_WORKSPACE_BYTES)
+constexpr int kKvChunk = 8;           // kv_prompt_kernel: blocks of a part at the least
 // kv_attend_kernel: parts that the whole work is split into at the most, besides those that sequences and heads are by
 // themselves (the CUs); blocks of a part at the least (one a wave); and places for the sums of parts.
 constexpr int kKvSplit = 256, kKvLeast = 4, kKvPlaces = 2 * kKvSplit + 2;
@@ -478,14 +479,69 @@ __device__ __forceinline__ bool kv_last_part(uint32_t *ticket, uint32_t parts, u
 }
 
 // Adds the parts of `rows` rows of D sums, part k in place(k) of po [..][R][D] and pm [..][R][2], and stores the
-// quotients.  Few rows: their quads of dims times as many runs of parts as there are threads for, which meet in LDS
-// (`met`, 24 bytes a thread); the order of the additions depends on sizes alone.
+// quotients.  Many rows: a thread has four quads of dims and four parts of each in flight (509 rows over 32768 slots, four
+// parts of 128 rows of 128: 330 -> 322 us; 1024 rows of heads of 64 in two parts 23 -> 19).  Few rows: their quads of
+// dims times as many runs of parts as there are threads for, which meet in LDS (`met`, 24 bytes a thread).  The order of
+// the additions depends on sizes alone.
 template <int R, int D, int NT, class Place, class Store>
 __device__ __forceinline__ void kv_join(__amdgpu_buffer_rsrc_t po, __amdgpu_buffer_rsrc_t pm, int rows, uint32_t parts, Place &&place,
                                         f4 *met, Store &&store) {
   constexpr int DQ = D / 4, HELD = 8;     // parts in flight
   constexpr int kOutOfRange = (int)0x80000000u;
   const int tid = threadIdx.x, items = rows * DQ, runs = max(1, NT / items);
+  if constexpr (R > 32) {                 // many rows: four a thread at once, four parts of each in flight
+    constexpr int U = 4, PARTS = 4;
+    if (runs == 1) {
+      for (int at = tid; at < items; at += U * NT) {
+        float most[U], sum[U];
+        f4 o[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          most[u] = kKvLowest;
+          sum[u] = 0.0f;
+          o[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (uint32_t i = 0; i < parts; i += PARTS) {
+          f4 part[U][PARTS];
+          u2v ml[U][PARTS];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int item = at + u * NT, r = item / DQ, d = item % DQ * 4;
+#pragma unroll
+            for (int e = 0; e < PARTS; ++e) {
+              const bool there = i + e < parts && item < items;
+              const uint32_t s = place(i + e);
+              part[u][e] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(po, there ? (int)((s * R + r) * D + d) * 4 : kOutOfRange, 0, kSysCoherent));
+              ml[u][e] = __builtin_amdgcn_raw_buffer_load_b64(pm, there ? (int)(s * R + r) * 8 : kOutOfRange, 0, kSysCoherent);
+            }
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float raised = most[u], top[PARTS];
+#pragma unroll
+            for (int e = 0; e < PARTS; ++e) {
+              top[e] = i + e < parts ? __builtin_bit_cast(float, (uint32_t)ml[u][e][0]) : kKvLowest;
+              raised = fmaxf(raised, top[e]);
+            }
+            const float shrink = __builtin_amdgcn_exp2f(most[u] - raised);
+            most[u] = raised;
+            sum[u] *= shrink;
+            o[u] *= shrink;
+#pragma unroll
+            for (int e = 0; e < PARTS; ++e) {
+              const float f = __builtin_amdgcn_exp2f(top[e] - raised);
+              sum[u] += f * __builtin_bit_cast(float, (uint32_t)ml[u][e][1]);
+              o[u] += f * part[u][e];
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (at + u * NT < items) store((at + u * NT) / DQ, (at + u * NT) % DQ * 4, o[u], sum[u]);
+      }
+      return;
+    }
+  }
   for (int at = 0; at < items; at += NT) {
     const int item = at + (runs > 1 ? tid % items : tid), run = runs > 1 ? tid / items : 0;
     const int r = item / DQ, d = item % DQ * 4;
@@ -995,7 +1051,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
   }
   const int closed = (first + count) / kKvBlock;
   const int blocks = (first + (tile * R + rows - 1) / p.group) / kKvBlock + 1;   // blocks that the last row sees some of
-  const int chunk = max(8, (blocks + p.splits - 1) / p.splits), parts = (blocks + chunk - 1) / chunk;
+  const int chunk = max(kKvChunk, (blocks + p.splits - 1) / p.splits), parts = (blocks + chunk - 1) / chunk;
   if (split >= parts) return;
   const int begin = split * chunk, stop = min(blocks, begin + chunk);
   const size_t bh = (size_t)b * p.c.kv_heads + h;
