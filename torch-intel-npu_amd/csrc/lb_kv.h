@@ -1020,7 +1020,7 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
 // What bounds it: of the cycles of a CU the matrix cores are busy 46% and the vector units 54% (per 64 slots and wave
 // D / 4 products of 32 cycles and, a lane, 32 exponentials at a quarter of the rate and some 150 other operations), which
 // two waves a SIMD overlap little.  8192 rows of 32 query and 8 KV heads of 128, fp8:
-// 575 us, 957 TFLOP/s; 509 rows over 32768 more slots 321 us; 8 x 500 rows, 9 and 3 heads of 64: 13.4 us.  Measured on
+// 575 to 579 us, 950 TFLOP/s; 509 rows over 32768 slots 318 us; 8 x 500 rows, 9 and 3 heads of 64: 13.6 us.  Measured on
 // the way: bank conflicts on a fifth of the cycles before the pieces' layout (620 us), scales asked for where they are
 // used (598 against 588).  Not kept: the next block's scores beside this one's exponentials (721 against 620, for want of
 // registers), 256 rows a workgroup (606 against 615, but 64 rows 45 us against 36).
