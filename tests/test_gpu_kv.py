@@ -728,7 +728,8 @@ def test_attention_of_wide_groups_appends(device, format, heads, kv_heads, dim, 
 
 
 @pytest.mark.parametrize('format', ['int8', 'fp8'])
-@pytest.mark.parametrize('heads,kv_heads,dim,seq', [(3, 1, 64, 70), (2, 1, 128, 133), (33, 1, 128, 1), (8, 2, 64, 40)])
+@pytest.mark.parametrize('heads,kv_heads,dim,seq', [(3, 1, 64, 70), (2, 1, 128, 133), (33, 1, 128, 1), (8, 2, 64, 40),
+                                                    (1, 1, 64, 129), (1, 1, 128, 131)])
 def test_attention_of_chunks_in_parts(device, format, heads, kv_heads, dim, seq):
     """Chunks of a prompt behind thousands of slots beside short ones and a padded one: a tile's slots in many parts."""
     announce('kv attention chunks', format, heads, kv_heads, dim, seq)
