@@ -436,6 +436,10 @@ constexpr float kKvLowest = -1e30f;   // a running maximum below every score (sc
 // Probabilities are 2^kKvLift above 1 at a row's running maximum, which is raised where a score exceeds it by more than
 // kKvSlack (in units of log2): fp16 then has them in [2^-24, 2^14], of which the smallest are 2^-34 of the largest.
 constexpr float kKvLift = 10.0f, kKvSlack = 4.0f;
+// The lift minus the maximum is one addend of a block's scores, which is off by half a step of the maximum: by 2^-15 here,
+// in a probability an eighth of its rounding to fp16, but by the whole lift from 2^27 on.  So a maximum further from zero
+// than this is subtracted from the scores first (0 to 1.5% of a call for asking).
+constexpr float kKvFar = 1024.0f;
 constexpr int kKvTickets = 1024;      // (LB_ZEROED_WORKSPACE_BYTES)
 constexpr int kKvChunk = 8;           // kv_prompt_kernel: blocks of a part at the least
 // kv_attend_kernel: parts that the whole work is split into at the most, besides those that sequences and heads are by
@@ -895,7 +899,7 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = fmaxf(most, s[t][i][e]);
-      if (__any(most > top[t] + kKvSlack)) {
+      if (__any(most - top[t] > kKvSlack)) {   // (a sum with the slack could round to a step of the maximum more)
         const float raised = fmaxf(top[t], kv_max_across(most));
         const float shrink = __builtin_amdgcn_exp2f(top[t] - raised);
         top[t] = raised;
@@ -903,7 +907,14 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[t][d] *= shrink;
       }
-      const float bias = kKvLift - top[t];
+      float bias = kKvLift - top[t];
+      if (__any(fabsf(top[t]) > kKvFar)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[t][i][e] -= top[t];
+        bias = kKvLift;
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         h8 x;
@@ -1216,7 +1227,7 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
           }
         factor = 1.0f;
       }
-      if (__any(most > top + kKvSlack)) {
+      if (__any(most - top > kKvSlack)) {
         const float raised = fmaxf(top, fmaxf(most, __shfl_xor(most, 32)));
         const float shrink = __builtin_amdgcn_exp2f(top - raised);
         top = raised;
@@ -1224,7 +1235,16 @@ __global__ __launch_bounds__(256, 2) void kv_prompt_kernel(KvAttendParams p) {
 #pragma unroll
         for (int d = 0; d < DT; ++d) acc[d] *= shrink;
       }
-      const float bias = kKvLift - 1.0f + shift - top;   // (at most 2^15 with the ratio's 2^2)
+      float bias = kKvLift - 1.0f + shift - top;   // (at most 2^15 with the ratio's 2^2)
+      if (__any(fabsf(top) > kKvFar)) {
+#pragma clang fp contract(off)            // (products rounded as the maximum was)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[a][e] = s[a][e] * factor - top;
+        factor = 1.0f;
+        bias = kKvLift - 1.0f + shift;
+      }
       float sum = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
