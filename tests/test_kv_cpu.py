@@ -314,3 +314,32 @@ def test_the_buffers_are_fixed():
         packed = bytes(twin._heads[lb.KVReadArgs])
         assert twin.key_codes.data_ptr().to_bytes(8, 'little') in packed
         assert cache.key_codes.data_ptr().to_bytes(8, 'little') not in packed
+
+
+# Sizes whose products pass 64 bits: a cache of 2^64 bytes, rows of 2^24 + 1 strides of 2^40 elements (2^65 bytes and a row).
+APART = {name: (1 + i) << 56 for i, name in enumerate((
+    'cache__key_codes', 'cache__value_codes', 'cache__key_scales', 'cache__value_scales', 'cache__key_tail', 'cache__value_tail',
+    'position'))}
+VAST = dict(APART, cache__head_dim=128, cache__batch=1 << 14, cache__kv_heads=1 << 15, cache__capacity=1 << 28)
+BEYOND = [
+    ('lb_kv_append', append, dict(VAST, k__data=8 << 56, v__data=9 << 56)),
+    ('lb_kv_read', read, {**{k: v for k, v in VAST.items() if k != 'position'}, 'keys__data': 8 << 56, 'values__data': 9 << 56,
+                          'keys__batch_stride': 1 << 40, 'keys__head_stride': 1 << 20, 'values__batch_stride': 1 << 40,
+                          'values__head_stride': 1 << 20}),
+    ('lb_kv_append', append, dict(seq=(1 << 24) + 1, k__row_stride=1 << 40, k__data=1 << 56, v__data=2 << 56)),
+    ('lb_kv_append', append, dict(seq=(1 << 24) + 1, v__row_stride=1 << 40, v__data=1 << 56, k__data=2 << 56)),
+    ('lb_kv_read', read, dict(APART, cache__batch=1, cache__capacity=1 << 28, start=0, count=(1 << 24) + 1, keys__row_stride=1 << 40,
+                              values__head_stride=1 << 40, keys__data=8 << 56, values__data=9 << 56)),
+    ('lb_kv_attention', attention, dict(cache__batch=1, seq=(1 << 24) + 1, q__row_stride=1 << 40, q__data=1 << 56, out__data=2 << 56)),
+    ('lb_kv_attention', attention, dict(cache__batch=1, seq=(1 << 24) + 1, out__row_stride=1 << 40, out__data=1 << 56,
+                                        q__data=2 << 56)),
+]
+BEYOND[4][2].pop('position')
+
+
+@pytest.mark.parametrize('entry,make,over', BEYOND, ids=[f'{entry}-{i}' for i, (entry, _, _) in enumerate(BEYOND)])
+def test_sizes_past_the_address_space_are_refused(entry, make, over):
+    """Every range is computed without overflow: what no memory can hold is refused, not taken for a short range."""
+    lib = lb.library()
+    assert getattr(lib, entry)(ctypes.byref(make(**over)), None) == lb.INVALID_ARGUMENT, lib.lb_last_error().decode()
+    assert 'address space' in lib.lb_last_error().decode()

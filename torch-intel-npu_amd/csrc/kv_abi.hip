@@ -14,6 +14,7 @@ using namespace lb::abi;
 namespace {
 
 constexpr int64_t kMaxCapacity = (int64_t)1 << 28, kMaxStride = (int64_t)1 << 40, kMaxRows = (int64_t)1 << 28;
+constexpr size_t kMaxBytes = (size_t)1 << 60;   // (no buffer is larger; sums of a few stay in 64 bits)
 constexpr float kMaxScale = 65536.0f;   // |q| and |k| are below 2^16, so scores stay within 2^56
 
 KvCache cache_params(const lb_kv_cache &c) {
@@ -41,8 +42,11 @@ lb_status check_cache(const char *what, const lb_kv_cache &c, Range (&r)[6]) {
   if (c.batch < 1 || c.batch > 65535 || c.kv_heads < 1 || c.kv_heads > 65535 || c.capacity < kKvBlock || c.capacity > kMaxCapacity ||
       c.capacity % kKvBlock != 0)
     return fail(LB_INVALID_ARGUMENT, "%s: batch and kv_heads 1..65535, capacity a multiple of %d up to 2^28 required", what, kKvBlock);
-  const size_t heads = (size_t)c.batch * c.kv_heads, codes = heads * c.capacity * c.head_dim, scales = heads * (c.capacity / kKvBlock) * 4,
-               tail = heads * (2 * kKvBlock) * c.head_dim * 2;   // (below 2^32 * 2^35 bytes)
+  const size_t heads = (size_t)c.batch * c.kv_heads;
+  if (heads > kMaxBytes / ((size_t)c.capacity * c.head_dim))
+    return fail(LB_INVALID_ARGUMENT, "%s: the cache's codes do not fit the address space", what);
+  const size_t codes = heads * c.capacity * c.head_dim, scales = heads * (c.capacity / kKvBlock) * 4,
+               tail = heads * (2 * kKvBlock) * c.head_dim * 2;   // (heads below 2^32, so scales below 2^56, tails 2^47)
   r[0] = range_of(c.key_codes, codes, "key_codes");
   r[1] = range_of(c.value_codes, codes, "value_codes");
   r[2] = range_of(c.key_scales, scales, "key_scales");
@@ -63,14 +67,14 @@ lb_status check_rows(const char *what, const char *name, const lb_kv_rows &v, in
                      bool written, Range &range) {
   if (!v.data || !aligned(v.data, 16)) return fail(LB_INVALID_ARGUMENT, "%s: %s must be non-NULL with 16-byte alignment", what, name);
   struct Axis { int64_t size, stride; } axes[3] = {{batch, v.batch_stride}, {seq, v.row_stride}, {heads, v.head_stride}};
-  int64_t span = dim;
+  unsigned __int128 span = dim;
   for (Axis &a : axes) {
     if (a.size == 1) a.stride = 0;
     if (a.stride < 0 || a.stride > kMaxStride || a.stride % 8 != 0)
       return fail(LB_INVALID_ARGUMENT, "%s: strides of %s must be multiples of 8, 0 to 2^40 elements", what, name);
-    span += (a.size - 1) * a.stride;   // (below 2^28 * 2^40 * 3)
+    span += (unsigned __int128)(a.size - 1) * a.stride;   // (up to 2^28 * 2^40 each)
   }
-  if (span > INT64_MAX / 4) return fail(LB_INVALID_ARGUMENT, "%s: %s is past the address space", what, name);
+  if (span > kMaxBytes / 2) return fail(LB_INVALID_ARGUMENT, "%s: %s is past the address space", what, name);
   if (written) {
     std::sort(axes, axes + 3, [](const Axis &a, const Axis &b) { return a.stride < b.stride; });
     int64_t extent = dim;
