@@ -312,8 +312,10 @@ lb_status lb_layer_rows(const lb_layer_rows_args *args, void *stream);
  *   LB_KV_FP8    scale = a / 448,         code = e4m3(448 x / a), to even (OCP e4m3fn)
  * and a code stands for code * scale.  A block is quantised once, when its last row arrives; until then, and until
  * the block after it is full too, its rows are held in fp16 in a ring of two blocks (slot mod 128).  So nothing is
- * ever quantised twice, the held values do not depend on how the rows were split into calls, and positions may be taken
- * back (drafted tokens that were rejected) as far as the start of the block before the one that is open.
+ * ever quantised twice, and the held values do not depend on how the rows were split into calls.
+ * Positions may be taken back (drafted tokens that were rejected, a new sequence in place of an old one): to the start of
+ * any block, and to a slot inside block i (slots 64 i ..) as long as the sequence, since slot 64 i was last appended, has
+ * never held 64 (i + 2) slots, rejected ones counted.  From then on the ring has other rows in that block's place.
  * A row with a key or value that is not finite gets a key of NaNs, and a block with one NaN scales: the rows that
  * attend to it are NaN, others are not.
  * Layouts, per sequence and KV head (row-major; D = head_dim, blocks = capacity / 64):

@@ -746,3 +746,41 @@ def test_attention_of_chunks_in_parts(device, format, heads, kv_heads, dim, seq)
     assert bool((out[2, rows[2]:] == 3).all())
     worst = check_attention(out, q, k, v, starts, rows, format, dim ** -0.5, kv_heads)
     print(f'[kv attention] chunks {format} {heads}/{kv_heads} {dim} {seq}: {worst:.2f} of the bound', flush=True)
+
+
+@pytest.mark.parametrize('format,dim,seed', [('int8', 64, 0), ('fp8', 64, 1), ('int8', 128, 2)])
+def test_positions_taken_back_again_and_again(device, format, dim, seed):
+    """Appends of one to 150 rows and positions taken back, as far as the header allows, over and over: to the start of any
+    block, and into a block whose rows the ring has yet.  What is held is at every stage what the rows say, bit for bit."""
+    announce('kv taken back again', format, dim, seed)
+    batch, heads, capacity, steps = 3, 1, 640, 60
+    rng = np.random.default_rng(160 + seed)
+    cache = fresh(device, batch, heads, capacity, dim, format, fill=0x7F)
+    k, v = (np.zeros((batch, capacity, heads, dim), np.float16) for _ in range(2))
+    length, most = [0] * batch, [{} for _ in range(batch)]   # most[b][i]: slots held at the most since slot 64 i was appended
+    inside = 0
+    for step in range(steps):
+        rows, seq = [], 150
+        for b in range(batch):
+            if length[b] and rng.random() < 0.6:             # taken back
+                may = [p for p in range(length[b] + 1) if p % 64 == 0 or most[b][p // 64] < 64 * (p // 64 + 2)]
+                to = int(rng.choice(may[-100:])) if rng.random() < 0.8 else int(rng.choice(may))
+                inside += to % 64 != 0 and to // 64 < length[b] // 64
+                length[b] = to
+            rows.append(min(capacity - length[b], int(rng.choice([0, 1, 2, rng.integers(1, 20), rng.integers(1, seq + 1)]))))
+        new = [rows_of(1000 * seed + 2 * step + i, batch, seq, heads, dim) for i in range(2)]
+        lb.kv_append(cache, dev(new[0], device), dev(new[1], device), ints(length, device), rows=ints(rows, device))
+        for b in range(batch):
+            start, end = length[b], length[b] + rows[b]
+            for t, x in zip((k, v), new):
+                t[b, start:end] = x[b, :rows[b]]
+            for i in range((start + 63) // 64, (end + 63) // 64):
+                most[b][i] = 0                               # its first slot is among these rows
+            most[b] = {i: max(n, end) for i, n in most[b].items()}
+            length[b] = end
+        got = lb.kv_read(cache, ints(length, device))
+        for g, t in zip(got, (k, v)):
+            g = g.cpu().numpy()
+            for b in range(batch):
+                same(g[b, 0, :length[b]], ko.read(t[b, :length[b], 0], format))
+    assert inside >= 5, inside
