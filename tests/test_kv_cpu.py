@@ -343,3 +343,29 @@ def test_sizes_past_the_address_space_are_refused(entry, make, over):
     lib = lb.library()
     assert getattr(lib, entry)(ctypes.byref(make(**over)), None) == lb.INVALID_ARGUMENT, lib.lb_last_error().decode()
     assert 'address space' in lib.lb_last_error().decode()
+
+
+class Cleared(torch.utils._python_dispatch.TorchDispatchMode):
+    """Bytes that operations under it fill with zeros."""
+    bytes = 0
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        out = func(*args, **(kwargs or {}))
+        if any(word in func.__name__ for word in ('zero', 'fill')):
+            self.bytes += out.numel() * out.element_size()
+        return out
+
+
+@pytest.mark.parametrize('captured', [True, False])
+def test_a_workspace_is_cleared_no_further_than_its_counters(monkeypatch, captured):
+    """The sums of parts behind LB_ZEROED_WORKSPACE_BYTES are written before they are read; a captured call's fill is
+    repeated by every replay."""
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: captured)
+    monkeypatch.setattr(lb, '_raw_stream', lambda device: 0)
+    monkeypatch.setattr(lb, '_kv_workspaces', {})
+    with Cleared() as cleared:
+        workspace = lb._kv_workspace(5 << 20, torch.device('cpu'))
+    assert workspace.numel() >= 5 << 20 and not bool(workspace[:4096].any())
+    assert cleared.bytes == 4096
+    again = lb._kv_workspace(1 << 20, torch.device('cpu'))
+    assert (again is workspace) is not captured

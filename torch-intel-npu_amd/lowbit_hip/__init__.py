@@ -1297,15 +1297,22 @@ def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, kee
 _kv_workspaces = {}   # by device and stream: calls on a stream are ordered, so they can share one
 
 
+def _kv_new_workspace(need, device):
+    """A workspace of lb_kv_attention, its counters zero (what lies behind them is written before it is read)."""
+    workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    workspace[:ZEROED_WORKSPACE_BYTES].zero_()
+    return workspace
+
+
 def _kv_workspace(need, device):
-    """A workspace of lb_kv_attention for a call on the device's current stream: zero once, its counters zero after every
-    call.  A call that is captured gets one of its own (cleared in the graph): replays may run on any stream."""
+    """The workspace of a call on the device's current stream: counters zero once, and zero again after every call.  A call
+    that is captured gets one of its own (its counters cleared in the graph): replays may run on any stream."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(need, dtype=torch.uint8, device=device)
+        return _kv_new_workspace(need, device)
     key = (device, _raw_stream(device))
     held = _kv_workspaces.get(key)
     if held is None or held.numel() < need:
-        held = _kv_workspaces[key] = torch.zeros(need, dtype=torch.uint8, device=device)
+        held = _kv_workspaces[key] = _kv_new_workspace(need, device)
     return held
 
 
@@ -1343,7 +1350,7 @@ class PreparedKVAttention(_PreparedKV):
         a, need = _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, None, False)
         keep = [q, cache, position, out, rows, k, v, cos, sin]
         if need:
-            keep.append(torch.zeros(need, dtype=torch.uint8, device=cache.device))
+            keep.append(_kv_new_workspace(need, cache.device))
             a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
         self._bind('lb_kv_attention', 'lb_kv_attention', a, cache.device, keep)
         self.out = out
