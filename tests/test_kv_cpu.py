@@ -369,3 +369,28 @@ def test_a_workspace_is_cleared_no_further_than_its_counters(monkeypatch, captur
     assert cleared.bytes == 4096
     again = lb._kv_workspace(1 << 20, torch.device('cpu'))
     assert (again is workspace) is not captured
+
+
+def test_whether_a_call_is_captured_is_asked_of_its_own_device(monkeypatch):
+    """The cache's device need not be the current one: its current stream is the one that may be capturing."""
+    current = [0]
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.index
+
+        def __exit__(self, *_):
+            current[0] = self.was
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: current[0])
+    monkeypatch.setattr(torch.cuda, 'device', device)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: current[0] == 1)   # a capture on device 1
+    monkeypatch.setattr(lb, '_raw_stream', lambda device: 0)
+    monkeypatch.setattr(lb, '_kv_workspaces', {})
+    monkeypatch.setattr(lb, '_kv_new_workspace', lambda need, device: torch.zeros(need, dtype=torch.uint8))
+    for index, shared in ((1, False), (0, True)):
+        first, second = (lb._kv_workspace(8192, torch.device('cuda', index)) for _ in range(2))
+        assert (first is second) is shared, index
+    assert [key[0].index for key in lb._kv_workspaces] == [0]

@@ -1297,6 +1297,14 @@ def _kv_attention_args(q, cache, position, out, rows, k, v, scale, cos, sin, kee
 _kv_workspaces = {}   # by device and stream: calls on a stream are ordered, so they can share one
 
 
+def _capturing(device):
+    """Whether the device's current stream is being captured."""
+    if device.index is None or device.index == torch._C._cuda_getDevice():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device.index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _kv_new_workspace(need, device):
     """A workspace of lb_kv_attention, its counters zero (what lies behind them is written before it is read)."""
     workspace = torch.empty(need, dtype=torch.uint8, device=device)
@@ -1307,7 +1315,7 @@ def _kv_new_workspace(need, device):
 def _kv_workspace(need, device):
     """The workspace of a call on the device's current stream: counters zero once, and zero again after every call.  A call
     that is captured gets one of its own (its counters cleared in the graph): replays may run on any stream."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(device):
         return _kv_new_workspace(need, device)
     key = (device, _raw_stream(device))
     held = _kv_workspaces.get(key)
