@@ -11,7 +11,7 @@ import torch
 import lowbit_hip as lb
 from conftest import announce
 from oracle import kv_oracle as ko
-from test_gpu_kv import dev, fresh, ints, rows_of
+from test_gpu_kv import check_attention, dev, fresh, ints, rows_of
 
 pytestmark = pytest.mark.gpu
 HALF = 2.0 ** -11
@@ -155,3 +155,75 @@ def test_scores_that_rise_by_a_little(device, format, rise, seq, factor):
         limit = weight * (2 * HALF + 2.0 ** -18 + 2.0 ** -13) + HALF * np.abs(want) + 2.0 ** -25 + n * 2.0 ** -32 * np.abs(hv).max()
         off = np.abs(got[0, i, 0] - want)
         assert (off <= limit).all(), (i, float((off / limit).max()), got[0, i, 0][:4], want[:4])
+
+
+@pytest.mark.parametrize('seq,heads', [(1, 2), (8, 2), (70, 2)])
+@pytest.mark.parametrize('format,dim', [('int8', 64), ('fp8', 128)])
+def test_small_probabilities_count(device, format, dim, seq, heads):
+    """Thousands of slots whose probabilities lie between 2^-14 and 2^-40 of the largest.
+
+    The bound is that of test_gpu_kv.py but for the probabilities that fp16 holds with fewer bits.  Lifted by 2^10 (2^9 in
+    tiles of 128 rows, where a ratio of value scales of up to 2^2 comes in) they are off by 2^-25
+    of that: n 2^-35 max|v| in the sum and in the total, n 2^-32 in tiles."""
+    announce('kv small probabilities', format, dim, seq, heads)
+    kv_heads, starts = 1, [9000, 4097]
+    batch, capacity = len(starts), 9152
+    total = max(starts) + seq
+    k, v = rows_of(230, batch, total, kv_heads, dim), rows_of(231, batch, total, kv_heads, dim)
+    q = rows_of(232, batch, seq, heads, dim)
+    # Values of 600, but of 0.01 where the first query's probability is above 2^-14 of the largest: the small ones are its sum.
+    t = np.einsum('bd,bnd->bn', q[:, 0, 0].astype(np.float64), k[:, :, 0].astype(np.float64)) * dim ** -0.5 / np.log(2)
+    seen = np.arange(total) <= np.array(starts)[:, None]
+    top = np.where(seen, t, -np.inf).max(1, keepdims=True)
+    v *= np.where(t > top - 14, 0.01, 600)[:, :, None, None].astype(np.float16)
+    assert 0.2 < ((t < top - 14) & (t > top - 40)).mean() < 0.6
+    cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device), rows=ints([s + seq for s in starts], device))
+    scale = float(np.float32(dim ** -0.5))
+    got = lb.kv_attention(dev(q, device), cache, ints(starts, device), scale=scale).float().cpu().numpy().astype(np.float64)
+    small = 2.0 ** (-35 if seq * heads <= 32 else -32)
+    worst = 0.0
+    for b in range(batch):
+        n = starts[b] + seq
+        kh, vh = (ko.held(t[b, :n, 0], format) for t in (k, v))
+        for h in range(heads):
+            out, weight, reach = ko.attend(q[b, :, h], kh, vh, starts[b], scale)
+            limit = (weight * (2 * HALF + 2 * (dim + 8) * 2.0 ** -24 * reach[:, None] + n * 2.0 ** -24) + 2 * n * small * np.abs(vh).max()
+                     + HALF * np.abs(out) + 2.0 ** -25)
+            off = np.abs(got[b, :, h] - out)
+            worst = max(worst, float((off / limit).max()))
+            assert (off <= limit).all(), (b, h, float((off / limit).max()))
+    print(f'[kv small probabilities] {format} {dim} {seq}: {worst:.2f} of the bound', flush=True)
+
+
+@pytest.mark.parametrize('appended', [False, True])
+@pytest.mark.parametrize('format', ['int8', 'fp8'])
+def test_long_sequences_far_apart_in_a_large_batch(device, format, appended):
+    """600 sequences, five of them long enough to be taken in parts: before, at and behind each 256th, where the search for a
+    workgroup's sequence goes on to the next 256; the last row in the cache already, or appended by the call."""
+    announce('kv large batch in parts', format, appended)
+    batch, heads, kv_heads, dim, capacity = 600, 2, 1, 64, 4096
+    rng = np.random.default_rng(240)
+    starts = [int(x) for x in rng.integers(0, 190, batch)]
+    far = {3: 4095, 255: 4031, 256: 3000, 511: 4094, 599: 4032}
+    for b, s in far.items():
+        starts[b] = s
+    some = sorted({*far, 0, 1, 254, 257, 510, 512, 598, *(int(x) for x in rng.integers(0, batch, 20))})
+    k, v = rows_of(241, batch, 192, kv_heads, dim), rows_of(242, batch, 192, kv_heads, dim, spread=.3)
+    more = [rows_of(243 + i, 1, capacity, kv_heads, dim) for i in range(2)]      # rows 192 .. of the long ones
+    q = rows_of(245, batch, 1, heads, dim)
+    lengths = [s + (not appended) for s in starts]
+    cache = fresh(device, batch, kv_heads, capacity, dim, format, fill=0x7F)
+    lb.kv_append(cache, dev(k, device), dev(v, device), ints([0] * batch, device), rows=ints([min(n, 192) for n in lengths], device))
+    wide = [dev(t[:, 192:], device).expand(batch, -1, -1, -1) for t in more]
+    lb.kv_append(cache, *wide, ints([192 if b in far else 0 for b in range(batch)], device),
+                 rows=ints([lengths[b] - 192 if b in far else 0 for b in range(batch)], device))
+    full = [np.concatenate((x[some], np.repeat(t[:, 192:], len(some), 0)), 1) for x, t in zip((k, v), more)]
+    last = {}
+    if appended:
+        rows = [np.stack([(x[b] if s < 192 else t[0])[s] for b, s in enumerate(starts)])[:, None] for x, t in zip((k, v), more)]
+        last = dict(k=dev(rows[0], device), v=dev(rows[1], device))
+    got = lb.kv_attention(dev(q, device), cache, ints(starts, device), **last)
+    worst = check_attention(got[some], q[some], *full, [starts[b] for b in some], [1] * len(some), format, dim ** -0.5, kv_heads)
+    print(f'[kv large batch in parts] {format}: {worst:.2f} of the bound', flush=True)
+    assert bool(torch.isfinite(got).all())
