@@ -174,3 +174,49 @@ def test_refusals(device):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)) and a.data_ptr() != b.data_ptr()
         for a, b in zip(lb.kv_read(c, cache._position), lb.kv_read(cache.cache, cache._position)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('format', ['int8', 'fp8'])
+def test_every_step_of_a_generation(device, format):
+    """generate_greedy over 8-bit caches: each step's logits against two of the oracle's layers in sequence, fed the tokens
+    that were produced, across the end of a block; each token is its step's largest logit.  Then GraphDecoder from the
+    prompt's snapshot: every replayed step against the oracle's fp16 decode going on from the values read back."""
+    announce('smollm kv every step', format)
+    cfg = smollm_random.config(theta=10000.0, layers=2)
+    weights, embedding, norm, _ = smollm_random.random_weights(3, 2, 0, std=0.06, embed_std=0.5)
+    layers = [FrozenSmolLayer(cfg, w, mode='w8a16', capacity=128, cache=format) for w in weights]
+    stack, io = FrozenSmolStack.from_layers(layers), FrozenSmolIO(cfg, embedding, norm).to(device)
+    oracles = [so.OracleLayer(layer._weights, {n: (q.format, q.shape, q.group_size, q.data, q.scales) for n, q in layer._packed.items()},
+                              theta=10000.0, capacity=128) for layer in layers]
+    model = so.OracleModel(oracles, embedding, norm)
+    ids, steps = smollm_random.prompt(1, 60), 10            # slots 60 .. 68: a block closes at 64
+    tokens, logits = generate_greedy(stack, io, ids, steps)
+    held = [HeldLayer(o, format) for o in oracles]
+
+    def through(x):
+        for layer in held:
+            x = layer.rows(x)
+        return model.logits(x[:, -1:])[0, 0]
+    want = through(model.embed(ids))
+    for step in range(steps):
+        assert rel_l2(logits[step], want) <= 1e-2, step
+        assert tokens[step] == int(logits[step].float().argmax()), step
+        if step < steps - 1:
+            want = through(model.embed(torch.tensor([[tokens[step]]])))
+    assert len(set(tokens)) > 1
+
+    with torch.no_grad():
+        _, caches = stack.prefill(io.embed_tokens(ids.to(device)))
+    decoder = GraphDecoder(stack, io)
+    decoder.load(caches, tokens[0])
+    decoder.capture()
+    kv = [tuple(t.cpu()[:, :, :60] for t in c.read()) for c in caches]
+    token = tokens[0]
+    for step in range(6):
+        x = model.embed(torch.tensor([[token]]))
+        for i, o in enumerate(oracles):
+            x, *kv[i] = o.decode(x, *kv[i], 60 + step)
+        token = decoder.generate(1)[0]
+        got = decoder.logits.view(-1).clone()
+        assert rel_l2(got, model.logits(x)[0, 0]) <= 1e-2, step
+        assert token == int(got.float().argmax()), step
