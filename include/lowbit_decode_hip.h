@@ -404,7 +404,7 @@ lb_status lb_kv_attention_workspace_bytes(const lb_kv_attention_args *args, size
  * (which holds position + rows slots, the query rows' own among them), scores, softmax and sums in fp32, the
  * probabilities rounded to fp16 for the product with V, the output to fp16.  Replaces the attention of the reference's
  * decode and prefill graphs (torch_npu_smollm.py:174-182, :195-340) over a cache that those did not have.  A sequence
- * whose rows lie outside the capacity gives NaN rows.
+ * whose rows lie outside the capacity (or whose count of them is not 0..seq) gives NaN in all seq of its out rows.
  */
 lb_status lb_kv_attention(const lb_kv_attention_args *args, void *stream);
 

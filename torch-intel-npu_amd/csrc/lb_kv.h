@@ -437,7 +437,7 @@ constexpr float kKvLowest = -1e30f;   // a running maximum below every score (sc
 // kKvSlack (in units of log2): fp16 then has them in [2^-24, 2^14], of which the smallest are 2^-34 of the largest.
 constexpr float kKvLift = 10.0f, kKvSlack = 4.0f;
 // The lift minus the maximum is one addend of a block's scores, which is off by half a step of the maximum: by 2^-15 here,
-// in a probability an eighth of its rounding to fp16, but by the whole lift from 2^27 on.  So a maximum further from zero
+// in a probability a twentieth of its rounding to fp16, but by the whole lift from 2^27 on.  So a maximum further from zero
 // than this is subtracted from the scores first (0 to 1.5% of a call for asking).
 constexpr float kKvFar = 1024.0f;
 constexpr int kKvTickets = 1024;      // (LB_ZEROED_WORKSPACE_BYTES)
@@ -613,9 +613,13 @@ __device__ __forceinline__ void kv_join(__amdgpu_buffer_rsrc_t po, __amdgpu_buff
 //     slots, 8 heads of 128, equal shares cut across sequences: 128 us).
 //   - Longer sequences first, and every other 256 workgroups backwards, so that the two that share a CU have together what
 //     others have: the same 64 sequences 100 us (5.4 TB/s) against 118 in the batch's order.  (Up to 64 sequences, by
-//     prefix sums in registers; sorting them outright took 50 ns a sequence.)
+//     prefix sums in registers; sorting them outright took 50 ns a sequence.)  Larger batches keep their own order, and every
+//     workgroup goes through the positions up to its sequence's: 1.2 us for 65 sequences, but as the square of the batch
+//     beyond (one block a sequence, 3 heads of 64: 256 sequences 7.1 us, 1024 27.7, 4096 195).
 //   - At 5 TB/s and more the loads in flight are what HBM takes; short ones are bound by the chain of position, codes, two
-//     products and the join: 4.1 us for one sequence of 150 slots and 3 heads of 64, 12.5 for 32 of 1984 with the append.
+//     products and the join: 4.2 us for one sequence of 150 slots and 3 heads of 64, 12.6 for 32 of 1984 with the append.
+//   - Of two query tiles 128 dims take 354 registers, one wave a SIMD: 64 sequences of 8192 slots, 8 KV heads of 128, five
+//     rows of four query heads 195 us (5.5 TB/s) against 189 for four rows in one tile; 16 of 4000 slots 39 against 30.
 //
 // Scores are K.Q^T and outputs V^T.P^T, so that a lane holds one query throughout (column lane % 16): its maximum,
 // total and rescaling are the lane's own, and the probabilities that it computes are the B operand of the second product
@@ -1028,10 +1032,11 @@ __global__ __launch_bounds__(256, (D == 64 && QT == 1 ? 4 : QT * D > 128 ? 1 : 2
 // block's scale, and the ratio vs / unit enters the exponent of the probabilities, whose total is divided by it once per
 // block.  A block whose ratio is past 4 either way sets the unit anew.
 //
-// What bounds it: of the cycles of a CU the matrix cores are busy 46% and the vector units 54% (per 64 slots and wave
+// What bounds it: of the cycles of a CU the matrix cores are busy 46% and the vector units 53% (per 64 slots and wave
 // D / 4 products of 32 cycles and, a lane, 32 exponentials at a quarter of the rate and some 150 other operations), which
 // two waves a SIMD overlap little.  8192 rows of 32 query and 8 KV heads of 128, fp8:
-// 575 to 579 us, 950 TFLOP/s; 509 rows over 32768 slots 318 us; 8 x 500 rows, 9 and 3 heads of 64: 13.6 us.  Measured on
+// 581 to 611 us by card, 946 to 900 TFLOP/s; 509 rows over 32768 slots 317 to 334 us; 8 x 500 rows, 9 and 3 heads of 64:
+// 13.6 us, 4096 rows of them 51 us, 377 TFLOP/s (half the products a block, as many other operations).  Measured on
 // the way: bank conflicts on a fifth of the cycles before the pieces' layout (620 us), scales asked for where they are
 // used (598 against 588).  Not kept: the next block's scores beside this one's exponentials (721 against 620, for want of
 // registers), 256 rows a workgroup (606 against 615, but 64 rows 45 us against 36).

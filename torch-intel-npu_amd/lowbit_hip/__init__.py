@@ -1328,7 +1328,8 @@ def kv_attention(q, cache, position, *, rows=None, k=None, v=None, out=None, sca
     """lb_kv_attention: causal grouped-query attention of q [batch, seq, heads, head_dim] over the cache.  Row i of
     sequence b lies at slot position[b] + i and attends over slots 0 .. position[b] + i, which the cache holds already, or
     gets here where k and v are given (kv_append's arguments).  rows (default: all): a sequence's query rows; out rows
-    behind them are left as they are (zero where out is allocated here).  scale: default head_dim ** -0.5.  cos and sin
+    behind them are left as they are (zero where out is allocated here).  A sequence whose rows do not lie in the capacity
+    is NaN in all of its out rows.  scale: default head_dim ** -0.5.  cos and sin
     rotate q (and k).  Any strides of q, k and v (a copy is made where rows are not 16-byte pieces)."""
     if out is None and isinstance(q, torch.Tensor):   # (what is not right with q is said below)
         out = (torch.empty if rows is None else torch.zeros)(q.shape, dtype=torch.float16, device=q.device)

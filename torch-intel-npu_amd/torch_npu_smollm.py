@@ -21,8 +21,9 @@ from a snapshot that is no longer the newest copies the storage first.
 
 cache='int8' or 'fp8' holds the KV cache in 8 bits (lowbit_hip.QuantizedKVCache; the reference has fp16 only): prefill
 and decode then attend over the held values with kv_attention, for any capacity and length, at half the memory and
-without a score matrix.  forward keeps no cache and stays as it is.  A snapshot more than 64 positions behind the newest
-one of its sequence goes on from the 8-bit values of its last, incomplete block of 64.
+without a score matrix; the rest of the layer runs staged, so it is slower than over fp16.  forward keeps no cache and
+stays as it is.  A snapshot whose last, incomplete block of 64 lies two or more blocks before the newest one's of its
+sequence goes on from that block's 8-bit values.
 """
 from dataclasses import dataclass, replace
 import json
