@@ -50,7 +50,19 @@ def test_one_score_far_above_the_others(device, format, dim, seq, power):
     Where the largest score is more than 40 (in log2) and twice the error of fp32 scores ahead of the next, the others have
     n 2^-40 together, and what is left is fp32 products (six of 2^-24 at the most) and the output's rounding."""
     announce('kv large scores', format, dim, seq, power)
-    heads, kv_heads, n, batch = 2, 1, 500, 3
+    clear_scores(device, format, dim, seq, power, 500)
+
+
+@pytest.mark.parametrize('power', [12, 27, 40])
+@pytest.mark.parametrize('format,dim', KINDS)
+def test_one_score_far_above_the_others_in_parts(device, format, dim, power):
+    """The same in tiles whose slots are taken in several parts (of eight blocks at the least): the parts' maxima meet."""
+    announce('kv large scores in parts', format, dim, power)
+    clear_scores(device, format, dim, 70, power, 2100)
+
+
+def clear_scores(device, format, dim, seq, power, n):
+    heads, kv_heads, batch = 2, 1, 3
     k, v = rows_of(200, batch, n, kv_heads, dim, spread=200), rows_of(201, batch, n, kv_heads, dim)
     q = rows_of(202, batch, seq, heads, dim, spread=200)
     k[1], q[1] = -np.abs(k[1]), np.abs(q[1])            # all scores below zero
@@ -61,7 +73,7 @@ def test_one_score_far_above_the_others(device, format, dim, seq, power):
     dots = [np.einsum('shd,nd->shn', q[b].astype(np.float64), held[b][0]) for b in range(batch)]
     scale = float(np.float32(2.0 ** power * 0.9 / max(np.abs(d).max() for d in dots) / 1.4426950408889634))
     assert 0 < scale <= 65536
-    cache = held_by(device, format, k, v, 512)
+    cache = held_by(device, format, k, v, (n + 63) // 64 * 64)
     got = lb.kv_attention(dev(q, device), cache, ints([first] * batch, device), scale=scale).float().cpu().numpy().astype(np.float64)
     clear = 0
     for b in range(batch):
