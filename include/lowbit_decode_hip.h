@@ -13,7 +13,8 @@
  *
  * Conventions are those of lowbit_hip.h: device pointers, caller-owned buffers,
  * asynchronous stream-ordered calls, lb_status results with lb_last_error().
- * Every activation here is one fp16 row (batch 1, one token).
+ * Every activation of a decode step is one fp16 row (batch 1, one token); the entry points for many rows and many
+ * requests say what they take.
  */
 #ifndef LOWBIT_DECODE_HIP_H
 #define LOWBIT_DECODE_HIP_H
@@ -443,6 +444,165 @@ lb_status lb_argmax_next(const void *logits, int64_t vocab, const void *embeddin
  */
 lb_status lb_head_next(const lb_fused_linear_args *head, const void *embedding, void *h_next, int64_t *tokens,
                        int64_t *token, int64_t *position, int64_t limit, void *stream);
+
+/*
+ * Serving many requests at once: rotary positions, a KV cache in pages with the attention that reads it, and low-rank
+ * adapters of many requests beside a shared projection.  The reference serves one sequence at a time
+ * (torch_npu_smollm.py:506-544) and has none of them.  No call reads a position, length, page or adapter number on the
+ * host, so that all of them may be captured into a HIP graph.
+ */
+typedef enum lb_type { LB_TYPE_FP16 = 0, LB_TYPE_BF16 = 1, LB_TYPE_FP32 = 2 } lb_type;
+
+/* Rows [batch, seq, heads] of contiguous values, strides in elements (0 to 2^40; written rows may not overlap). */
+typedef struct lb_rows {
+  void *data;
+  int64_t batch_stride, row_stride, head_stride;
+} lb_rows;
+
+/* How positions turn heads: pair i of the first `dims` dims turns by the angle position * frequencies[i], its cosine and
+ * sine times `scale`:  a' = scale (a cos - b sin),  b' = scale (b cos + a sin).  Dims from `dims` on stay. */
+#define LB_PAIRS_HALF 0u        /* pairs (i, i + dims / 2) */
+#define LB_PAIRS_NEIGHBOURS 1u  /* pairs (2 i, 2 i + 1) */
+#define LB_ROTARY_MAX_DIMS 1024
+
+typedef struct lb_rotation {
+  const double *frequencies; /* device [dims / 2], 8-byte aligned; NULL (where a call allows it): nothing turns */
+  uint32_t dims;             /* even, 2 .. head_dim */
+  uint32_t pairs;            /* LB_PAIRS_* */
+  float scale;               /* finite */
+  uint32_t reserved;
+} lb_rotation;
+
+typedef struct lb_rotary_args {
+  uint32_t struct_size;      /* sizeof(lb_rotary_args) */
+  uint32_t type;             /* lb_type */
+  int64_t batch, seq;        /* rows per sequence */
+  int64_t head_dim;          /* 2 .. LB_ROTARY_MAX_DIMS */
+  int64_t heads, k_heads;    /* k_heads 0: no keys */
+  lb_rows q, out;            /* [batch, seq, heads]; out may be q itself (the same address and strides) */
+  lb_rows k, out_k;          /* [batch, seq, k_heads], the same */
+  const int64_t *position;   /* device: [batch], row i at position[b] + i; with per_row [batch, seq], each row's own */
+  uint32_t per_row;
+  uint32_t back;             /* turns by the negative angle (still times scale): the transpose, the gradient's direction */
+  lb_rotation rotation;
+} lb_rotary_args;
+
+/*
+ * Rows of queries and keys turned by their positions, in one launch: products and sums in fp32, rounded once; angles are
+ * formed and reduced in 64 bits, so positions of any size (up to 2^53, below zero too) are as exact as the frequencies.
+ * Replaces the RoPE gather of the reference's graphs (torch_npu_smollm.py:262-303), whose tables and products are fp16,
+ * for any position, type, pairing, part of the head and scaling.  Fastest where rows are whole 16-byte pieces.
+ */
+lb_status lb_rotary(const lb_rotary_args *args, void *stream);
+
+/*
+ * A KV cache in pages.  A page holds `page` slots of every KV head of a layer; a sequence's slot p lies in page
+ * table[b][p / page], at slot p mod page of it.  Pages may belong to several sequences (a shared prefix), as long as no
+ * two of them append into one.  Layouts (row-major; D = head_dim):
+ *   keys    [pages][kv_heads][page][D]
+ *   values  [pages][kv_heads][page / 16][D][16]: by chunks of 16 slots, the slots of a dim side by side (the order in which
+ *           the matrix instructions take them)
+ */
+#define LB_PAGE_CHUNK 16
+
+typedef struct lb_paged_cache {
+  uint32_t type;               /* LB_TYPE_FP16 or LB_TYPE_BF16 */
+  uint32_t head_dim;           /* 64 or 128 */
+  int64_t pages;               /* 1 .. 2^31 - 1 */
+  int64_t kv_heads;            /* 1 .. 65535 */
+  int64_t page;                /* slots: 16, 32, .. 1024 (powers of two) */
+  void *keys, *values;         /* 16-byte aligned */
+} lb_paged_cache;
+
+typedef struct lb_page_table {
+  const int32_t *data;         /* device [batch] rows of `longest` page numbers */
+  int64_t stride;              /* elements between rows (0: every sequence has the same pages) */
+  int64_t longest;             /* entries of a row; page * longest at most 2^30.  Entries behind a sequence's pages are not read */
+} lb_page_table;
+
+typedef struct lb_paged_append_args {
+  uint32_t struct_size;        /* sizeof(lb_paged_append_args) */
+  uint32_t reserved;
+  lb_paged_cache cache;
+  lb_page_table table;
+  int64_t batch;               /* 1 .. 65535 */
+  int64_t seq;                 /* rows of k and v per sequence */
+  lb_rows k, v;                /* [batch, seq, kv_heads] rows of the cache's type, whole 16-byte pieces */
+  const int64_t *position;     /* device [batch]: the slot of a sequence's first row */
+  const int64_t *rows;         /* device [batch], 0..seq, or NULL: how many of its rows are appended (a padded batch) */
+  lb_rotation rotation;        /* of the keys by their slots (frequencies NULL: appended as they are) */
+} lb_paged_append_args;
+
+/*
+ * Appends rows[b] (NULL: seq) rows to every sequence, at slots position[b] .. .  A sequence whose rows do not lie in
+ * 0 .. page * longest - 1 is left alone, as are rows whose entry of the table is not a page.  One launch.
+ */
+lb_status lb_paged_append(const lb_paged_append_args *args, void *stream);
+
+typedef struct lb_paged_attention_args {
+  uint32_t struct_size;        /* sizeof(lb_paged_attention_args) */
+  uint32_t reserved;
+  lb_paged_cache cache;
+  lb_page_table table;
+  int64_t batch;               /* 1 .. 65535 */
+  int64_t heads;               /* a multiple of kv_heads: query head h uses KV head h / (heads / kv_heads) */
+  lb_rows q, out;              /* [batch, 1, heads] rows of the cache's type, whole 16-byte pieces (row_stride is not read) */
+  const int64_t *position;     /* device [batch]: the slot of a sequence's new token; -1: it has none, and out is 0 */
+  lb_rows k, v;                /* data NULL: the token's row is in its page already; else [batch, 1, kv_heads], appended */
+  lb_rotation rotation;        /* of q (and k) by position, rounded to the type (frequencies NULL: taken as they are) */
+  float scale;                 /* score scale, finite (usually 1 / sqrt(head_dim)) */
+  uint32_t reserved2;
+  void *workspace;             /* lb_paged_attention_workspace_bytes, 256-byte aligned.  Its first LB_ZEROED_WORKSPACE_BYTES
+                                  are zero before its first use, and every call leaves them zero again; for any calls,
+                                  which must be ordered (one stream) */
+  size_t workspace_bytes;
+} lb_paged_attention_args;
+
+/* Bytes of workspace lb_paged_attention needs for these arguments (0 when none), which depend on the cache's head_dim and
+ * page, kv_heads, heads, batch and the table's length alone; host-only. */
+lb_status lb_paged_attention_workspace_bytes(const lb_paged_attention_args *args, size_t *bytes);
+
+/*
+ * Grouped-query attention of one new token a sequence: the token at slot p attends over slots 0 .. p.  Scores, softmax and
+ * sums in fp32, the probabilities rounded to the type for the product with the values, out rounded once.  The slots are
+ * split over the chip by what the sequences hold, found on the device, and the parts joined in a fixed order.  What lies
+ * behind slot p in its page is not looked at, whatever it is.  A position past the table (or below -1), or an entry of
+ * the table below a sequence's length that is not a page, gives NaN in the sequence's out.
+ */
+lb_status lb_paged_attention(const lb_paged_attention_args *args, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside a projection that they share: out[m] = y[m] + s_a (x[m] A_a^T) B_a^T for row m
+ * with adapter a = index[m], out[m] = y[m] where a is -1, and NaN where it is no adapter.  Rows are taken in any order of
+ * adapters; those of one adapter are fastest side by side.
+ */
+#define LB_ADAPTERS_MAX_RANK 128
+
+typedef struct lb_adapters_args {
+  uint32_t struct_size;        /* sizeof(lb_adapters_args) */
+  uint32_t type;               /* LB_TYPE_FP16 or LB_TYPE_BF16 */
+  int64_t M, N, K;             /* rows; outputs; inputs (a multiple of 8) */
+  int64_t rank;                /* a multiple of 8 up to LB_ADAPTERS_MAX_RANK (factors of a lower rank are filled with zeros) */
+  int64_t count;               /* adapters */
+  const void *down;            /* A [count, rank, K], 16-byte aligned */
+  const void *up;              /* B [count, N, rank], 16-byte aligned */
+  const float *scales;         /* [count], or NULL: 1 */
+  const int64_t *index;        /* device [M] */
+  const void *x;               /* [M, ldx], 16-byte aligned, ldx a multiple of 8 */
+  int64_t ldx;
+  const void *y;               /* [M, ldy] */
+  int64_t ldy;
+  void *out;                   /* [M, ldo]; may be y itself (the same ldo) */
+  int64_t ldo;
+  void *workspace;             /* lb_adapters_workspace_bytes, 256-byte aligned; any contents */
+  size_t workspace_bytes;
+} lb_adapters_args;
+
+/* Bytes of workspace lb_adapters needs for these sizes; host-only. */
+lb_status lb_adapters_workspace_bytes(const lb_adapters_args *args, size_t *bytes);
+
+/* x A^T in fp32, taken as a sum of two 16-bit numbers into the product with B; sums in fp32, out rounded once. */
+lb_status lb_adapters(const lb_adapters_args *args, void *stream);
 
 #ifdef __cplusplus
 }

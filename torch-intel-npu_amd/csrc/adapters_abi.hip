@@ -1,0 +1,138 @@
+// lb_adapters: the low-rank adapters of many requests beside a shared projection.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "lb_adapters.h"
+#include "serve_check.h"
+
+using namespace lb;
+using namespace lb::abi;
+
+namespace {
+
+struct AdaptersPlan {
+  int rows;                 // rows of a tile / 16
+  int64_t tiles;
+  int slices, shares_down, span, shares_up;
+  size_t bytes;
+};
+
+AdaptersPlan adapters_plan(const lb_adapters_args *a) {
+  AdaptersPlan plan{};
+  // Tiles of 64 rows where there are rows enough for half the chip's CUs, else of 16.  (Of 32 with ranks past 64, whose sums fill
+  // the registers.)
+  plan.rows = a->M >= 2048 ? (a->rank > 64 ? 2 : 4) : 1;
+  plan.tiles = (a->M + 16 * plan.rows - 1) / (16 * plan.rows);
+  const int64_t most = std::min<int64_t>(a->count, 16 * plan.rows), pieces = (a->K + 63) / 64;
+  plan.shares_down = (int)std::max<int64_t>(1, std::min<int64_t>(most, 512 / plan.tiles));
+  plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (plan.tiles * plan.shares_down), (pieces + 7) / 8, 8}));
+  plan.span = a->N >= 4096 ? 512 : 256;
+  const int64_t spans = (a->N + plan.span - 1) / plan.span;
+  plan.shares_up = (int)std::max<int64_t>(1, std::min<int64_t>(most, 2048 / (plan.tiles * spans)));
+  plan.bytes = ((size_t)plan.slices * a->M * a->rank * 4 + 255) / 256 * 256;
+  return plan;
+}
+
+lb_status check_sizes(const char *what, const lb_adapters_args *a) {
+  if (a->type > LB_TYPE_BF16) return fail(LB_INVALID_ARGUMENT, "%s: type must be fp16 or bf16", what);
+  if (a->M < 1 || a->M > (1 << 28) || a->N < 1 || a->N > (1 << 28) || a->K < 8 || a->K > (1 << 28) || a->K % 8 != 0)
+    return fail(LB_INVALID_ARGUMENT, "%s: M, N and K 1 to 2^28 and K a multiple of 8 required", what);
+  if (a->rank < 8 || a->rank > LB_ADAPTERS_MAX_RANK || a->rank % 8 != 0)
+    return fail(LB_INVALID_ARGUMENT, "%s: rank must be a multiple of 8 up to %d", what, LB_ADAPTERS_MAX_RANK);
+  if (a->count < 1 || a->count > (1 << 24)) return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^24 adapters required", what);
+  const AdaptersPlan plan = adapters_plan(a);
+  if (plan.tiles * std::max<int64_t>(plan.slices, (a->N + plan.span - 1) / plan.span) > (1 << 23))   // 2^32 threads a launch
+    return fail(LB_UNSUPPORTED, "%s: more than 2^23 tiles of outputs", what);
+  return LB_OK;
+}
+
+lb_status check_matrix(const char *what, const char *name, const void *p, int64_t rows, int64_t columns, int64_t ld, bool pieces, bool written, Range &r) {
+  if (rows > 1 && written && ld < columns) return fail(LB_INVALID_ARGUMENT, "%s: rows of %s overlap one another", what, name);
+  return check_strided(what, name, lb_rows{const_cast<void *>(p), 0, ld, 0}, 1, rows, 1, columns, 2, pieces, false, r);
+}
+
+template <class T>
+void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) {
+  AdaptersParams<T> p{};
+  p.x = static_cast<const T *>(a->x);
+  p.y = static_cast<const T *>(a->y);
+  p.out = static_cast<T *>(a->out);
+  p.down = static_cast<const T *>(a->down);
+  p.up = static_cast<const T *>(a->up);
+  p.scales = a->scales;
+  p.index = a->index;
+  p.z = static_cast<float *>(a->workspace);
+  p.ldx = a->ldx;
+  p.ldy = a->ldy;
+  p.ldo = a->ldo;
+  p.M = (int)a->M;
+  p.N = (int)a->N;
+  p.K = (int)a->K;
+  p.rank = (int)a->rank;
+  p.count = (int)a->count;
+  p.slices = plan.slices;
+  p.span = plan.span;
+  p.wide = a->N % 8 == 0 && aligned(a->y, 16) && aligned(a->out, 16) && (a->M == 1 || (a->ldy % 8 == 0 && a->ldo % 8 == 0));
+  const dim3 down((unsigned)(plan.tiles * plan.slices), (unsigned)plan.shares_down);
+  const dim3 up((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares_up);
+  auto go = [&](auto rt, auto mt) {
+    constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
+    p.shares = plan.shares_down;
+    hipLaunchKernelGGL((adapters_down_kernel<T, RT, MT>), down, dim3(256), 0, s, p);
+    p.shares = plan.shares_up;
+    hipLaunchKernelGGL((adapters_up_kernel<T, (RT + 1) / 2, MT>), up, dim3(256), 0, s, p);
+  };
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 2> Two;
+  typedef std::integral_constant<int, 4> Four;
+  typedef std::integral_constant<int, 8> Eight;
+  const bool one = plan.rows == 1;
+  if (a->rank <= 16) one ? go(One{}, One{}) : go(One{}, Four{});
+  else if (a->rank <= 32) one ? go(Two{}, One{}) : go(Two{}, Four{});
+  else if (a->rank <= 64) one ? go(Four{}, One{}) : go(Four{}, Four{});
+  else one ? go(Eight{}, One{}) : go(Eight{}, Two{});
+}
+
+}  // namespace
+
+extern "C" {
+
+lb_status lb_adapters_workspace_bytes(const lb_adapters_args *a, size_t *bytes) {
+  const char *what = "lb_adapters_workspace_bytes";
+  if (!a || !bytes) return fail(LB_INVALID_ARGUMENT, "%s: args and bytes must be non-NULL", what);
+  *bytes = 0;
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  if (const lb_status st = check_sizes(what, a); st != LB_OK) return st;
+  *bytes = adapters_plan(a).bytes;
+  return ok();
+}
+
+lb_status lb_adapters(const lb_adapters_args *a, void *stream) {
+  const char *what = "lb_adapters";
+  if (const lb_status bad = refuse_if_failed(what); bad != LB_OK) return bad;
+  if (!a) return fail(LB_INVALID_ARGUMENT, "%s: args is NULL", what);
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  if (const lb_status st = check_sizes(what, a); st != LB_OK) return st;
+  Range reads[6], writes[2];
+  const size_t factor = (size_t)a->count * a->rank * 2;   // (below 2^32; K and N below 2^28)
+  if (const lb_status st = check_matrix(what, "x", a->x, a->M, a->K, a->ldx, true, false, reads[0]); st != LB_OK) return st;
+  if (const lb_status st = check_array(what, "down", a->down, factor * a->K, 16, true, reads[1]); st != LB_OK) return st;
+  if (const lb_status st = check_array(what, "up", a->up, factor * a->N, 16, true, reads[2]); st != LB_OK) return st;
+  if (const lb_status st = check_array(what, "scales", a->scales, (size_t)a->count * 4, 4, false, reads[3]); st != LB_OK) return st;
+  if (const lb_status st = check_array(what, "index", a->index, (size_t)a->M * 8, 8, true, reads[4]); st != LB_OK) return st;
+  if (const lb_status st = check_matrix(what, "y", a->y, a->M, a->N, a->ldy, false, false, reads[5]); st != LB_OK) return st;
+  if (const lb_status st = check_matrix(what, "out", a->out, a->M, a->N, a->ldo, false, true, writes[0]); st != LB_OK) return st;
+  const AdaptersPlan plan = adapters_plan(a);
+  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < plan.bytes)
+    return fail(LB_INVALID_ARGUMENT, "%s: a 256-byte aligned workspace of %zu bytes required (got %zu)", what, plan.bytes, a->workspace_bytes);
+  writes[1] = range_of(a->workspace, plan.bytes, "workspace");
+  const bool in_place = a->out == a->y && (a->M == 1 || a->ldo == a->ldy);
+  if (const lb_status st = check_apart(what, writes, 2, reads, 5); st != LB_OK) return st;
+  if (const lb_status st = check_apart(what, in_place ? writes + 1 : writes, in_place ? 1 : 2, reads + 5, 1); st != LB_OK) return st;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  a->type == LB_TYPE_FP16 ? launch<f16>(a, plan, s) : launch<bf16>(a, plan, s);
+  return launch_status(what);
+}
+
+}  // extern "C"

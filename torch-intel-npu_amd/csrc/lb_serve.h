@@ -1,0 +1,51 @@
+// What the kernels of lowbit_decode_hip.h that serve many requests share: 16-bit types and their matrix products, rows with strides, and the
+// rotation of heads by their positions.
+#pragma once
+#include "lb_common.h"
+
+namespace lb {
+
+typedef __bf16 bf16;
+
+// T x 8 and T x 4, and the 16x16x32 product of two operands of 8 (lane (j, g): row or column j, elements 8 g ..).
+template <class T> struct Of16;
+template <> struct Of16<f16> {
+  typedef f16 x8 __attribute__((ext_vector_type(8)));
+  typedef f16 x4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f4 mma(x8 a, x8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Of16<bf16> {
+  typedef bf16 x8 __attribute__((ext_vector_type(8)));
+  typedef bf16 x4 __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ f4 mma(x8 a, x8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// Rows of contiguous values, strides in elements.
+template <class T>
+struct Rows {
+  T *data;
+  long long batch, row, head;
+  __device__ __forceinline__ T *at(int b, int i, int h) const { return data + b * batch + i * row + h * head; }
+};
+
+// The rotation: pair i of the first `dims` dims turns by position * frequencies[i] (64 bits).
+struct Turn {
+  const double *frequencies;   // null: nothing turns
+  int dims, neighbours;        // pairs (i, i + dims / 2), or (2 i, 2 i + 1)
+  float scale;
+};
+
+// scale cos and scale sin of pair i at a position.  The angle is formed in 64 bits and reduced to a part of a turn there
+// (at position 2^20 a product in 32 bits is off by 0.06); the sine and cosine are 32 bits' own, right to an ulp or two.
+__device__ __forceinline__ float2 turn_of(const Turn &t, int i, double position) {
+  const double turns = position * t.frequencies[i] * 0.15915494309189533577;
+  float s, c;
+  sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &s, &c);
+  return make_float2(t.scale * c, t.scale * s);
+}
+
+// First dim of pair i, and how far from it the second one lies.
+__device__ __forceinline__ int pair_first(const Turn &t, int i) { return t.neighbours ? 2 * i : i; }
+__device__ __forceinline__ int pair_step(const Turn &t) { return t.neighbours ? 1 : t.dims / 2; }
+
+}  // namespace lb

@@ -1,0 +1,108 @@
+// lb_rotary: rows of heads turned by their positions.
+#include <hip/hip_runtime.h>
+
+#include "lb_rotary.h"
+#include "serve_check.h"
+
+using namespace lb;
+using namespace lb::abi;
+
+namespace {
+
+// Whether rows may be read and written in pieces of V values.
+bool in_pieces(const lb_rows &r, int64_t batch, int64_t seq, int64_t heads, int V, size_t size) {
+  return aligned(r.data, V * size) && (batch == 1 || r.batch_stride % V == 0) && (seq == 1 || r.row_stride % V == 0) &&
+         (heads == 1 || r.head_stride % V == 0);
+}
+
+template <class T, int V>
+void launch(const lb_rotary_args *a, bool in_place, hipStream_t s) {
+  RotaryParams<T> p{};
+  const lb_rows *x[2] = {&a->q, &a->k}, *out[2] = {&a->out, &a->out_k};
+  const int64_t heads[2] = {a->heads, a->k_heads};
+  for (int i = 0; i < 2; ++i) {
+    p.x[i] = strided<const T>(*x[i]);
+    p.out[i] = strided<T>(*out[i]);
+    p.heads[i] = (int)heads[i];
+  }
+  p.position = a->position;
+  p.turn = turn_params(a->rotation);
+  p.batch = (int)a->batch;
+  p.seq = (int)a->seq;
+  p.dim = (int)a->head_dim;
+  p.per_row = a->per_row != 0;
+  p.back = a->back != 0;
+  p.copies = in_place ? 0 : (int)((a->head_dim - p.turn.dims + 2 * V - 1) / (2 * V));
+  const int64_t rows = a->batch * a->seq, pieces = p.turn.dims / (2 * V) + p.copies, all = a->heads + a->k_heads;
+  // Heads side by side until there are threads enough for the chip; past that a thread's sines serve several heads.
+  p.lanes = (int)std::max<int64_t>(1, std::min<int64_t>(all, (1 << 19) / (rows * pieces)));
+  const int64_t threads = rows * pieces * p.lanes;
+  hipLaunchKernelGGL((rotary_kernel<T, V>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
+}
+
+}  // namespace
+
+extern "C" lb_status lb_rotary(const lb_rotary_args *a, void *stream) {
+  const char *what = "lb_rotary";
+  if (const lb_status bad = refuse_if_failed(what); bad != LB_OK) return bad;
+  if (!a) return fail(LB_INVALID_ARGUMENT, "%s: args is NULL", what);
+  if (a->struct_size < sizeof *a) return fail(LB_INVALID_ARGUMENT, "%s: struct_size %u < %zu", what, a->struct_size, sizeof *a);
+  if (a->type > LB_TYPE_FP32) return fail(LB_INVALID_ARGUMENT, "%s: unknown type %u", what, a->type);
+  if (a->head_dim < 2 || a->head_dim > LB_ROTARY_MAX_DIMS || a->heads < 1 || a->heads > 65535 || a->k_heads < 0 || a->k_heads > 65535)
+    return fail(LB_INVALID_ARGUMENT, "%s: head_dim 2 to %d, heads 1 to 65535 and k_heads 0 to 65535 required", what, LB_ROTARY_MAX_DIMS);
+  if (a->batch < 1 || a->seq < 1 || a->batch > kMaxSeq || a->seq > kMaxSeq / a->batch)
+    return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^28 rows required", what);
+  const size_t size = a->type == LB_TYPE_FP32 ? 4 : 2;
+  Range reads[4], writes[2];
+  if (const lb_status st = check_strided(what, "q", a->q, a->batch, a->seq, a->heads, a->head_dim, size, false, false, reads[0]); st != LB_OK) return st;
+  if (const lb_status st = check_strided(what, "out", a->out, a->batch, a->seq, a->heads, a->head_dim, size, false, true, writes[0]); st != LB_OK) return st;
+  if (a->k_heads) {
+    if (const lb_status st = check_strided(what, "k", a->k, a->batch, a->seq, a->k_heads, a->head_dim, size, false, false, reads[1]); st != LB_OK) return st;
+    if (const lb_status st = check_strided(what, "out_k", a->out_k, a->batch, a->seq, a->k_heads, a->head_dim, size, false, true, writes[1]); st != LB_OK) return st;
+  }
+  if (const lb_status st = check_array(what, "position", a->position, (size_t)(a->per_row ? a->batch * a->seq : a->batch) * 8, 8, true, reads[2]); st != LB_OK) return st;
+  if (const lb_status st = check_rotation(what, a->rotation, a->head_dim, true, reads[3]); st != LB_OK) return st;
+  // In place: out is q's rows and out_k k's, which may lie between one another (slices of one projection's rows).
+  const bool q_same = same_rows(a->q, a->out, a->batch, a->seq, a->heads);
+  const bool k_same = !a->k_heads || same_rows(a->k, a->out_k, a->batch, a->seq, a->k_heads);
+  const bool in_place = q_same && k_same;
+  if (in_place) {
+    if (a->k_heads) {                     // interleaved slices of one tensor share its range, but not its rows
+      if (overlaps(writes[0], writes[1])) {
+        const uintptr_t apart = writes[0].lo < writes[1].lo ? writes[1].lo - writes[0].lo : writes[0].lo - writes[1].lo;
+        const lb_rows &lower = writes[0].lo < writes[1].lo ? a->q : a->k, &upper = writes[0].lo < writes[1].lo ? a->k : a->q;
+        const int64_t nl = writes[0].lo < writes[1].lo ? a->heads : a->k_heads, nu = writes[0].lo < writes[1].lo ? a->k_heads : a->heads;
+        const int64_t wl = (nl == 1 ? 0 : (nl - 1) * lower.head_stride) + a->head_dim, wu = (nu == 1 ? 0 : (nu - 1) * upper.head_stride) + a->head_dim;
+        const int64_t pitch = a->seq > 1 ? lower.row_stride : lower.batch_stride;
+        const bool pitched = (a->seq == 1 || lower.row_stride == upper.row_stride) && (a->batch == 1 || lower.batch_stride == upper.batch_stride) &&
+                             (a->batch == 1 || a->seq == 1 || lower.batch_stride % lower.row_stride == 0);
+        if (!pitched || apart < (size_t)wl * size || apart + (size_t)wu * size > (size_t)pitch * size)
+          return fail(LB_INVALID_ARGUMENT, "%s: rows of q and k overlap", what);
+      }
+    }
+    const Range others[2] = {reads[2], reads[3]};
+    for (const Range &w : writes)
+      if (const lb_status st = check_apart(what, &w, 1, others, 2); st != LB_OK) return st;
+  } else {
+    if (q_same != k_same && a->k_heads)
+      return fail(LB_INVALID_ARGUMENT, "%s: q and k are turned in place both or neither", what);
+    if (const lb_status st = check_apart(what, writes, 2, reads, 4); st != LB_OK) return st;
+  }
+  auto fits = [&](int V) {
+    return a->rotation.dims % (2 * V) == 0 && a->head_dim % V == 0 && in_pieces(a->q, a->batch, a->seq, a->heads, V, size) &&
+           in_pieces(a->out, a->batch, a->seq, a->heads, V, size) &&
+           (!a->k_heads || (in_pieces(a->k, a->batch, a->seq, a->k_heads, V, size) && in_pieces(a->out_k, a->batch, a->seq, a->k_heads, V, size)));
+  };
+  const int V = size == 2 && fits(8) ? 8 : fits(4) ? 4 : 1;
+  if (a->batch * a->seq * (a->head_dim / (2 * V) + 2) > (int64_t)1 << 31)
+    return fail(LB_UNSUPPORTED, "%s: more than 2^31 pieces of rows", what);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->type == LB_TYPE_FP32) {
+    V == 4 ? launch<float, 4>(a, in_place, s) : launch<float, 1>(a, in_place, s);
+  } else if (a->type == LB_TYPE_FP16) {
+    V == 8 ? launch<f16, 8>(a, in_place, s) : V == 4 ? launch<f16, 4>(a, in_place, s) : launch<f16, 1>(a, in_place, s);
+  } else {
+    V == 8 ? launch<bf16, 8>(a, in_place, s) : V == 4 ? launch<bf16, 4>(a, in_place, s) : launch<bf16, 1>(a, in_place, s);
+  }
+  return launch_status(what);
+}

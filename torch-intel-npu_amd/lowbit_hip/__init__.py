@@ -18,7 +18,7 @@ import torch
 
 LIBRARY_PATH = Path(os.environ.get('LOWBIT_HIP_LIBRARY', Path(__file__).resolve().parent.parent / 'liblowbit_hip.so'))
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 OK, INVALID_ARGUMENT, OUT_OF_MEMORY, UNSUPPORTED, DEVICE_FAILED, INTERNAL = 0, 1, 2, 5, 10, 12
 FORMATS = {'int8': 0, 'int4': 1, 'nf4': 2, 'fp16': 3}
 FLAG_FORCE_GEMV, FLAG_FORCE_GEMM, FLAG_FORCE_GENERIC, FLAG_FORCE_STREAM, FLAG_FORCE_WIDE = 0x1, 0x2, 0x4, 0x20, 0x40
@@ -32,7 +32,8 @@ NOALLOC_SCRATCH_BYTES = 32 << 20   # LB_NOALLOC_SCRATCH_BYTES
 DECODE_EXPORTS = ('lb_fused_linear', 'lb_decode_attention', 'lb_argmax_next', 'lb_head_next', 'lb_decode_layer',
                   'lb_decode_stack_prepare', 'lb_decode_stack', 'lb_decode_stack_release', 'lb_decode_check',
                   'lb_rms_rows', 'lb_layer_rows', 'lb_kv_append', 'lb_kv_read', 'lb_kv_attention_workspace_bytes',
-                  'lb_kv_attention')
+                  'lb_kv_attention', 'lb_rotary', 'lb_paged_append', 'lb_paged_attention_workspace_bytes',
+                  'lb_paged_attention', 'lb_adapters_workspace_bytes', 'lb_adapters')
 PROLOGUES = {'none': 0, 'rmsnorm': 1, 'silu_mul': 2}
 MAX_PROBLEMS, MAX_RANK, MAX_FUSED_K = 3, 32, 1536
 KV_BLOCK = 64                                # LB_KV_BLOCK: slots of a cache block that share a scale
@@ -283,6 +284,7 @@ def library():
             getattr(lib, name).argtypes = [ctypes.POINTER(args), ctypes.c_void_p]
         lib.lb_kv_attention_workspace_bytes.restype = ctypes.c_int
         lib.lb_kv_attention_workspace_bytes.argtypes = [ctypes.POINTER(KVAttentionArgs), ctypes.POINTER(ctypes.c_size_t)]
+        serve.declare(lib)
         if lib.lb_abi_version() != ABI_VERSION:
             raise RuntimeError(f'liblowbit_hip ABI {lib.lb_abi_version()} != expected {ABI_VERSION}')
         _lib = lib
@@ -1363,3 +1365,9 @@ class PreparedKVAttention(_PreparedKV):
             a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
         self._bind('lb_kv_attention', 'lb_kv_attention', a, cache.device, keep)
         self.out = out
+
+
+# ---------------------------------------------------------------- serving many requests at once
+from . import serve   # noqa: E402  (it builds on what stands above)
+from .serve import (Adapters, PagedKVCache, PreparedAdapters, PreparedPagedAppend, PreparedPagedAttention, PreparedRotary,  # noqa: E402,F401
+                    Rotary, adapters_add, paged_append, paged_attention, rotary, rotary_frequencies)
