@@ -12,24 +12,33 @@ using namespace lb::abi;
 namespace {
 
 struct AdaptersPlan {
-  int rows;                 // rows of a tile / 16
+  bool fused;               // adapters_rows_kernel
+  int rows;                 // adapters_down_kernel: rows of a tile / 16
   int64_t tiles;
-  int slices, shares_down, span, shares_up;
+  int slices, shares, shares_up, span, stack;
   size_t bytes;
 };
 
 AdaptersPlan adapters_plan(const lb_adapters_args *a) {
   AdaptersPlan plan{};
-  // Tiles of 64 rows where there are rows enough for half the chip's CUs, else of 16.  (Of 32 with ranks past 64, whose sums fill
-  // the registers.)
-  plan.rows = a->M >= 2048 ? (a->rank > 64 ? 2 : 4) : 1;
+  const int64_t most = std::min<int64_t>(a->count, 16), tiles16 = (a->M + 15) / 16;
+  plan.fused = a->M <= 128 && a->rank <= 64 && a->K * a->rank <= 1 << 15;
+  if (plan.fused) {
+    plan.tiles = tiles16;
+    plan.span = 256;
+    plan.shares = (int)most;
+    plan.bytes = 256;
+    return plan;
+  }
+  // Tiles of 64 rows (of 32 with ranks past 64, whose sums fill the registers), and parts of K until there is a workgroup a CU.
+  plan.rows = a->M < 1024 ? 1 : a->rank > 64 ? 2 : 4;
   plan.tiles = (a->M + 16 * plan.rows - 1) / (16 * plan.rows);
-  const int64_t most = std::min<int64_t>(a->count, 16 * plan.rows), pieces = (a->K + 63) / 64;
-  plan.shares_down = (int)std::max<int64_t>(1, std::min<int64_t>(most, 512 / plan.tiles));
-  plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (plan.tiles * plan.shares_down), (pieces + 7) / 8, 8}));
-  plan.span = a->N >= 4096 ? 512 : 256;
-  const int64_t spans = (a->N + plan.span - 1) / plan.span;
-  plan.shares_up = (int)std::max<int64_t>(1, std::min<int64_t>(most, 2048 / (plan.tiles * spans)));
+  plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / plan.tiles, (a->K + 511) / 512, 4}));
+  plan.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(a->count, 16 * plan.rows), 512 / (plan.tiles * plan.slices)));
+  plan.stack = tiles16 >= 4 ? 4 : tiles16 >= 2 ? 2 : 1;
+  plan.shares_up = (int)(a->M < 1024 ? most : 1);
+  plan.span = 512;
+  while (plan.rows == 1 && plan.span > 128 && tiles16 * plan.shares_up * ((a->N + plan.span - 1) / plan.span) < 2048) plan.span /= 2;
   plan.bytes = ((size_t)plan.slices * a->M * a->rank * 4 + 255) / 256 * 256;
   return plan;
 }
@@ -42,7 +51,7 @@ lb_status check_sizes(const char *what, const lb_adapters_args *a) {
     return fail(LB_INVALID_ARGUMENT, "%s: rank must be a multiple of 8 up to %d", what, LB_ADAPTERS_MAX_RANK);
   if (a->count < 1 || a->count > (1 << 24)) return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^24 adapters required", what);
   const AdaptersPlan plan = adapters_plan(a);
-  if (plan.tiles * std::max<int64_t>(plan.slices, (a->N + plan.span - 1) / plan.span) > (1 << 23))   // 2^32 threads a launch
+  if ((a->M + 15) / 16 * std::max<int64_t>(plan.slices, (a->N + plan.span - 1) / plan.span) > (1 << 23))   // 2^32 threads a launch
     return fail(LB_UNSUPPORTED, "%s: more than 2^23 tiles of outputs", what);
   return LB_OK;
 }
@@ -74,19 +83,29 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
   p.slices = plan.slices;
   p.span = plan.span;
   p.wide = a->N % 8 == 0 && aligned(a->y, 16) && aligned(a->out, 16) && (a->M == 1 || (a->ldy % 8 == 0 && a->ldo % 8 == 0));
-  const dim3 down((unsigned)(plan.tiles * plan.slices), (unsigned)plan.shares_down);
-  const dim3 up((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares_up);
-  auto go = [&](auto rt, auto mt) {
-    constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
-    p.shares = plan.shares_down;
-    hipLaunchKernelGGL((adapters_down_kernel<T, RT, MT>), down, dim3(256), 0, s, p);
-    p.shares = plan.shares_up;
-    hipLaunchKernelGGL((adapters_up_kernel<T, (RT + 1) / 2, MT>), up, dim3(256), 0, s, p);
-  };
+  p.shares = plan.shares;
+  p.shares_up = plan.shares_up;
+  p.stack = plan.stack;
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
+  if (plan.fused) {
+    const dim3 grid((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares);
+    auto go = [&](auto rt) { hipLaunchKernelGGL((adapters_rows_kernel<T, decltype(rt)::value>), grid, dim3(64 * kRowsWaves), 0, s, p); };
+    a->rank <= 16 ? go(One{}) : a->rank <= 32 ? go(Two{}) : go(Four{});
+    return;
+  }
+  const int64_t wide = plan.span * (4 / plan.stack), rows = 16 * plan.stack;   // of a workgroup of adapters_up_kernel
+  const dim3 down((unsigned)(plan.tiles * plan.slices), (unsigned)plan.shares);
+  const dim3 up((unsigned)((a->M + rows - 1) / rows * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up);
+  const dim3 tile((unsigned)((a->M + 63) / 64 * ((a->N + plan.span - 1) / plan.span)));
+  auto go = [&](auto rt, auto mt) {
+    constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
+    hipLaunchKernelGGL((adapters_down_kernel<T, RT, MT>), down, dim3(512), 0, s, p);
+    if (MT > 1 && p.wide) hipLaunchKernelGGL((adapters_tile_kernel<T, (RT + 1) / 2>), tile, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((adapters_up_kernel<T, (RT + 1) / 2>), up, dim3(256), 0, s, p);
+  };
   const bool one = plan.rows == 1;
   if (a->rank <= 16) one ? go(One{}, One{}) : go(One{}, Four{});
   else if (a->rank <= 32) one ? go(Two{}, One{}) : go(Two{}, Four{});

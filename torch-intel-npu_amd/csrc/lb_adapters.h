@@ -10,6 +10,8 @@
 
 namespace lb {
 
+constexpr int kRowsWaves = 8;   // of a workgroup of adapters_rows_kernel
+
 template <class T>
 struct AdaptersParams {
   const T *x, *y, *down, *up;
@@ -20,8 +22,8 @@ struct AdaptersParams {
   long long ldx, ldy, ldo;
   int M, N, K, rank, count;
   int slices;               // parts of K, added by adapters_up_kernel
-  int shares;               // workgroups that share a tile's adapters
-  int span;                 // adapters_up_kernel: outputs of a workgroup
+  int shares, shares_up;    // workgroups that share a tile's adapters, in each launch
+  int span, stack;          // adapters_up_kernel: outputs of a wave, tiles of a workgroup (adapters_rows_kernel: outputs of one)
   int wide;                 // rows of y and out are whole 16-byte pieces
 };
 
@@ -45,11 +47,11 @@ __device__ __forceinline__ void each_adapter(int id, int share, int shares, F &&
   }
 }
 
-// z of 16 MT rows over one slice of K: waves take every fourth 64 of it and meet in LDS.
+// z of 16 MT rows over one slice of K: waves take every eighth 64 of it and meet in LDS.
 template <class T, int RT, int MT>
-__global__ __launch_bounds__(256) void adapters_down_kernel(AdaptersParams<T> p) {
+__global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
-  constexpr int W = 4, TILES = RT * MT, AHEAD = RT + MT > 5 ? 1 : RT + MT > 2 ? 2 : 4;   // pieces of 64 in flight
+  constexpr int W = 8, TILES = RT * MT, AHEAD = RT + MT > 6 ? 1 : 2;   // pieces of 64 in flight
   __shared__ f4 met[W][TILES][64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -104,110 +106,378 @@ __global__ __launch_bounds__(256) void adapters_down_kernel(AdaptersParams<T> p)
   });
 }
 
-// out = y + s z B^T of 16 MT rows and `span` outputs, 64 of them a wave at a time.  z enters as the sum of two 16-bit
-// numbers (16 bits of bf16 and 22 of fp16, after a power of two has brought the row's largest one below 1, so that no
-// z is too large or small for fp16), so its rounding stays far below that of the output.
-template <class T, int RC, int MT>
-__global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
+// Rows of a tile without an adapter, and those whose adapter there is not: y's values or NaNs, outputs from .. to - 1, by the
+// lanes of a wave.
+template <class T>
+__device__ __forceinline__ void rows_without(const AdaptersParams<T> &p, int id, int rows, int first, int lane, int from, int to) {
   typedef typename Of16<T>::x8 x8;
-  constexpr int W = 4;
-  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int spans = (p.N + p.span - 1) / p.span;
-  const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * (16 * MT);
-  const int id = adapter_of(p, first, lane, 16 * MT);
-  const x8 none = {};
-  if (blockIdx.y == 0) {                  // rows without an adapter, and those whose adapter there is not
-    uint64_t left = __ballot(lane < 16 * MT && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y));
-    while (left) {
-      const int row = __builtin_ctzll(left);
-      left &= left - 1;
-      const bool bad = __builtin_amdgcn_readlane(id, row) == -2;
-      const T *const y = p.y + (size_t)(first + row) * p.ldy;
-      T *const out = p.out + (size_t)(first + row) * p.ldo;
-      for (int n = from + threadIdx.x; n < to; n += 64 * W) out[n] = bad ? (T)__builtin_nanf("") : y[n];
+  uint64_t left = __ballot(lane < rows && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y));
+  while (left) {
+    const int row = __builtin_ctzll(left);
+    left &= left - 1;
+    const bool bad = __builtin_amdgcn_readlane(id, row) == -2;
+    const T *const y = p.y + (size_t)(first + row) * p.ldy;
+    T *const out = p.out + (size_t)(first + row) * p.ldo;
+    if (p.wide && !bad) {
+      for (int n = from + 8 * lane; n < to; n += 512) *reinterpret_cast<x8 *>(out + n) = *reinterpret_cast<const x8 *>(y + n);
+    } else {
+      for (int n = from + lane; n < to; n += 64) out[n] = bad ? (T)__builtin_nanf("") : y[n];
     }
   }
-  each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
-    x8 zh[RC][MT], zl[RC][MT];
-    float scale[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      const bool live = mine >> (16 * t + j) & 1;
-      float z[RC][8], top = 0.0f;
-#pragma unroll
-      for (int c = 0; c < RC; ++c) {
-        f4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-        if (live && 32 * c + 8 * g < p.rank)
-          for (int s = 0; s < p.slices; ++s) {
-            const float *const at = p.z + ((size_t)s * p.M + first + 16 * t + j) * p.rank + 32 * c + 8 * g;
-            lo += *reinterpret_cast<const f4 *>(at);
-            hi += *reinterpret_cast<const f4 *>(at + 4);
-          }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          z[c][e] = e < 4 ? lo[e] : hi[e - 4];
-          top = fmaxf(top, fabsf(z[c][e]));
-        }
-      }
-      scale[t] = p.scales ? p.scales[a] : 1.0f;
-      if constexpr (__is_same(T, f16)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const int e2 = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-#pragma unroll
-        for (int c = 0; c < RC; ++c)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z[c][e] = __builtin_amdgcn_ldexpf(z[c][e], -e2);
-        scale[t] = __builtin_amdgcn_ldexpf(scale[t], e2);
-      }
+}
+
+// z of a row as the sum of two 16-bit numbers (16 bits of bf16 and 22 of fp16, after a power of two has brought the row's
+// largest one below 1, so that no z is too large or small for fp16): its rounding stays far below that of the output.
+// A lane holds ranks 32 c + 8 g .. of row j; scale takes the power of two back.
+template <class T, int RC>
+struct Halves {
+  typename Of16<T>::x8 high[RC], low[RC];
+  // LANES: 0 where the lanes of a row are 16 apart, else as many side by side.
+  template <int LANES = 0>
+  __device__ __forceinline__ void split(float (&z)[RC][8], float &scale) {
+    if constexpr (__is_same(T, f16)) {
+      float top = 0.0f;
 #pragma unroll
       for (int c = 0; c < RC; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const T h = (T)z[c][e];
-          const float rest = z[c][e] - (float)h;
-          zh[c][t][e] = h;
-          zl[c][t][e] = (T)(fabsf((float)h) < INFINITY ? rest : 0.0f);
-        }
-    }
-    const T *const up = p.up + (size_t)a * p.N * p.rank;
-    for (int n0 = from + 64 * wave; n0 < to; n0 += 64 * W) {
-      f4 acc[4][MT] = {};
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(z[c][e]));
+      if constexpr (LANES == 0) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+      } else {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {       // row j of tile s: output 32 (s / 2) + 8 (j / 4) + 4 (s % 2) + j % 4
-        const int n = min(n0 + 32 * (s / 2) + 8 * (j / 4) + 4 * (s & 1) + (j & 3), p.N - 1);
+        for (int d = LANES / 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+      }
+      const int e2 = top > 0.0f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e] = __builtin_amdgcn_ldexpf(z[c][e], -e2);
+      scale = __builtin_amdgcn_ldexpf(scale, e2);
+    }
+#pragma unroll
+    for (int c = 0; c < RC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const T h = (T)z[c][e];
+        high[c][e] = h;
+        low[c][e] = (T)(fabsf((float)h) < INFINITY ? z[c][e] - (float)h : 0.0f);
+      }
+  }
+};
+
+// 64 outputs of 16 rows: their factors, and y and what is stored.  Row j of tile s is output 32 (s / 2) + 8 (j / 4) + 4 (s % 2) +
+// j % 4, so that a lane has 8 outputs side by side of its row, twice.
+template <class T, int RC>
+struct Factors {
+  typename Of16<T>::x8 up[4][RC];
+  __device__ __forceinline__ void fetch(const AdaptersParams<T> &p, const T *factor, int n0, int j, int g) {
+    typedef typename Of16<T>::x8 x8;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int n = min(n0 + 32 * (s / 2) + 8 * (j / 4) + 4 * (s & 1) + (j & 3), p.N - 1);
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        up[s][c] = 32 * c + 8 * g < p.rank ? *reinterpret_cast<const x8 *>(factor + (size_t)n * p.rank + 32 * c + 8 * g) : x8{};
+    }
+  }
+};
+
+template <class T>
+struct Base {
+  typedef typename Of16<T>::x8 x8;
+  x8 y[2];
+  __device__ __forceinline__ void fetch(const AdaptersParams<T> &p, const T *yrow, int n0, int to, bool live, int g) {
+    if (p.wide && live)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (n0 + 32 * s + 8 * g < to) y[s] = *reinterpret_cast<const x8 *>(yrow + n0 + 32 * s + 8 * g);
+  }
+  template <int RC>
+  __device__ __forceinline__ void store(const AdaptersParams<T> &p, const Factors<T, RC> &f, const Halves<T, RC> &z, float scale, const T *yrow, T *out,
+                                        int n0, int to, bool live, int g) const {
+    f4 acc[4] = {};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int c = 0; c < RC; ++c) {
+        acc[s] = Of16<T>::mma(f.up[s][c], z.high[c], acc[s]);
+        acc[s] = Of16<T>::mma(f.up[s][c], z.low[c], acc[s]);
+      }
+    if (!live) return;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int n = n0 + 32 * s + 8 * g;
+      if (p.wide) {
+        if (n >= to) continue;
+        x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (T)((float)y[s][e] + scale * acc[2 * s + e / 4][e % 4]);
+        *reinterpret_cast<x8 *>(out + n) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (n + e < to) out[n + e] = (T)((float)yrow[n + e] + scale * acc[2 * s + e / 4][e % 4]);
+      }
+    }
+  }
+};
+
+// Outputs from .. to - 1 of 16 rows, 64 at a time, every `step`, what they read requested one time ahead.
+template <class T, int RC>
+struct Writer {
+  Factors<T, RC> factors;
+  Base<T> base;
+  __device__ __forceinline__ void begin(const AdaptersParams<T> &p, const T *up, const T *y, int from, int to, bool live, int j, int g) {
+    factors.fetch(p, up, from, j, g);
+    base.fetch(p, y, from, to, live, g);
+  }
+  __device__ __forceinline__ void run(const AdaptersParams<T> &p, const T *up, const T *y, T *out, const Halves<T, RC> &z, float scale, int from, int to,
+                                      int step, bool live, int j, int g) {
+    for (int n0 = from; n0 < to; n0 += step) {
+      const Factors<T, RC> f = factors;
+      const Base<T> held = base;
+      if (n0 + step < to) begin(p, up, y, n0 + step, to, live, j, g);
+      held.store(p, f, z, scale, y, out, n0, to, live, g);
+    }
+  }
+};
+
+// z of row j of 16 from `first` on, its slices added in their order.
+template <class T, int RC>
+__device__ __forceinline__ void gather(const AdaptersParams<T> &p, int first, bool live, int j, int g, float (&z)[RC][8]) {
+  for (int s0 = 0; s0 < p.slices; s0 += 4) {
+    f4 part[4][RC][2] = {};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (live && s0 + s < p.slices && 32 * c + 8 * g < p.rank) {
+          const float *const at = p.z + ((size_t)(s0 + s) * p.M + first + j) * p.rank + 32 * c + 8 * g;
+          part[s][c][0] = *reinterpret_cast<const f4 *>(at);
+          part[s][c][1] = *reinterpret_cast<const f4 *>(at + 4);
+        }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e] += part[s][c][e / 4][e % 4];
+  }
+}
+
+// out = y + s z B^T.  A wave takes 16 rows and `span` outputs; the waves of a workgroup have `stack` tiles of rows and 4 / stack
+// spans.
+template <class T, int RC>
+__global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
+  const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int beside = 4 / p.stack, spans = (p.N + p.span * beside - 1) / (p.span * beside);
+  const int from = (blockIdx.x % spans * beside + wave / p.stack) * p.span, to = min(p.N, from + p.span);
+  const int first = (blockIdx.x / spans * p.stack + wave % p.stack) * 16;
+  if (from >= to) return;
+  const int id = adapter_of(p, first, lane, 16);
+  if (blockIdx.y == 0) rows_without(p, id, 16, first, lane, from, to);
+  each_adapter(id, blockIdx.y, p.shares_up, [&](int a, uint64_t mine) {
+    const bool live = mine >> j & 1;
+    const T *const up = p.up + (size_t)a * p.N * p.rank;
+    const T *const y = p.y + (size_t)(first + j) * p.ldy;
+    T *const out = p.out + (size_t)(first + j) * p.ldo;
+    Writer<T, RC> writer;
+    writer.begin(p, up, y, from, to, live, j, g);
+    float scale = p.scales ? p.scales[a] : 1.0f, z[RC][8] = {};
+    gather<T, RC>(p, first, live, j, g, z);
+    Halves<T, RC> halves;
+    halves.split(z, scale);
+    writer.run(p, up, y, out, halves, scale, from, to, 64, live, j, g);
+  });
+}
+
+// out = y + s z B^T of 64 rows and `span` outputs, 128 at a time, for many rows (p.wide).  y is read and out written in rows of
+// 256 bytes, 1 KB a wave at once, since a transfer whose lanes have 16 rows costs the address unit twice that of whole lines;
+// the products come to the lanes of those rows through LDS.  z is added up and split once a workgroup, and kept in LDS; the
+// factors of 32 outputs, which a wave holds, serve all rows of the tile.
+template <class T, int RC>
+__global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p) {
+  typedef typename Of16<T>::x8 x8;
+  constexpr int ROWS = 64, NB = 128, PITCH = NB + 4, ZP = 32 * RC + 8, PER = ROWS * NB / 2048, LANES = 4 * RC;   // LANES: of a row's ranks
+  __shared__ __align__(16) float mem[ROWS][PITCH];
+  __shared__ __align__(16) T zh[ROWS][ZP], zl[ROWS][ZP];
+  __shared__ float scales[ROWS];
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int spans = (p.N + p.span - 1) / p.span;
+  const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * ROWS;
+  const int id = adapter_of(p, first, lane, ROWS);
+  x8 yn[PER];
+  auto piece_at = [&](int i, int n0, int &row, int &n) {
+    row = 16 * i + tid / 16;
+    n = n0 + tid % 16 * 8;
+    return first + row < p.M && n < to;
+  };
+  auto fetch = [&](int n0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row, n;
+      if (piece_at(i, n0, row, n)) yn[i] = *reinterpret_cast<const x8 *>(p.y + (size_t)(first + row) * p.ldy + n);
+    }
+  };
+  fetch(from);
+#pragma unroll
+  for (int r0 = 0; r0 < ROWS; r0 += 256 / LANES) {       // z of a row by LANES lanes, 8 ranks each
+    const int row = r0 + tid / LANES, rank = tid % LANES * 8;
+    const int a = __shfl(id, row);
+    f4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    if (a >= 0 && rank < p.rank)
+      for (int s0 = 0; s0 < p.slices; s0 += 4) {
+        f4 part[4][2] = {};
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+          if (s0 + s < p.slices) {
+            const float *const at = p.z + ((size_t)(s0 + s) * p.M + first + row) * p.rank + rank;
+            part[s][0] = *reinterpret_cast<const f4 *>(at);
+            part[s][1] = *reinterpret_cast<const f4 *>(at + 4);
+          }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          lo += part[s][0];
+          hi += part[s][1];
+        }
+      }
+    float scale = a >= 0 && p.scales ? p.scales[a] : 1.0f, z[1][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) z[0][e] = e < 4 ? lo[e] : hi[e - 4];
+    Halves<T, 1> halves;
+    halves.template split<LANES>(z, scale);
+    *reinterpret_cast<x8 *>(&zh[row][rank]) = halves.high[0];
+    *reinterpret_cast<x8 *>(&zl[row][rank]) = halves.low[0];
+    if (rank == 0) scales[row] = scale;
+  }
+  __syncthreads();
+  for (int n0 = from; n0 < to; n0 += NB) {
+    each_adapter(id, 0, 1, [&](int a, uint64_t mine) {
+      const T *const up = p.up + (size_t)a * p.N * p.rank;
+      x8 factors[2][RC];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {       // row j of tile s: output 8 (j / 4) + 4 s + j % 4 of the wave's 32
+        const int n = min(n0 + 32 * wave + 8 * (j / 4) + 4 * s + (j & 3), p.N - 1);
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+          factors[s][c] = 32 * c + 8 * g < p.rank ? *reinterpret_cast<const x8 *>(up + (size_t)n * p.rank + 32 * c + 8 * g) : x8{};
+      }
+#pragma unroll
+      for (int t = 0; t < ROWS / 16; ++t) {
+        if ((mine >> (16 * t) & 0xFFFF) == 0) continue;
+        f4 acc[2] = {};
 #pragma unroll
         for (int c = 0; c < RC; ++c) {
-          const x8 u = 32 * c + 8 * g < p.rank ? *reinterpret_cast<const x8 *>(up + (size_t)n * p.rank + 32 * c + 8 * g) : none;
+          const x8 h = *reinterpret_cast<const x8 *>(&zh[16 * t + j][32 * c + 8 * g]), l = *reinterpret_cast<const x8 *>(&zl[16 * t + j][32 * c + 8 * g]);
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            acc[s][t] = Of16<T>::mma(u, zh[c][t], acc[s][t]);
-            acc[s][t] = Of16<T>::mma(u, zl[c][t], acc[s][t]);
+          for (int s = 0; s < 2; ++s) {
+            acc[s] = Of16<T>::mma(factors[s][c], h, acc[s]);
+            acc[s] = Of16<T>::mma(factors[s][c], l, acc[s]);
           }
         }
-      }
+        if (mine >> (16 * t + j) & 1) {
+          const float scale = scales[16 * t + j];
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (!(mine >> (16 * t + j) & 1)) continue;
-        const T *const y = p.y + (size_t)(first + 16 * t + j) * p.ldy;
-        T *const out = p.out + (size_t)(first + 16 * t + j) * p.ldo;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int n = n0 + 32 * s + 8 * g;
-          if (p.wide) {
-            if (n >= to) continue;
-            x8 v = *reinterpret_cast<const x8 *>(y + n);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (T)((float)v[e] + scale[t] * acc[2 * s + e / 4][t][e % 4]);
-            *reinterpret_cast<x8 *>(out + n) = v;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < to) out[n + e] = (T)((float)y[n + e] + scale[t] * acc[2 * s + e / 4][t][e % 4]);
-          }
+          for (int s = 0; s < 2; ++s) *reinterpret_cast<f4 *>(&mem[16 * t + j][32 * wave + 8 * g + 4 * s]) = acc[s] * scale;
         }
       }
+    });
+    __syncthreads();
+    x8 y[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) y[i] = yn[i];
+    if (n0 + NB < to) fetch(n0 + NB);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      int row, n;
+      const bool there = piece_at(i, n0, row, n);
+      const int whose = __shfl(id, row);
+      if (!there || (whose == -1 && p.out == p.y)) continue;
+      const f4 lo = *reinterpret_cast<const f4 *>(&mem[row][n - n0]), hi = *reinterpret_cast<const f4 *>(&mem[row][n - n0 + 4]);
+      x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float sum = (float)y[i][e] + (e < 4 ? lo[e] : hi[e - 4]);
+        v[e] = whose >= 0 ? (T)sum : whose == -1 ? y[i][e] : (T)__builtin_nanf("");
+      }
+      *reinterpret_cast<x8 *>(p.out + (size_t)(first + row) * p.ldo + n) = v;
+    }
+    __syncthreads();                      // (mem is read)
+  }
+}
+
+// Both products of 16 rows in one launch, for few rows: a workgroup of W waves computes z of an adapter of the tile itself (its
+// waves take every W-th 64 of K and meet in LDS) and `span` outputs, 64 a wave at a time, whose factors and y are requested
+// before z is there.  Every span's workgroup reads the whole of A again, from the caches.
+template <class T, int RT>
+__global__ __launch_bounds__(64 * kRowsWaves) void adapters_rows_kernel(AdaptersParams<T> p) {
+  typedef typename Of16<T>::x8 x8;
+  constexpr int W = kRowsWaves, RC = (RT + 1) / 2, AHEAD = RT == 1 ? 4 : RT == 2 ? 2 : 1;
+  __shared__ f4 met[W][RT][64];
+  __shared__ __align__(16) float zs[16][32 * RC + 4];
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int spans = (p.N + p.span - 1) / p.span;
+  const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * 16;
+  const int id = adapter_of(p, first, lane, 16), all = (p.K + 63) / 64;
+  if (blockIdx.y == 0) {
+    const int n = from + 64 * wave;       // (64 outputs a wave, so rows of spans past 1024 go round)
+    for (int n0 = n; n0 < to; n0 += 64 * W) rows_without(p, id, 16, first, lane, n0, min(to, n0 + 64));
+  }
+  const x8 none = {};
+  each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
+    const bool live = mine >> j & 1;
+    const T *const up = p.up + (size_t)a * p.N * p.rank;
+    const T *const y = p.y + (size_t)(first + j) * p.ldy;
+    T *const out = p.out + (size_t)(first + j) * p.ldo;
+    Writer<T, RC> writer;
+    const int mine0 = from + 64 * wave;
+    if (mine0 < to) writer.begin(p, up, y, mine0, to, live, j, g);
+    float scale = p.scales ? p.scales[a] : 1.0f;
+    f4 acc[RT] = {};
+    const T *const down = p.down + (size_t)a * p.rank * p.K + 8 * g, *const x = p.x + (size_t)(first + j) * p.ldx + 8 * g;
+    for (int piece = wave; piece < all; piece += W * AHEAD) {
+      x8 d[AHEAD][2][RT], xv[AHEAD][2];
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int k = (piece + n * W) * 64 + 32 * c;
+          const bool there = k + 8 * g < p.K;
+#pragma unroll
+          for (int r = 0; r < RT; ++r) d[n][c][r] = there ? *reinterpret_cast<const x8 *>(down + (size_t)min(16 * r + j, p.rank - 1) * p.K + k) : none;
+          xv[n][c] = there && live ? *reinterpret_cast<const x8 *>(x + k) : none;
+        }
+#pragma unroll
+      for (int n = 0; n < AHEAD; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) acc[r] = Of16<T>::mma(d[n][c][r], xv[n][c], acc[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) met[wave][r][lane] = acc[r];
+    __syncthreads();
+    for (int i = tid; i < RT * 256; i += 64 * W) {       // element i % 4 of lane i / 4 of its tile
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += reinterpret_cast<const float *>(&met[w][0][0])[i];
+      const int at = i / 4 % 64;
+      zs[at & 15][16 * (i / 256) + 4 * (at >> 4) + i % 4] = sum;
+    }
+    __syncthreads();
+    if (mine0 < to) {
+      float z[RC][8];
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[c][e] = live && 32 * c + 8 * g < p.rank ? zs[j][32 * c + 8 * g + e] : 0.0f;
+      Halves<T, RC> halves;
+      halves.split(z, scale);
+      writer.run(p, up, y, out, halves, scale, mine0, to, 64 * W, live, j, g);
     }
   });
 }
