@@ -32,85 +32,95 @@ struct PagedAppendParams {
   Rows<const T> k, v;
   const int64_t *position, *rows;
   Turn turn;
-  int seq;
+  int seq, heads;           // heads: KV heads of a workgroup
 };
 
-// A workgroup takes one chunk of 16 slots that new rows fall into, for all KV heads of a sequence: the chunk's sines and
-// cosines are computed once, into LDS.  A thread holds 8 dims of 4 slots, so that keys are written in 16-byte pieces and
-// values in the 8 bytes that 4 slots of a dim are.
+// A workgroup takes one chunk of 16 slots that new rows fall into, for `heads` KV heads of a sequence.  Values are read in rows and
+// turned in LDS into the 16 bytes that 8 slots of a dim are, so that both sides move whole lines; the chunk's sines and cosines are
+// computed behind their loads, once for all heads, into LDS; then keys, 8 dims of a row a thread.  (One loop body for every
+// key: straight-line code of four rows took a short call as long to fetch as to run.)
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> p) {
   typedef typename Of16<T>::x8 x8;
-  typedef typename Of16<T>::x4 x4;
-  constexpr int CH = D / 8, PER = 4 * CH, LANES = 256 / PER;   // threads of a head; heads at once
+  constexpr int CH = D / 8, LANES = 256 / (kChunk * CH), PITCH = D + 8;   // pieces of a row; heads at once
   __shared__ float2 turns[kChunk][D / 2];
-  const int tid = threadIdx.x, b = blockIdx.y;
+  __shared__ __align__(16) T tile[LANES][kChunk][PITCH];
+  const int tid = threadIdx.x, b = blockIdx.y, head0 = blockIdx.z * p.heads, head1 = min(head0 + p.heads, p.c.kv_heads);
   const int64_t at = p.position[b], n = p.rows ? p.rows[b] : p.seq;
   if (at < 0 || n < 0 || n > p.seq || at > p.c.slots() - n) return;
   const int first = (int)at, end = first + (int)n, chunk = first / kChunk + blockIdx.x, base = chunk * kChunk;
   if (base >= end) return;
   const int id = p.c.table[b * p.c.table_stride + (chunk >> p.c.shift)];
   if ((unsigned)id >= (unsigned)p.c.pages) return;
+  const int from = max(first, base), to = min(end, base + kChunk);
   const int half = p.turn.frequencies ? p.turn.dims / 2 : 0;
-  if (half) {
-    for (int i = tid; i < kChunk * half; i += 256) turns[i / half][i % half] = turn_of(p.turn, i % half, (double)(base + i / half));
+  const int lane = tid / (kChunk * CH), piece = tid % (kChunk * CH), mine = base + piece / CH;   // this thread's piece of a head, its slot
+  auto value = [&](int h) {
+    return h < head1 && mine >= from && mine < to ? *reinterpret_cast<const x8 *>(p.v.at(b, mine - first, h) + 8 * (piece % CH)) : x8{};
+  };
+  x8 next = value(head0 + lane);
+#pragma unroll 1
+  for (int i = tid; i < kChunk * (D / 2); i += 256)
+    if (i % (D / 2) < half) turns[i / (D / 2)][i % (D / 2)] = turn_of(p.turn, i % (D / 2), (double)(base + i / (D / 2)));
+  for (int h0 = head0; h0 < head1; h0 += LANES) {
+    *reinterpret_cast<x8 *>(&tile[lane][piece / CH][8 * (piece % CH)]) = next;
+    __syncthreads();
+    next = value(h0 + LANES + lane);
+    const int h = h0 + lane, dim = piece / 2, low = 8 * (piece % 2);      // 8 slots of a dim
+    if (h < head1) {
+      x8 v;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[lane][low + e][dim];
+      T *const out = p.c.values + p.c.template chunk<D>(id, h, chunk) + dim * kChunk + low;
+      if (base + low >= from && base + low + 8 <= to) {
+        *reinterpret_cast<x8 *>(out) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (base + low + e >= from && base + low + e < to) out[e] = v[e];
+      }
+    }
     __syncthreads();
   }
-  const int dim = 8 * (tid % CH), quad = tid / CH % 4;
+  // Keys.
   const bool pieces = p.turn.neighbours || half % 8 == 0;     // a pair's second dims are a piece too
-  for (int h = tid / PER; h < p.c.kv_heads; h += LANES) {
-    x8 k[4], v[4];
-    uint32_t have = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int slot = base + 4 * quad + i;
-      k[i] = v[i] = x8{};
-      if (slot < first || slot >= end) continue;
-      have |= 1u << i;
-      const T *const row = p.k.at(b, slot - first, h);
-      k[i] = *reinterpret_cast<const x8 *>(row + dim);
-      v[i] = *reinterpret_cast<const x8 *>(p.v.at(b, slot - first, h) + dim);
-      if (dim >= 2 * half) continue;
-      const float2 *const cs = turns[4 * quad + i];
+  const int items = (head1 - head0) * (kChunk * CH);
+  for (int i = tid; i < items; i += 256) {
+    const int dim = 8 * (i % CH), slot = base + i / CH % kChunk, h = head0 + i / (CH * kChunk);
+    if (slot < from || slot >= to) continue;
+    const T *const row = p.k.at(b, slot - first, h);
+    x8 k = *reinterpret_cast<const x8 *>(row + dim);
+    if (dim < 2 * half) {
+      const float2 *const cs = turns[slot - base];
       if (p.turn.neighbours) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
           if (dim + e >= 2 * half) continue;
           const float2 t = cs[(dim + e) / 2];
-          const float x = (float)k[i][e], y = (float)k[i][e + 1];
-          k[i][e] = (T)(x * t.x - y * t.y);
-          k[i][e + 1] = (T)(y * t.x + x * t.y);
+          const float x = (float)k[e], y = (float)k[e + 1];
+          k[e] = (T)(x * t.x - y * t.y);
+          k[e + 1] = (T)(y * t.x + x * t.y);
         }
       } else {
         x8 other = {};
-        if (pieces) other = *reinterpret_cast<const x8 *>(row + (dim < half ? dim + half : dim - half));
-        else
+        if (pieces) {
+          other = *reinterpret_cast<const x8 *>(row + (dim < half ? dim + half : dim - half));
+        } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (dim + e < 2 * half) other[e] = row[dim + e < half ? dim + e + half : dim + e - half];
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           if (dim + e >= 2 * half) continue;
           const bool low = dim + e < half;
           const float2 t = cs[low ? dim + e : dim + e - half];
-          const float x = (float)k[i][e], y = (float)other[e];
-          k[i][e] = (T)(low ? x * t.x - y * t.y : x * t.x + y * t.y);
+          const float x = (float)k[e], y = (float)other[e];
+          k[e] = (T)(low ? x * t.x - y * t.y : x * t.x + y * t.y);
         }
       }
     }
-    const size_t to = p.c.template chunk<D>(id, h, chunk);
-    T *const kd = p.c.keys + to + 4 * quad * D + dim, *const vd = p.c.values + to + dim * kChunk + 4 * quad;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (have >> i & 1) *reinterpret_cast<x8 *>(kd + i * D) = k[i];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (have == 15u) *reinterpret_cast<x4 *>(vd + e * kChunk) = x4{v[0][e], v[1][e], v[2][e], v[3][e]};
-      else
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (have >> i & 1) vd[e * kChunk + i] = v[i][e];
-    }
+    *reinterpret_cast<x8 *>(p.c.keys + p.c.template chunk<D>(id, h, chunk) + (slot - base) * D + dim) = k;
   }
 }
 
@@ -124,6 +134,7 @@ struct PagedAttendParams {
   Turn turn;
   uint32_t *tickets;        // kPagedParts zero words
   float *partial;           // [places][16][D] sums, then [places][16][2] references and totals
+  uint32_t parts;           // batches past 64: parts that the work is split into at the most, besides sequences and heads
   int batch, group, tiles;  // group: query heads of a KV head; tiles of up to 16 of them
   float scale;              // score scale * log2(e)
 };
@@ -132,7 +143,7 @@ constexpr int kUnit = 2 * kChunk;     // slots of a wave's step
 // Parts that the whole work is split into at the most, besides those that sequences and heads are by themselves, and places
 // for the sums of parts.
 constexpr int kPagedParts = 1024, kPagedPlaces = 2 * kPagedParts + 2;
-constexpr int kPagedLeast = 16;       // units of a part at the least
+constexpr int kPagedLeast = 16;       // units of a part at the least: two a wave
 constexpr float kPagedLowest = -3.402823466e38f;
 // Probabilities are taken relative to a reference 2^kPagedLift below a row's running maximum when it was set, and it is
 // set anew where a score exceeds it by kPagedLift + kPagedSlack (units of log2): fp16 then has the probabilities in
@@ -143,7 +154,7 @@ constexpr float kPagedLift = 10.0f, kPagedSlack = 4.0f;
 __device__ __forceinline__ uint32_t lanes_sum(uint32_t x) { return __builtin_amdgcn_readlane(kv_scan(x), 63); }
 
 // One new token a sequence.  A workgroup takes a part of a sequence's slots for a KV head (and up to 16 of its query heads),
-// its W waves every W-th unit of 32 slots each with a reference and total of their own, joined in LDS; parts are joined by
+// its W waves every W-th unit of slots each with a reference and total of their own, joined in LDS; parts are joined by
 // the workgroup that counts last.  Which part it takes is found from the positions, on the device.
 //
 // TURNED: queries are turned by their position (and the new key).  A turned query enters the product as the sum of two numbers of
@@ -152,7 +163,7 @@ template <class T, int D, int W, bool TURNED>
 __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<T> p) {
   typedef typename Of16<T>::x8 x8;
   typedef typename Of16<T>::x4 x4;
-  constexpr int NT = 64 * W, R = 16, U = D / 32, DT = D / 16, PITCH = D + 4, DQ = D / 4, QP = D + 8;
+  constexpr int NT = 64 * W, R = 16, U = D / 32, DT = D / 16, C = 2, UNIT = kUnit, PER = 64 / C, PITCH = D + 4, DQ = D / 4, QP = D + 8;
   __shared__ __align__(16) float sums[W][R][PITCH];
   __shared__ float tops[W][R], totals[W][R];
   __shared__ __align__(16) T rows_[R + 2][QP];      // queries, and the new key and value
@@ -165,14 +176,47 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
 
   // Units of a sequence: those of its slots, none where there is no token, one where it lies outside (to write NaNs).
   const int64_t slots = p.c.slots();
-  auto units_of = [&](int64_t at) -> uint32_t { return at < 0 ? 1 : at >= slots ? 1 : (uint32_t)(at / kUnit) + 1; };
+  auto units_of = [&](int64_t at) -> uint32_t { return at < 0 ? 1 : at >= slots ? 1 : (uint32_t)(at / UNIT) + 1; };
   const uint32_t heads = p.c.kv_heads * p.tiles, hh = blockIdx.x % heads, ticket = blockIdx.x / heads;
   const int h = hh / p.tiles, tile = hh % p.tiles;
   const int64_t at0 = lane < p.batch ? p.position[lane] : 0;
   uint32_t all = lane < p.batch ? units_of(at0) : 0;
   for (int i = lane + 64; i < p.batch; i += 64) all += units_of(p.position[i]);
   all = lanes_sum(all);
-  const uint32_t most = max((uint32_t)(((uint64_t)all * heads + kPagedParts - 1) / kPagedParts), (uint32_t)kPagedLeast);
+  // Units of a part at the most.  A CU holds one workgroup, and takes `kStart` units' time to start it; the memory takes 1.4 times
+  // a CU's time for a 256th of the work.  So rounds of 256 workgroups, as few as cost the least (half a part of a sequence
+  // and head lies idle in the mean), and parts no smaller than they must be to fit in them.
+  uint32_t most = kPagedLeast;
+  if (p.batch > 64) {
+    most = max((uint32_t)(((uint64_t)all * heads + p.parts - 1) / p.parts), most);
+  } else {
+    const uint32_t n = lane < p.batch ? units_of(at0) : 0;
+    if (__any(n > most)) {
+      constexpr float kStart = D == 128 ? 10.0f : 20.0f;
+      const float work = (float)all * heads, pairs = (float)p.batch * heads;
+      float longest = (float)n;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) longest = fmaxf(longest, __shfl_xor(longest, d));
+      float least = INFINITY, size = 0.0f;
+      uint32_t room = 0;
+#pragma unroll
+      for (int k = 1; k <= kPagedParts / 256; ++k) {
+        const float m = fminf(longest, work * __builtin_amdgcn_rcpf(fmaxf(256.0f * k - 0.5f * pairs, 1.0f)));
+        const float cost = fmaxf(work * (1.4f / 256), k * (fmaxf(m, (float)kPagedLeast) + kStart));
+        if (256 * k >= pairs && cost < 0.95f * least) {
+          least = cost;
+          size = m;
+          room = 256 * k;
+        }
+      }
+      if (room == 0) {                    // more sequences and heads than that
+        room = ~0u;
+        size = work * (1.0f / kPagedParts);
+      }
+      most = max((uint32_t)size + 1, most);
+      for (int i = 0; i < 4 && lanes_sum((n + most - 1) / most) * heads > room; ++i) most += most / 8 + 1;
+    }
+  }
   uint32_t b = ~0u, part = 0, ahead = 0, parts_before = 0, units_before = 0;
   int64_t token = 0;
   for (int c = 0; c < p.batch; c += 64) {
@@ -203,14 +247,14 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   const uint32_t size = (n + parts - 1) / parts, from = part * size, to = min(n, from + size);
   const bool appends = p.k.data && to == n;
 
-  // Pages: lane l holds that of the wave's unit number l % 32 (from `held` on), its first chunk or, from lane 32 on, its second.
+  // Pages: lane l holds that of chunk l / PER of the wave's unit number l % PER (from a first one on).
   const int32_t *const table = p.c.table + b * p.c.table_stride;
   const int last_chunk = pos / kChunk;
   bool bad = false;
   auto pages_from = [&](int unit) {
-    const int chunk = 2 * (unit + (lane & 31) * W) + (lane >> 5);
+    const int chunk = C * (unit + lane % PER * W) + lane / PER;
     int id = 0;
-    if (chunk <= last_chunk && chunk < (int)(2 * to)) {
+    if (chunk <= last_chunk && chunk < (int)(C * to)) {
       id = table[chunk >> p.c.shift];
       if ((unsigned)id >= (unsigned)p.c.pages) {
         id = 0;
@@ -221,29 +265,33 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   };
   int unit = (int)from + wave, step = 0;
   int ids = pages_from(unit);
-  const T *kc[2], *vc[2];
-  x8 kn[2][U];
-  x4 vn[2][DT];
+  // Every load is 1 KB of whole lines of one chunk (lanes with 64 bytes of 16 rows each take the address unit more than twice as
+  // long).  Of the keys of two chunks, 32 slots, product s has 8 rows of each, slots 8 q + 4 s + r (r = 0 .. 3) of the 8 q from
+  // row 4 q on: half a line by lanes j < 8, the other by j >= 8, who then swap.  The lanes (., g) thus get the scores of
+  // slots 8 g .. 8 g + 7 in the two products.  Of the values, two tiles of 16 dims by halves of the wave, swapped likewise.
+  const int kd = (8 * (j / 4 % 2) + j % 4) * D + 32 * (j / 8) + 8 * g, vd = (16 * (g / 2) + j) * kChunk + 8 * (g % 2);
+  const T *kc[C], *vc[C];
+  u4 kn[C][U], vn[C][DT / 2];             // [chunk][4-slot product s, 64 dims], [chunk][32 dims]
   auto find = [&](int unit, int step) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int id = __builtin_amdgcn_readlane(ids, step + 32 * t);
-      const size_t at = p.c.template chunk<D>(id, h, 2 * unit + t);
+    for (int t = 0; t < C; ++t) {
+      const int id = __builtin_amdgcn_readlane(ids, step + PER * t);
+      const size_t at = p.c.template chunk<D>(id, h, C * unit + t);
       kc[t] = p.c.keys + at;
       vc[t] = p.c.values + at;
     }
   };
   auto fetch_keys = [&]() {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < C; ++t)
 #pragma unroll
-      for (int u = 0; u < U; ++u) kn[t][u] = *reinterpret_cast<const x8 *>(kc[t] + j * D + 32 * u + 8 * g);
+      for (int u = 0; u < U; ++u) kn[t][u] = *reinterpret_cast<const u4 *>(kc[t] + kd + (u & 1) * 4 * D + u / 2 * 64);
   };
   auto fetch_values = [&]() {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < C; ++t)
 #pragma unroll
-      for (int d = 0; d < DT; ++d) vn[t][d] = *reinterpret_cast<const x4 *>(vc[t] + (16 * d + j) * kChunk + 4 * g);
+      for (int d = 0; d < DT / 2; ++d) vn[t][d] = *reinterpret_cast<const u4 *>(vc[t] + vd + d * 32 * kChunk);
   };
   if (unit < (int)to) {
     find(unit, 0);
@@ -300,56 +348,78 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   for (int d = 0; d < DT; ++d) acc[d] = zero;
   float ref = kPagedLowest, total = 0.0f;
   for (; unit < (int)to; unit += W) {
-    const int base = unit * kUnit, next = unit + W;
-    const bool edge = base + kUnit > pos;
-    if (edge && appends) {
+    const int base = unit * UNIT, next = unit + W;
+    const bool edge = base + UNIT > pos;
+    f4 s[C];                              // s[2 t + i]: slots base + 32 t + 8 g + 4 i ..
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (base + kChunk * t + j == pos)
+    for (int t = 0; t < C; t += 2)
 #pragma unroll
-          for (int u = 0; u < U; ++u) kn[t][u] = *reinterpret_cast<const x8 *>(&rows_[R][32 * u + 8 * g]);
-    }
-    f4 s[2] = {zero, zero};
+      for (int i = 0; i < 2; ++i) {
+        const bool fresh = edge && appends && base + 16 * t + 8 * (j / 4) + 4 * i + j % 4 == pos;
+        s[t + i] = zero;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+        for (int u = 0; u < U; u += 2) {  // 64 dims
+          u4 a[2];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if constexpr (TURNED) s[t] = Of16<T>::mma(kn[t][u], ql[u], s[t]);
-        s[t] = Of16<T>::mma(kn[t][u], q[u], s[t]);
+          for (int e = 0; e < 4; ++e) {
+            a[0][e] = __builtin_amdgcn_update_dpp(kn[t][u + i][e], kn[t + 1][u + i][e], 0x128, 0xF, 0xC, false);   // row_ror 8, lanes 8 .. 15
+            a[1][e] = __builtin_amdgcn_update_dpp(kn[t + 1][u + i][e], kn[t][u + i][e], 0x128, 0xF, 0x3, false);   // lanes 0 .. 7
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const x8 k = __builtin_bit_cast(x8, fresh ? *reinterpret_cast<const u4 *>(&rows_[R][32 * (u + c) + 8 * g]) : a[c]);
+            if constexpr (TURNED) s[t + i] = Of16<T>::mma(k, ql[u + c], s[t + i]);
+            s[t + i] = Of16<T>::mma(k, q[u + c], s[t + i]);
+          }
+        }
+        s[t + i] *= p.scale;              // (before the mask: the scale may be 0 or negative)
       }
-      s[t] *= p.scale;                    // (before the mask: the scale may be 0 or negative)
-    }
-    ++step;
-    if (step == 32) {                     // the pages of the next 32 units
+    if (++step == PER) {                  // the pages of the next units
       ids = pages_from(next);
       step = 0;
     }
-    x4 vf[2][DT];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int d = 0; d < DT; ++d) vf[t][d] = vn[t][d];
     if (next < (int)to) {
       find(next, step);
       fetch_keys();
     }
-    if (edge) {
+    x8 vf[C / 2][DT];                     // 8 slots base + 32 t + 8 g .. of dim 16 d + j
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < C; t += 2)
+#pragma unroll
+      for (int d = 0; d < DT; d += 2) {
+        u4 lo, hi;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int slot = base + kChunk * t + 4 * g + e;
-          if (slot > pos) s[t][e] = -INFINITY;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            if (slot > pos) vf[t][d][e] = (T)0.0f;
-            if (appends && slot == pos) vf[t][d][e] = rows_[R + 1][16 * d + j];
-          }
+          const auto two = __builtin_amdgcn_permlane32_swap(vn[t][d / 2][e], vn[t + 1][d / 2][e], false, false);
+          lo[e] = two[0];
+          hi[e] = two[1];
         }
+        vf[t / 2][d] = __builtin_bit_cast(x8, lo);
+        vf[t / 2][d + 1] = __builtin_bit_cast(x8, hi);
+      }
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < C / 2; ++t) {
+        const int there = pos + 1 - (base + 32 * t + 8 * g), held = there - (appends ? 1 : 0);   // slots that there are, and values held
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e >= there) s[2 * t + e / 4][e % 4] = -INFINITY;
+        u4 mask, mine;                    // of the values: what is kept, and where the new one goes
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          mask[e] = (2 * e < held ? 0xFFFFu : 0u) | (2 * e + 1 < held ? 0xFFFF0000u : 0u);
+          mine[e] = !appends || held < 2 * e || held > 2 * e + 1 ? 0u : held & 1 ? 0xFFFF0000u : 0xFFFFu;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const uint32_t fresh = __builtin_bit_cast(uint16_t, rows_[R + 1][16 * d + j]) * 0x10001u;
+          vf[t][d] = __builtin_bit_cast(x8, (__builtin_bit_cast(u4, vf[t][d]) & mask) | (mine & fresh));
+        }
+      }
     }
     float top = kPagedLowest;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < C; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][e]);
     if (__any(top - ref > kPagedLift + kPagedSlack)) {
@@ -360,15 +430,20 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= shrink;
     }
-    x8 x;
+    x8 x[C / 2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = (T)__builtin_amdgcn_exp2f(s[e / 4][e % 4] - ref);
-      total += (float)x[e];
-    }
+    for (int t = 0; t < C; ++t)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-      acc[d] = Of16<T>::mma(__builtin_shufflevector(vf[0][d], vf[1][d], 0, 1, 2, 3, 4, 5, 6, 7), x, acc[d]);
+      for (int e = 0; e < 4; ++e) {
+        const T prob = (T)__builtin_amdgcn_exp2f(s[t][e] - ref);
+        x[t / 2][t % 2 * 4 + e] = prob;
+        total += (float)prob;
+      }
+#pragma unroll
+    for (int t = 0; t < C; t += 2)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        acc[d] = Of16<T>::mma(vf[t / 2][d], x[t / 2], acc[d]);
     if (next < (int)to) fetch_values();
   }
   if (__any(bad)) total = __builtin_nanf("");

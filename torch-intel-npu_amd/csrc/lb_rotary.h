@@ -29,51 +29,48 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams<T> p) {
   const int lane = rest / pieces, piece = rest % pieces;
   const int b = row / p.seq, i = row % p.seq;
   const int all = p.heads[0] + p.heads[1];
-  if (piece >= turned) {                  // dims that do not turn
-    const int dim = p.turn.dims + (piece - turned) * 2 * V;
-    for (int h = lane; h < all; h += p.lanes) {
-      const int s = h >= p.heads[0], hs = s ? h - p.heads[0] : h;
-      const T *in = (s ? p.x[1] : p.x[0]).at(b, i, hs) + dim;
-      T *out = (s ? p.out[1] : p.out[0]).at(b, i, hs) + dim;
-      const Piece v = *reinterpret_cast<const Piece *>(in);
-      if (dim + V < p.dim) *reinterpret_cast<Piece *>(out + V) = *reinterpret_cast<const Piece *>(in + V);
-      *reinterpret_cast<Piece *>(out) = v;
-    }
-    return;
-  }
-  const double position = (double)(p.per_row ? p.position[row] : p.position[b] + i);
+  // A piece's two halves: the dims of its pairs, or 2 V of those that do not turn (the last one's second half may be none).
+  const bool turns = piece < turned;
+  const int first = !turns ? p.turn.dims + (piece - turned) * 2 * V : p.turn.neighbours ? 2 * V * piece : V * piece;
+  const int step = turns && !p.turn.neighbours ? p.turn.dims / 2 : V;
+  const bool both = first + step < p.dim;
   float c[V], s[V];
+  if (turns) {
+    const double position = (double)(p.per_row ? p.position[row] : p.position[b] + i);
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float2 cs = turn_of(p.turn, piece * V + e, position);
-    c[e] = cs.x;
-    s[e] = p.back ? -cs.y : cs.y;
+    for (int e = 0; e < V; ++e) {
+      const float2 cs = turn_of(p.turn, piece * V + e, position);
+      c[e] = cs.x;
+      s[e] = p.back ? -cs.y : cs.y;
+    }
   }
-  const int first = p.turn.neighbours ? 2 * V * piece : V * piece, step = p.turn.neighbours ? V : p.turn.dims / 2;
   for (int h = lane; h < all; h += p.lanes) {
     const int side = h >= p.heads[0], hs = side ? h - p.heads[0] : h;
     const T *in = (side ? p.x[1] : p.x[0]).at(b, i, hs) + first;
     T *out = (side ? p.out[1] : p.out[0]).at(b, i, hs) + first;
-    Piece lo = *reinterpret_cast<const Piece *>(in), hi = *reinterpret_cast<const Piece *>(in + step);
-    if (!p.turn.neighbours || V == 1) {
+    Piece lo = *reinterpret_cast<const Piece *>(in), hi = {};
+    if (both) hi = *reinterpret_cast<const Piece *>(in + step);
+    if (turns) {
+      if (!p.turn.neighbours || V == 1) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float x = (float)lo[e], y = (float)hi[e];
-        lo[e] = (T)(x * c[e] - y * s[e]);
-        hi[e] = (T)(y * c[e] + x * s[e]);
-      }
-    } else {
+        for (int e = 0; e < V; ++e) {
+          const float x = (float)lo[e], y = (float)hi[e];
+          lo[e] = (T)(x * c[e] - y * s[e]);
+          hi[e] = (T)(y * c[e] + x * s[e]);
+        }
+      } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {       // pairs of lo, then of hi
-        Piece &v = e < V / 2 ? lo : hi;
-        constexpr int mask = V - 1;
-        const float x = (float)v[2 * e & mask], y = (float)v[(2 * e + 1) & mask];
-        v[2 * e & mask] = (T)(x * c[e] - y * s[e]);
-        v[(2 * e + 1) & mask] = (T)(y * c[e] + x * s[e]);
+        for (int e = 0; e < V; ++e) {     // pairs of lo, then of hi
+          Piece &v = e < V / 2 ? lo : hi;
+          constexpr int mask = V - 1;
+          const float x = (float)v[2 * e & mask], y = (float)v[(2 * e + 1) & mask];
+          v[2 * e & mask] = (T)(x * c[e] - y * s[e]);
+          v[(2 * e + 1) & mask] = (T)(y * c[e] + x * s[e]);
+        }
       }
     }
     *reinterpret_cast<Piece *>(out) = lo;
-    *reinterpret_cast<Piece *>(out + step) = hi;
+    if (both) *reinterpret_cast<Piece *>(out + step) = hi;
   }
 }
 

@@ -180,13 +180,33 @@ class Rotary:
             raise ValueError('scale must be finite')
         self.frequencies, self.pairs, self.scale = frequencies, pairs, float(scale)
         self.dims, self.device = 2 * frequencies.numel(), frequencies.device
+        self._bound()
+
+    def _bound(self):
+        """What calls are given of it."""
+        self.__dict__['_bytes'] = _ROTATION.pack(self.frequencies.data_ptr(), self.dims, PAIRS[self.pairs], self.scale, 0)
+
+    def __setattr__(self, name, value):
+        """Fixed: its address and values are in what calls are given."""
+        if '_bytes' in self.__dict__:
+            raise AttributeError(f'{name}: a Rotary is fixed; make another')
+        super().__setattr__(name, value)
+
+    def __getstate__(self):
+        """Copies and pickles have frequencies of their own."""
+        return {name: value for name, value in self.__dict__.items() if name != '_bytes'}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.__dict__['device'] = self.frequencies.device
+        self._bound()
 
     def _packed(self, device, head_dim):
         if self.device != device:
             raise ValueError(f'the frequencies must be on {device} with the rest (found {self.device})')
         if self.dims > head_dim:
             raise ValueError(f'{self.dims} dims turn, but heads have {head_dim}')
-        return _ROTATION.pack(self.frequencies.data_ptr(), self.dims, PAIRS[self.pairs], self.scale, 0)
+        return self._bytes
 
 
 def _rotation(rotary, device, head_dim):
@@ -197,41 +217,41 @@ def _rotation(rotary, device, head_dim):
     return rotary._packed(device, head_dim)
 
 
-def _head_rows(t, name, like, heads):
-    """Rows of heads of contiguous values, at any alignment."""
-    if (not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.ndim != 4 or t.shape[:2] != like.shape[:2]
-            or t.shape[3] != like.shape[3] or (heads is not None and t.shape[2] != heads) or t.numel() == 0):
-        raise ValueError(f'{name} must be {like.dtype} [batch, seq, heads, head_dim] = [{like.shape[0]}, {like.shape[1]}, '
-                         f'{"heads" if heads is None else heads}, {like.shape[3]}]')
-    if t.device != like.device:
-        raise ValueError(f'{name} must be on {like.device} with q (found {t.device})')
-    if t.stride(3) != 1 and t.shape[3] > 1:
+def _head_rows(t, name, shape, dtype, device):
+    """(address, strides) of rows of heads of contiguous values, at any alignment."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape:
+        raise ValueError(f'{name} must be {dtype} [batch, seq, heads, head_dim] = {list(shape)}')
+    if t.device != device:
+        raise ValueError(f'{name} must be on {device} with q (found {t.device})')
+    b, i, h, d = t.stride()
+    if d != 1 and shape[3] > 1:
         raise ValueError(f'the heads of {name} must be contiguous')
-    b, i, h, _ = t.stride()
     return t.data_ptr(), b, i, h
 
 
 def _rotary_args(q, position, rotary, out, k, out_k, back):
-    if not isinstance(q, torch.Tensor) or q.device.type != 'cuda' or q.dtype not in TYPES or q.ndim != 4 or q.numel() == 0:
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in TYPES or q.ndim != 4 or q.numel() == 0:
         raise ValueError('q must be fp16, bf16 or fp32 [batch, seq, heads, head_dim] on a ROCm device')
     if not isinstance(rotary, Rotary):
         raise ValueError('rotary must be a Rotary')
+    shape, dtype, device = q.shape, q.dtype, q.device
+    batch, seq, heads, dim = shape
     if (k is None) != (out_k is None):
         raise ValueError('k and out_k go together')
-    batch, seq, heads, dim = q.shape
-    rows = _head_rows(q, 'q', q, None) + _head_rows(out, 'out', q, heads)
-    k_heads = 0
-    if k is not None:
-        rows += _head_rows(k, 'k', q, None)
-        k_heads = k.shape[2]
-        rows += _head_rows(out_k, 'out_k', q, k_heads)
+    q, out = _head_rows(q, 'q', shape, dtype, device), _head_rows(out, 'out', shape, dtype, device)
+    if k is None:
+        k_heads, k, out_k = 0, _NO_ROWS, _NO_ROWS
     else:
-        rows += _NO_ROWS + _NO_ROWS
+        if not isinstance(k, torch.Tensor) or k.ndim != 4 or k.numel() == 0:
+            raise ValueError(f'k must be {dtype} [batch, seq, heads, head_dim]')
+        k_heads = k.shape[2]
+        shape = (batch, seq, k_heads, dim)
+        k, out_k = _head_rows(k, 'k', shape, dtype, device), _head_rows(out_k, 'out_k', shape, dtype, device)
     per_row = isinstance(position, torch.Tensor) and position.ndim == 2
-    at = _counts(position, 'position', (batch, seq) if per_row else (batch,), q.device)
+    at = _counts(position, 'position', (batch, seq) if per_row else (batch,), device)
     return RotaryArgs.from_buffer_copy(_ROTARY.pack(
-        ctypes.sizeof(RotaryArgs), TYPES[q.dtype], batch, seq, dim, heads, k_heads, *rows, at, per_row, bool(back))
-        + rotary._packed(q.device, dim))
+        ctypes.sizeof(RotaryArgs), TYPES[dtype], batch, seq, dim, heads, k_heads, *q, *out, *k, *out_k, at, per_row, bool(back))
+        + rotary._packed(device, dim))
 
 
 def rotary(q, position, rotary, *, k=None, out=None, out_k=None, back=False):
