@@ -598,7 +598,7 @@ typedef struct lb_adapters_args {
   size_t workspace_bytes;
 } lb_adapters_args;
 
-/* Bytes of workspace lb_adapters needs for these sizes; host-only. */
+/* Bytes of workspace lb_adapters needs for these sizes (0 when none); host-only. */
 lb_status lb_adapters_workspace_bytes(const lb_adapters_args *args, size_t *bytes);
 
 /* x A^T in fp32, taken as a sum of two 16-bit numbers into the product with B; sums in fp32, out rounded once. */

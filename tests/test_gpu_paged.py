@@ -105,6 +105,10 @@ CASES = [
     ('fp16', 9, 3, 64, 64, [5003]),
     ('bf16', 8, 2, 128, 16, [9001, 20]),
     ('fp16', 3, 3, 64, 16, [(b * 37) % 90 + 1 for b in range(70)]),
+    ('fp16', 8, 8, 64, 64, [100 + (b * 7919) % 3500 for b in range(18)]),
+    ('bf16', 6, 2, 128, 16, [1 + (b * 7919) % 2500 for b in range(40)]),
+    ('fp16', 16, 16, 64, 32, [2100, 900] + [1 + b % 40 for b in range(62)]),
+    ('bf16', 16, 16, 64, 32, [2100] + [1 + b % 40 for b in range(69)]),
     ('bf16', 4, 1, 64, 32, [1 + (b % 7) * 400 * (b % 31 == 0) + b % 50 for b in range(200)]),
 ]
 

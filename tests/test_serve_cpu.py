@@ -119,8 +119,9 @@ BAD_ADAPTERS = [
     (dict(up=0x200008), 'up must'), (dict(scales=0x300002), 'scales'), (dict(index=0), 'index'), (dict(x=0x400002), 'x must'),
     (dict(ldx=580), 'strides of x'), (dict(y=0), 'y must'), (dict(out=0x600001), 'out must'), (dict(ldo=575), 'rows of out overlap'),
     (dict(out=0x500002), 'out overlaps y'), (dict(out=0x500000, ldo=640), 'out overlaps y'), (dict(out=0x400000), 'out overlaps x'),
-    (dict(out=0x310000), 'out overlaps'), (dict(workspace=0), 'workspace'), (dict(workspace=0x700010), 'workspace'),
-    (dict(workspace_bytes=255), 'workspace'), (dict(workspace=0x500000), 'workspace overlaps y'), (dict(workspace=0x600000), 'out overlaps workspace'),
+    (dict(out=0x310000), 'out overlaps'), (dict(M=200, workspace=0), 'workspace'), (dict(M=200, workspace=0x700010), 'workspace'),
+    (dict(M=200, workspace_bytes=12799), 'workspace'), (dict(M=200, workspace=0x500000), 'workspace overlaps y'),
+    (dict(M=200, workspace=0x600000), 'out overlaps workspace'),
 ]
 
 
@@ -164,7 +165,8 @@ def test_workspaces():
     assert ask('lb_paged_attention_workspace_bytes', attention(table__longest=10 ** 5)) == 0
     assert lb.ZEROED_WORKSPACE_BYTES < size.value < 64 << 20
     assert ask('lb_paged_attention_workspace_bytes', attention(heads=10)) == 1 and size.value == 0
-    assert ask('lb_adapters_workspace_bytes', adapters()) == 0 and size.value >= 20 * 16 * 4
+    assert ask('lb_adapters_workspace_bytes', adapters()) == 0 and size.value == 0      # both products in one launch
+    assert ask('lb_adapters_workspace_bytes', adapters(K=4096)) == 0 and size.value >= 20 * 16 * 4
     assert ask('lb_adapters_workspace_bytes', adapters(rank=9)) == 1 and size.value == 0
 
 

@@ -27,7 +27,7 @@ AdaptersPlan adapters_plan(const lb_adapters_args *a) {
     plan.tiles = tiles16;
     plan.span = 256;
     plan.shares = (int)most;
-    plan.bytes = 256;
+    plan.bytes = 0;
     return plan;
   }
   // Tiles of 64 rows (of 32 with ranks past 64, whose sums fill the registers), and parts of K until there is a workgroup a CU.
@@ -143,9 +143,9 @@ lb_status lb_adapters(const lb_adapters_args *a, void *stream) {
   if (const lb_status st = check_matrix(what, "y", a->y, a->M, a->N, a->ldy, false, false, reads[5]); st != LB_OK) return st;
   if (const lb_status st = check_matrix(what, "out", a->out, a->M, a->N, a->ldo, false, true, writes[0]); st != LB_OK) return st;
   const AdaptersPlan plan = adapters_plan(a);
-  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < plan.bytes)
+  if (plan.bytes && (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < plan.bytes))
     return fail(LB_INVALID_ARGUMENT, "%s: a 256-byte aligned workspace of %zu bytes required (got %zu)", what, plan.bytes, a->workspace_bytes);
-  writes[1] = range_of(a->workspace, plan.bytes, "workspace");
+  if (plan.bytes) writes[1] = range_of(a->workspace, plan.bytes, "workspace");
   const bool in_place = a->out == a->y && (a->M == 1 || a->ldo == a->ldy);
   if (const lb_status st = check_apart(what, writes, 2, reads, 5); st != LB_OK) return st;
   if (const lb_status st = check_apart(what, in_place ? writes + 1 : writes, in_place ? 1 : 2, reads + 5, 1); st != LB_OK) return st;

@@ -134,7 +134,7 @@ struct PagedAttendParams {
   Turn turn;
   uint32_t *tickets;        // kPagedParts zero words
   float *partial;           // [places][16][D] sums, then [places][16][2] references and totals
-  uint32_t parts;           // batches past 64: parts that the work is split into at the most, besides sequences and heads
+  int rounds;               // of 256 workgroups, besides those of sequences and heads: what the grid has
   int batch, group, tiles;  // group: query heads of a KV head; tiles of up to 16 of them
   float scale;              // score scale * log2(e)
 };
@@ -185,10 +185,11 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   all = lanes_sum(all);
   // Units of a part at the most.  A CU holds one workgroup, and takes `kStart` units' time to start it; the memory takes 1.4 times
   // a CU's time for a 256th of the work.  So rounds of 256 workgroups, as few as cost the least (half a part of a sequence
-  // and head lies idle in the mean), and parts no smaller than they must be to fit in them.
+  // and head lies idle in the mean), and parts no smaller than they must be to fit in them.  (Parts are never more than
+  // sequences times heads and 256 rounds: each sequence has less than one part over what its share of the work is.)
   uint32_t most = kPagedLeast;
   if (p.batch > 64) {
-    most = max((uint32_t)(((uint64_t)all * heads + p.parts - 1) / p.parts), most);
+    most = max((uint32_t)(((uint64_t)all * heads + 256 * p.rounds - 1) / (256 * p.rounds)), most);
   } else {
     const uint32_t n = lane < p.batch ? units_of(at0) : 0;
     if (__any(n > most)) {
@@ -199,8 +200,7 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
       for (int d = 32; d > 0; d >>= 1) longest = fmaxf(longest, __shfl_xor(longest, d));
       float least = INFINITY, size = 0.0f;
       uint32_t room = 0;
-#pragma unroll
-      for (int k = 1; k <= kPagedParts / 256; ++k) {
+      for (int k = 1; k <= p.rounds; ++k) {
         const float m = fminf(longest, work * __builtin_amdgcn_rcpf(fmaxf(256.0f * k - 0.5f * pairs, 1.0f)));
         const float cost = fmaxf(work * (1.4f / 256), k * (fmaxf(m, (float)kPagedLeast) + kStart));
         if (256 * k >= pairs && cost < 0.95f * least) {
@@ -211,7 +211,7 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
       }
       if (room == 0) {                    // more sequences and heads than that
         room = ~0u;
-        size = work * (1.0f / kPagedParts);
+        size = work / (256.0f * p.rounds);
       }
       most = max((uint32_t)size + 1, most);
       for (int i = 0; i < 4 && lanes_sum((n + most - 1) / most) * heads > room; ++i) most += most / 8 + 1;

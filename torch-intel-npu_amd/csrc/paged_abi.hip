@@ -62,7 +62,7 @@ void with_kind(const lb_paged_cache &c, F &&f) {
 }
 
 struct AttendPlan {
-  int tiles, parts;
+  int tiles, rounds;
   int64_t grid;
   size_t bytes;
 };
@@ -71,12 +71,13 @@ AttendPlan attend_plan(const lb_paged_attention_args *a) {
   AttendPlan plan{};
   const lb_paged_cache &c = a->cache;
   plan.tiles = (int)((a->heads / c.kv_heads + 15) / 16);
-  const int64_t heads = c.kv_heads * plan.tiles, unit = kUnit;
-  const int64_t units = (a->table.longest * c.page + unit - 1) / unit;
-  plan.parts = (int)std::min<int64_t>(kPagedParts, 256 + heads * a->batch);
-  // A workgroup per sequence and head, and where sequences can be long enough as many again as they can be split into.
+  const int64_t heads = c.kv_heads * plan.tiles, pairs = heads * a->batch, units = (a->table.longest * c.page + kUnit - 1) / kUnit;
+  // A workgroup per sequence and head, and where sequences can be long enough the rounds of 256 that they can be split into: few
+  // sequences are split evenly in one, more of them need more to end together.
   const bool split = units > kPagedLeast;
-  plan.grid = heads * (a->batch + (split ? (plan.parts + heads - 1) / heads : 0));
+  plan.rounds = pairs <= 64 ? 1 : pairs <= 128 ? 2 : kPagedParts / 256;
+  plan.grid = pairs + (split ? 256 * plan.rounds : 0);
+  plan.grid = (plan.grid + heads - 1) / heads * heads;   // whole tickets
   plan.bytes = split ? LB_ZEROED_WORKSPACE_BYTES + (size_t)kPagedPlaces * 16 * (c.head_dim + 2) * sizeof(float) : 0;
   return plan;
 }
@@ -184,7 +185,7 @@ lb_status lb_paged_attention(const lb_paged_attention_args *a, void *stream) {
     p.turn = turn_params(a->rotation);
     p.tickets = static_cast<uint32_t *>(a->workspace);
     p.partial = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + LB_ZEROED_WORKSPACE_BYTES);
-    p.parts = plan.parts;
+    p.rounds = plan.rounds;
     p.batch = (int)a->batch;
     p.group = (int)(a->heads / c.kv_heads);
     p.tiles = plan.tiles;

@@ -560,8 +560,9 @@ def adapters_add(y, x, adapters, index, *, out=None):
     out = y if out is None else out
     keep = []
     a, need = _adapters_args(y, x, adapters, index, out, keep, True)
-    workspace = torch.empty(need, dtype=torch.uint8, device=adapters.device)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), need
+    if need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=adapters.device)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
     _kv_run(library().lb_adapters, a, adapters.device, 'lb_adapters')
     return out
 
@@ -574,7 +575,9 @@ class PreparedAdapters(_PreparedKV):
     def __init__(self, y, x, adapters, index, out=None):
         out = y if out is None else out
         a, need = _adapters_args(y, x, adapters, index, out, None, False)
-        workspace = torch.empty(need, dtype=torch.uint8, device=adapters.device)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), need
-        self._bind('lb_adapters', 'lb_adapters', a, adapters.device, [y, x, adapters, index, out, workspace])
+        keep = [y, x, adapters, index, out]
+        if need:
+            keep.append(torch.empty(need, dtype=torch.uint8, device=adapters.device))
+            a.workspace, a.workspace_bytes = keep[-1].data_ptr(), need
+        self._bind('lb_adapters', 'lb_adapters', a, adapters.device, keep)
         self.out = out
