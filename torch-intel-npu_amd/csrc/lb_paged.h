@@ -153,6 +153,17 @@ constexpr float kPagedLift = 10.0f, kPagedSlack = 4.0f;
 // Sum over the wave's lanes.
 __device__ __forceinline__ uint32_t lanes_sum(uint32_t x) { return __builtin_amdgcn_readlane(kv_scan(x), 63); }
 
+// The largest of them.
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x111, 0xF, 0xF, true));   // row_shr 1, 2, 4, 8
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x112, 0xF, 0xF, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x114, 0xF, 0xF, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x118, 0xF, 0xF, true));
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x142, 0xA, 0xF, false));  // row_bcast 15, 31
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0u, x, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
 // One new token a sequence.  A workgroup takes a part of a sequence's slots for a KV head (and up to 16 of its query heads),
 // its W waves every W-th unit of slots each with a reference and total of their own, joined in LDS; parts are joined by
 // the workgroup that counts last.  Which part it takes is found from the positions, on the device.
@@ -195,9 +206,7 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
     if (__any(n > most)) {
       constexpr float kStart = D == 128 ? 10.0f : 20.0f;
       const float work = (float)all * heads, pairs = (float)p.batch * heads;
-      float longest = (float)n;
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) longest = fmaxf(longest, __shfl_xor(longest, d));
+      const float longest = (float)lanes_max(n);
       float least = INFINITY, size = 0.0f;
       uint32_t room = 0;
       for (int k = 1; k <= p.rounds; ++k) {

@@ -75,7 +75,7 @@ AttendPlan attend_plan(const lb_paged_attention_args *a) {
   // A workgroup per sequence and head, and where sequences can be long enough the rounds of 256 that they can be split into: few
   // sequences are split evenly in one, more of them need more to end together.
   const bool split = units > kPagedLeast;
-  plan.rounds = pairs <= 64 ? 1 : pairs <= 128 ? 2 : kPagedParts / 256;
+  plan.rounds = pairs <= 128 ? 1 : kPagedParts / 256;
   plan.grid = pairs + (split ? 256 * plan.rounds : 0);
   plan.grid = (plan.grid + heads - 1) / heads * heads;   // whole tickets
   plan.bytes = split ? LB_ZEROED_WORKSPACE_BYTES + (size_t)kPagedPlaces * 16 * (c.head_dim + 2) * sizeof(float) : 0;
