@@ -287,10 +287,14 @@ class QuantizedLinear(torch.nn.Module):
             self._bias_device[key] = torch.frombuffer(bytearray(self._bias), dtype=torch.float16).to(device)
         return self._bias_device[key]
 
-    def forward(self, x):
+    def forward(self, x, adapters=None, index=None):
         """y = x . W^T (+ bias) in fp16 (reference :339-360).  compact_groups selects the per-group
         fp16 products and balanced add tree of the reference's compact graph (:235-256);
-        activation_scale selects W8A8 (:224-231), int8 activations on that power-of-two grid."""
+        activation_scale selects W8A8 (:224-231), int8 activations on that power-of-two grid.
+        With adapters (lowbit_hip.Adapters of this weight's shape, fp16) each row also gets what the adapter
+        index[m] adds to it (int64 [M] on the device, -1: none; lowbit_hip.adapters_add)."""
+        if (adapters is None) != (index is None):
+            raise ValueError('adapters and index go together')
         _validate_activation(x, self._weight.shape[1])
         call = self._bound.get(x.device)
         if call is None:
@@ -300,4 +304,5 @@ class QuantizedLinear(torch.nn.Module):
             call = self._bound[x.device] = lowbit_hip.BoundLinear(
                 codes, scales, format=self._weight.format, N=n, K=k, group_size=self._weight.group_size,
                 bias=self._device_bias(x.device), flags=flags, activation_scale=self._activation_scale)
-        return call(x)
+        y = call(x)
+        return y if adapters is None else lowbit_hip.adapters_add(y, x, adapters, index)
