@@ -91,14 +91,14 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
   typedef std::integral_constant<int, 4> Four;
   typedef std::integral_constant<int, 8> Eight;
   if (plan.fused) {
-    const dim3 grid((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares);
+    const dim3 grid((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares + 1);
     auto go = [&](auto rt) { hipLaunchKernelGGL((adapters_rows_kernel<T, decltype(rt)::value>), grid, dim3(64 * kRowsWaves), 0, s, p); };
     a->rank <= 16 ? go(One{}) : a->rank <= 32 ? go(Two{}) : go(Four{});
     return;
   }
   const int64_t wide = plan.span * (4 / plan.stack), rows = 16 * plan.stack;   // of a workgroup of adapters_up_kernel
   const dim3 down((unsigned)(plan.tiles * plan.slices), (unsigned)plan.shares);
-  const dim3 up((unsigned)((a->M + rows - 1) / rows * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up);
+  const dim3 up((unsigned)((a->M + rows - 1) / rows * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up + 1);
   const dim3 tile((unsigned)((a->M + 63) / 64 * ((a->N + plan.span - 1) / plan.span)));
   auto go = [&](auto rt, auto mt) {
     constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;

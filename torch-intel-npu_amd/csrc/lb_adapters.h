@@ -10,7 +10,7 @@
 
 namespace lb {
 
-constexpr int kRowsWaves = 8;   // of a workgroup of adapters_rows_kernel
+constexpr int kRowsWaves = 8;   // of a workgroup of adapters_rows_kernel (16 spill, which makes every launch 5 us longer)
 
 template <class T>
 struct AdaptersParams {
@@ -58,36 +58,50 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
   const int slice = blockIdx.x % p.slices, first = blockIdx.x / p.slices * (16 * MT);
   const int id = adapter_of(p, first, lane, 16 * MT);
   const int all = (p.K + 63) / 64, size = (all + p.slices - 1) / p.slices, from = slice * size, to = min(all, from + size);
-  const x8 none = {};
   each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
     f4 acc[RT][MT] = {};
     const T *const down = p.down + (size_t)a * p.rank * p.K;
-    const T *dr[RT], *xr[MT];
+    const int row = j % 8, at = 32 * (j / 8) + 8 * g;       // (see rows_from_lines)
+    const T *dr[RT][2], *xr[MT][2];
+    bool live[MT][2];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) dr[r] = down + (size_t)min(16 * r + j, p.rank - 1) * p.K + 8 * g;
+    for (int b = 0; b < 2; ++b) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xr[t] = p.x + (size_t)min(first + 16 * t + j, p.M - 1) * p.ldx + 8 * g;
+      for (int r = 0; r < RT; ++r) dr[r][b] = down + (size_t)min(16 * r + 8 * b + row, p.rank - 1) * p.K + at;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        live[t][b] = mine >> (16 * t + 8 * b + row) & 1;
+        xr[t][b] = p.x + (size_t)min(first + 16 * t + 8 * b + row, p.M - 1) * p.ldx + at;
+      }
+    }
+    const u4 none = {0, 0, 0, 0};
     for (int piece = from + wave; piece < to; piece += W * AHEAD) {
-      x8 d[AHEAD][2][RT], x[AHEAD][2][MT];
+      u4 d[AHEAD][2][RT], x[AHEAD][2][MT];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int k = (piece + n * W) * 64 + 32 * c;
-          const bool there = piece + n * W < to && k + 8 * g < p.K;
+        for (int b = 0; b < 2; ++b) {
+          const int k = (piece + n * W) * 64;
+          const bool there = piece + n * W < to && k + at < p.K;
 #pragma unroll
-          for (int r = 0; r < RT; ++r) d[n][c][r] = there ? *reinterpret_cast<const x8 *>(dr[r] + k) : none;
+          for (int r = 0; r < RT; ++r) d[n][b][r] = there ? *reinterpret_cast<const u4 *>(dr[r][b] + k) : none;
 #pragma unroll
-          for (int t = 0; t < MT; ++t) x[n][c][t] = there && (mine >> (16 * t + j) & 1) ? *reinterpret_cast<const x8 *>(xr[t] + k) : none;
+          for (int t = 0; t < MT; ++t) x[n][b][t] = there && live[t][b] ? *reinterpret_cast<const u4 *>(xr[t][b] + k) : none;
         }
 #pragma unroll
-      for (int n = 0; n < AHEAD; ++n)
+      for (int n = 0; n < AHEAD; ++n) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) rows_from_lines(d[n][0][r], d[n][1][r]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) rows_from_lines(x[n][0][t], x[n][1][t]);
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) acc[r][t] = Of16<T>::mma(d[n][c][r], x[n][c][t], acc[r][t]);
+            for (int t = 0; t < MT; ++t)
+              acc[r][t] = Of16<T>::mma(__builtin_bit_cast(x8, d[n][c][r]), __builtin_bit_cast(x8, x[n][c][t]), acc[r][t]);
+      }
     }
     __syncthreads();                      // (what an earlier adapter left is read)
 #pragma unroll
@@ -106,22 +120,22 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
   });
 }
 
-// Rows of a tile without an adapter, and those whose adapter there is not: y's values or NaNs, outputs from .. to - 1, by the
-// lanes of a wave.
+// Rows of 16 without an adapter, and those whose adapter there is not: y's values or NaNs, outputs from .. to - 1, by the lanes of a
+// wave, 8 outputs a lane at once.
 template <class T>
-__device__ __forceinline__ void rows_without(const AdaptersParams<T> &p, int id, int rows, int first, int lane, int from, int to) {
+__device__ __forceinline__ void rows_without(const AdaptersParams<T> &p, int id, int first, int lane, int from, int to) {
   typedef typename Of16<T>::x8 x8;
-  uint64_t left = __ballot(lane < rows && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y));
-  while (left) {
-    const int row = __builtin_ctzll(left);
-    left &= left - 1;
-    const bool bad = __builtin_amdgcn_readlane(id, row) == -2;
-    const T *const y = p.y + (size_t)(first + row) * p.ldy;
-    T *const out = p.out + (size_t)(first + row) * p.ldo;
-    if (p.wide && !bad) {
-      for (int n = from + 8 * lane; n < to; n += 512) *reinterpret_cast<x8 *>(out + n) = *reinterpret_cast<const x8 *>(y + n);
+  if (!__ballot(lane < 16 && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y))) return;
+  const int pieces = (to - from + 7) / 8;
+  for (int i = lane; i < 16 * pieces; i += 64) {
+    const int row = i / pieces, n = from + 8 * (i - row * pieces), whose = __shfl(id, row);
+    if (first + row >= p.M || whose >= 0 || (whose == -1 && p.out == p.y)) continue;
+    const T *const y = p.y + (size_t)(first + row) * p.ldy + n;
+    T *const out = p.out + (size_t)(first + row) * p.ldo + n;
+    if (p.wide && whose == -1) {
+      *reinterpret_cast<x8 *>(out) = *reinterpret_cast<const x8 *>(y);
     } else {
-      for (int n = from + lane; n < to; n += 64) out[n] = bad ? (T)__builtin_nanf("") : y[n];
+      for (int e = 0; e < 8 && n + e < to; ++e) out[e] = whose == -1 ? y[e] : (T)__builtin_nanf("");
     }
   }
 }
@@ -277,7 +291,10 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
   const int first = (blockIdx.x / spans * p.stack + wave % p.stack) * 16;
   if (from >= to) return;
   const int id = adapter_of(p, first, lane, 16);
-  if (blockIdx.y == 0) rows_without(p, id, 16, first, lane, from, to);
+  if (blockIdx.y == p.shares_up) {        // (workgroups of their own, so that no product waits for it)
+    rows_without(p, id, first, lane, from, to);
+    return;
+  }
   each_adapter(id, blockIdx.y, p.shares_up, [&](int a, uint64_t mine) {
     const bool live = mine >> j & 1;
     const T *const up = p.up + (size_t)a * p.N * p.rank;
@@ -423,11 +440,10 @@ __global__ __launch_bounds__(64 * kRowsWaves) void adapters_rows_kernel(Adapters
   const int spans = (p.N + p.span - 1) / p.span;
   const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * 16;
   const int id = adapter_of(p, first, lane, 16), all = (p.K + 63) / 64;
-  if (blockIdx.y == 0) {
-    const int n = from + 64 * wave;       // (64 outputs a wave, so rows of spans past 1024 go round)
-    for (int n0 = n; n0 < to; n0 += 64 * W) rows_without(p, id, 16, first, lane, n0, min(to, n0 + 64));
+  if (blockIdx.y == p.shares) {           // (workgroups of their own, so that no product waits for it)
+    for (int n0 = from + 64 * wave; n0 < to; n0 += 64 * W) rows_without(p, id, first, lane, n0, min(to, n0 + 64));
+    return;
   }
-  const x8 none = {};
   each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
     const bool live = mine >> j & 1;
     const T *const up = p.up + (size_t)a * p.N * p.rank;
@@ -448,8 +464,8 @@ __global__ __launch_bounds__(64 * kRowsWaves) void adapters_rows_kernel(Adapters
           const int k = (piece + n * W) * 64 + 32 * c;
           const bool there = k + 8 * g < p.K;
 #pragma unroll
-          for (int r = 0; r < RT; ++r) d[n][c][r] = there ? *reinterpret_cast<const x8 *>(down + (size_t)min(16 * r + j, p.rank - 1) * p.K + k) : none;
-          xv[n][c] = there && live ? *reinterpret_cast<const x8 *>(x + k) : none;
+          for (int r = 0; r < RT; ++r) d[n][c][r] = there ? *reinterpret_cast<const x8 *>(down + (size_t)min(16 * r + j, p.rank - 1) * p.K + k) : x8{};
+          xv[n][c] = there && live ? *reinterpret_cast<const x8 *>(x + k) : x8{};
         }
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n)

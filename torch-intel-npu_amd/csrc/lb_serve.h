@@ -28,6 +28,18 @@ struct Rows {
   __device__ __forceinline__ T *at(int b, int i, int h) const { return data + b * batch + i * row + h * head; }
 };
 
+// 64 values of 16 rows as two operands of a product (lane (j, g): row j, values 8 g .. and 32 + 8 g ..), from two loads of whole lines:
+// a has rows 0 .. 7 and b rows 8 .. 15, values 8 g + 32 (j / 8) .. of row j % 8 of them.  (A load whose lanes have half a line of 16
+// rows each takes the address unit twice as long.)
+__device__ __forceinline__ void rows_from_lines(u4 &a, u4 &b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t x = a[e], y = b[e];
+    a[e] = __builtin_amdgcn_update_dpp(x, y, 0x128, 0xF, 0xC, false);   // row_ror 8 into lanes 8 .. 15
+    b[e] = __builtin_amdgcn_update_dpp(y, x, 0x128, 0xF, 0x3, false);   // into lanes 0 .. 7
+  }
+}
+
 // The rotation: pair i of the first `dims` dims turns by position * frequencies[i] (64 bits).
 struct Turn {
   const double *frequencies;   // null: nothing turns
