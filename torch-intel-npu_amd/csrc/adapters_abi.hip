@@ -12,10 +12,10 @@ using namespace lb::abi;
 namespace {
 
 struct AdaptersPlan {
-  bool fused;               // adapters_rows_kernel
-  int rows;                 // adapters_down_kernel: rows of a tile / 16
+  bool fused, tile;         // adapters_rows_kernel; adapters_tile_kernel
+  int rows, ranks, groups;  // adapters_down_kernel: rows and ranks of a tile / 16, groups of those ranks
   int64_t tiles;
-  int slices, shares, shares_up, span, stack;
+  int slices, shares, shares_up, span, wide_span, stack;   // (wide_span: of adapters_tile_kernel)
   size_t bytes;
 };
 
@@ -30,15 +30,24 @@ AdaptersPlan adapters_plan(const lb_adapters_args *a) {
     plan.bytes = 0;
     return plan;
   }
-  // Tiles of 64 rows (of 32 with ranks past 64, whose sums fill the registers), and parts of K until there is a workgroup a CU.
-  plan.rows = a->M < 1024 ? 1 : a->rank > 64 ? 2 : 4;
+  // Tiles of 64 rows and 64 ranks where x is large, so that it is read once (4096x4096 rank 128 of 3000 rows: 16, 32, 64 ranks a
+  // workgroup 68.4, 51.7, 47.0 us); elsewhere of 16 rows, and of 16 ranks where those are few, for more workgroups (rank 128
+  // of 40 rows 13.2, 14.3, 16.2 us; rank 64 of 827 rows 25.7, 22.9, 24.0).  Parts of K, of 1024 at the least, until there is a
+  // workgroup a CU (4096x14336 rank 32 of one row: 4, 8, 14 parts 13.5, 10.8, 10.3 us).
+  plan.rows = a->M * a->K < 3 << 21 ? 1 : 4;
   plan.tiles = (a->M + 16 * plan.rows - 1) / (16 * plan.rows);
-  plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / plan.tiles, (a->K + 511) / 512, 4}));
-  plan.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(a->count, 16 * plan.rows), 512 / (plan.tiles * plan.slices)));
+  const int64_t rank16 = (a->rank + 15) / 16;
+  plan.ranks = rank16 <= 1 ? 1 : plan.rows == 1 ? (a->M <= 256 ? 1 : 2) : rank16 <= 2 ? 2 : 4;
+  plan.groups = (int)((rank16 + plan.ranks - 1) / plan.ranks);
+  const int64_t alone = plan.tiles * plan.groups;
+  plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / alone, (a->K + 1023) / 1024, 16}));
+  plan.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(a->count, 16 * plan.rows), 512 / (alone * plan.slices)));
+  plan.tile = a->M >= 256;    // (4096x4096 rank 32: 500 rows 13.5 -> 12.0 us, 763 rows of 14336x4096 24.5 -> 18.7)
   plan.stack = tiles16 >= 4 ? 4 : tiles16 >= 2 ? 2 : 1;
   plan.shares_up = (int)(a->M < 1024 ? most : 1);
-  plan.span = 512;
-  while (plan.rows == 1 && plan.span > 128 && tiles16 * plan.shares_up * ((a->N + plan.span - 1) / plan.span) < 2048) plan.span /= 2;
+  plan.span = plan.wide_span = 512;
+  while (plan.span > (a->rank > 32 ? 64 : 128) && tiles16 * plan.shares_up * ((a->N + plan.span - 1) / plan.span) < 2048) plan.span /= 2;
+  while (plan.wide_span > 128 && (a->M + 63) / 64 * ((a->N + plan.wide_span - 1) / plan.wide_span) < 512) plan.wide_span /= 2;
   plan.bytes = ((size_t)plan.slices * a->M * a->rank * 4 + 255) / 256 * 256;
   return plan;
 }
@@ -51,7 +60,7 @@ lb_status check_sizes(const char *what, const lb_adapters_args *a) {
     return fail(LB_INVALID_ARGUMENT, "%s: rank must be a multiple of 8 up to %d", what, LB_ADAPTERS_MAX_RANK);
   if (a->count < 1 || a->count > (1 << 24)) return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^24 adapters required", what);
   const AdaptersPlan plan = adapters_plan(a);
-  if ((a->M + 15) / 16 * std::max<int64_t>(plan.slices, (a->N + plan.span - 1) / plan.span) > (1 << 23))   // 2^32 threads a launch
+  if ((a->M + 15) / 16 * std::max<int64_t>(plan.slices, (a->N + 63) / 64) > (1 << 23))   // 2^32 threads a launch
     return fail(LB_UNSUPPORTED, "%s: more than 2^23 tiles of outputs", what);
   return LB_OK;
 }
@@ -81,6 +90,7 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
   p.rank = (int)a->rank;
   p.count = (int)a->count;
   p.slices = plan.slices;
+  p.groups = plan.groups;
   p.span = plan.span;
   p.wide = a->N % 8 == 0 && aligned(a->y, 16) && aligned(a->out, 16) && (a->M == 1 || (a->ldy % 8 == 0 && a->ldo % 8 == 0));
   p.shares = plan.shares;
@@ -89,7 +99,6 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
   typedef std::integral_constant<int, 1> One;
   typedef std::integral_constant<int, 2> Two;
   typedef std::integral_constant<int, 4> Four;
-  typedef std::integral_constant<int, 8> Eight;
   if (plan.fused) {
     const dim3 grid((unsigned)(plan.tiles * ((a->N + plan.span - 1) / plan.span)), (unsigned)plan.shares + 1);
     auto go = [&](auto rt) { hipLaunchKernelGGL((adapters_rows_kernel<T, decltype(rt)::value>), grid, dim3(64 * kRowsWaves), 0, s, p); };
@@ -97,20 +106,29 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
     return;
   }
   const int64_t wide = plan.span * (4 / plan.stack), rows = 16 * plan.stack;   // of a workgroup of adapters_up_kernel
-  const dim3 down((unsigned)(plan.tiles * plan.slices), (unsigned)plan.shares);
+  const dim3 down((unsigned)(plan.tiles * plan.slices * plan.groups), (unsigned)plan.shares);
   const dim3 up((unsigned)((a->M + rows - 1) / rows * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up + 1);
-  const dim3 tile((unsigned)((a->M + 63) / 64 * ((a->N + plan.span - 1) / plan.span)));
-  auto go = [&](auto rt, auto mt) {
-    constexpr int RT = decltype(rt)::value, MT = decltype(mt)::value;
-    hipLaunchKernelGGL((adapters_down_kernel<T, RT, MT>), down, dim3(512), 0, s, p);
-    if (MT > 1 && p.wide) hipLaunchKernelGGL((adapters_tile_kernel<T, (RT + 1) / 2>), tile, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((adapters_up_kernel<T, (RT + 1) / 2>), up, dim3(256), 0, s, p);
+  const dim3 tile((unsigned)((a->M + 63) / 64 * ((a->N + plan.wide_span - 1) / plan.wide_span)));
+  auto first = [&](auto rt) {
+    constexpr int RT = decltype(rt)::value;
+    if constexpr (RT <= 2)
+      if (plan.rows == 1) {
+        hipLaunchKernelGGL((adapters_down_kernel<T, RT, 1>), down, dim3(512), 0, s, p);
+        return;
+      }
+    hipLaunchKernelGGL((adapters_down_kernel<T, RT, 4>), down, dim3(512), 0, s, p);
   };
-  const bool one = plan.rows == 1;
-  if (a->rank <= 16) one ? go(One{}, One{}) : go(One{}, Four{});
-  else if (a->rank <= 32) one ? go(Two{}, One{}) : go(Two{}, Four{});
-  else if (a->rank <= 64) one ? go(Four{}, One{}) : go(Four{}, Four{});
-  else one ? go(Eight{}, One{}) : go(Eight{}, Two{});
+  plan.ranks == 1 ? first(One{}) : plan.ranks == 2 ? first(Two{}) : first(Four{});
+  auto second = [&](auto rc) {
+    constexpr int RC = decltype(rc)::value;
+    if (plan.tile && p.wide) {
+      p.span = plan.wide_span;
+      hipLaunchKernelGGL((adapters_tile_kernel<T, RC>), tile, dim3(256), 0, s, p);
+    } else {
+      hipLaunchKernelGGL((adapters_up_kernel<T, RC>), up, dim3(256), 0, s, p);
+    }
+  };
+  a->rank <= 32 ? second(One{}) : a->rank <= 64 ? second(Two{}) : second(Four{});
 }
 
 }  // namespace

@@ -21,7 +21,7 @@ struct AdaptersParams {
   float *z;                 // [slices][M][rank]
   long long ldx, ldy, ldo;
   int M, N, K, rank, count;
-  int slices;               // parts of K, added by adapters_up_kernel
+  int slices, groups;       // parts of K, added in the second launch; groups of ranks
   int shares, shares_up;    // workgroups that share a tile's adapters, in each launch
   int span, stack;          // adapters_up_kernel: outputs of a wave, tiles of a workgroup (adapters_rows_kernel: outputs of one)
   int wide;                 // rows of y and out are whole 16-byte pieces
@@ -47,7 +47,7 @@ __device__ __forceinline__ void each_adapter(int id, int share, int shares, F &&
   }
 }
 
-// z of 16 MT rows over one slice of K: waves take every eighth 64 of it and meet in LDS.
+// z of 16 MT rows and 16 RT ranks over one slice of K: waves take every eighth 64 of it and meet in LDS.
 template <class T, int RT, int MT>
 __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
   __shared__ f4 met[W][TILES][64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slice = blockIdx.x % p.slices, first = blockIdx.x / p.slices * (16 * MT);
+  const int slice = blockIdx.x % p.slices, rest = blockIdx.x / p.slices, rank0 = rest % p.groups * (16 * RT), first = rest / p.groups * (16 * MT);
   const int id = adapter_of(p, first, lane, 16 * MT);
   const int all = (p.K + 63) / 64, size = (all + p.slices - 1) / p.slices, from = slice * size, to = min(all, from + size);
   each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
-      for (int r = 0; r < RT; ++r) dr[r][b] = down + (size_t)min(16 * r + 8 * b + row, p.rank - 1) * p.K + at;
+      for (int r = 0; r < RT; ++r) dr[r][b] = down + (size_t)min(rank0 + 16 * r + 8 * b + row, p.rank - 1) * p.K + at;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         live[t][b] = mine >> (16 * t + 8 * b + row) & 1;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
       f4 sum = met[0][i][lane];
 #pragma unroll
       for (int w = 1; w < W; ++w) sum += met[w][i][lane];
-      const int rank = i / MT * 16 + 4 * g, row = i % MT * 16 + j;
+      const int rank = rank0 + i / MT * 16 + 4 * g, row = i % MT * 16 + j;
       if (rank < p.rank && (mine >> row & 1))
         *reinterpret_cast<f4 *>(p.z + ((size_t)slice * p.M + first + row) * p.rank + rank) = sum;
     }
