@@ -176,6 +176,7 @@ def test_struct_sizes():
     assert serve._ROTARY.size + r == ctypes.sizeof(serve.RotaryArgs)
     head = serve._PAGED_HEAD.size + serve._PAGED_CACHE.size
     assert head + serve._APPEND.size + r == ctypes.sizeof(serve.PagedAppendArgs)
+    assert serve._ADAPTERS.size == ctypes.sizeof(serve.AdaptersArgs)
     assert head + serve._ATTENTION.size + r + serve._ATTENTION_TAIL.size == ctypes.sizeof(serve.PagedAttentionArgs)
     for fn, a in (('lb_rotary', rotary()), ('lb_paged_append', append()), ('lb_paged_attention', attention()), ('lb_adapters', adapters())):
         a.struct_size -= 1

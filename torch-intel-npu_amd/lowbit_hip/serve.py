@@ -497,7 +497,27 @@ class Adapters:
         self.down, self.up, self.scales = down, up, scales
         self.count, self.rank, self.N, self.K = count, rank, up.shape[1], k
         self.dtype, self.device = down.dtype, down.device
-        self._needs = {}
+        self._bound()
+
+    def _bound(self):
+        """What calls are given of them, and the workspaces that calls need by their rows."""
+        at = self.down.data_ptr(), self.up.data_ptr(), 0 if self.scales is None else self.scales.data_ptr()
+        self.__dict__.update(_at=at, _needs={})
+
+    def __setattr__(self, name, value):
+        """The factors are fixed: their addresses are in what calls are given."""
+        if '_at' in self.__dict__:
+            raise AttributeError(f'{name}: the factors of Adapters are fixed (their contents are not); make others of other tensors')
+        super().__setattr__(name, value)
+
+    def __getstate__(self):
+        """Copies and pickles have factors of their own."""
+        return {name: value for name, value in self.__dict__.items() if name not in ('_at', '_needs')}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.__dict__['device'] = self.down.device
+        self._bound()
 
     @classmethod
     def stack(cls, factors, *, scales=None, dtype=torch.float16, device='cuda'):
@@ -521,6 +541,9 @@ class Adapters:
         return cls(downs, ups, scales=scales)
 
 
+_ADAPTERS = struct.Struct('=IIqqqqqQQQQQqQqQqQQ')    # size, type, M, N, K, rank, count; down, up, scales, index; x, ldx, y, ldy, out, ldo; workspace, bytes
+
+
 def _adapters_args(y, x, adapters, index, out, keep, copy):
     """The argument struct without its workspace, and the bytes that it needs of one."""
     if not isinstance(adapters, Adapters):
@@ -529,21 +552,28 @@ def _adapters_args(y, x, adapters, index, out, keep, copy):
     if not isinstance(x, torch.Tensor) or x.dtype != dtype or x.ndim != 2 or x.shape[1] != K or x.shape[0] < 1:
         raise ValueError(f'x must be {dtype} [M, {K}]')
     M = x.shape[0]
-    for t, name in ((y, 'y'), (out, 'out')):
-        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (M, N) or (N > 1 and t.stride(1) != 1):
-            raise ValueError(f'{name} must be {dtype} [{M}, {N}] with contiguous rows')
-    for t, name in ((x, 'x'), (y, 'y'), (out, 'out')):
+    places = []
+    for t, name in ((y, 'y'),) if out is y else ((y, 'y'), (out, 'out')):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != (M, N):
+            raise ValueError(f'{name} must be {dtype} [{M}, {N}]')
         if t.device != device:
             raise ValueError(f'{name} must be on {device} with the adapters (found {t.device})')
+        ld, step = t.stride()
+        if step != 1 and N > 1:
+            raise ValueError(f'the rows of {name} must be contiguous')
+        places += (t.data_ptr(), ld)
+    if x.device != device:
+        raise ValueError(f'x must be on {device} with the adapters (found {x.device})')
     at = _counts(index, 'index', (M,), device)
-    if x.stride(1) != 1 or x.data_ptr() % 16 or (M > 1 and x.stride(0) % 8):
+    ldx, step = x.stride()
+    if step != 1 or x.data_ptr() % 16 or (M > 1 and ldx % 8):
         if not copy:
             raise ValueError('the rows of x must be 16-byte pieces')
         x = _aligned(x)
         keep.append(x)
-    a = AdaptersArgs(ctypes.sizeof(AdaptersArgs), TYPES[dtype], M, N, K, adapters.rank, adapters.count, adapters.down.data_ptr(),
-                     adapters.up.data_ptr(), None if adapters.scales is None else adapters.scales.data_ptr(), at, x.data_ptr(),
-                     x.stride(0), y.data_ptr(), y.stride(0), out.data_ptr(), out.stride(0), None, 0)
+        ldx = x.stride(0)
+    a = AdaptersArgs.from_buffer_copy(_ADAPTERS.pack(_ADAPTERS.size, TYPES[dtype], M, N, K, adapters.rank, adapters.count, *adapters._at, at,
+                                                     x.data_ptr(), ldx, *places[:2], *places[-2:], 0, 0))
     need = adapters._needs.get(M)
     if need is None:
         need = _needed(library().lb_adapters_workspace_bytes, 'lb_adapters_workspace_bytes', a)
