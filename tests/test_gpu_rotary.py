@@ -134,6 +134,22 @@ def test_back_is_the_gradient(device):
     assert torch.equal(on.T, off)
 
 
+@pytest.mark.parametrize('out', ['apart', 'in place'])
+def test_many_rows(device, out):
+    """Rows of more bytes than the caches keep have the values of the same rows in smaller calls."""
+    announce('rotary many rows', out)
+    x = make(device, 'fp16', 2, 2300, 64, 128, 10)
+    before = x.clone()
+    rotary = lb.Rotary(lb.rotary_frequencies(128, device=device))
+    got = lb.rotary(x, torch.tensor([5, 70000], device=device), rotary, out=x if out == 'in place' else None)
+    for b, first in enumerate((5, 70000)):
+        for at in (0, 1000, 2000):
+            part = before[b:b + 1, at:at + 1000]
+            assert torch.equal(got[b:b + 1, at:at + 1000], lb.rotary(part, torch.tensor([first + at], device=device), rotary))
+    if out == 'apart':
+        assert torch.equal(x, before)
+
+
 def test_capture_and_streams(device):
     """A captured call reads its positions at each replay; calls on other streams give the same."""
     announce('rotary capture')

@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> 
   const int half = p.turn.frequencies ? p.turn.dims / 2 : 0;
   const int lane = tid / (kChunk * CH), piece = tid % (kChunk * CH), mine = base + piece / CH;   // this thread's piece of a head, its slot
   auto value = [&](int h) {
-    return h < head1 && mine >= from && mine < to ? *reinterpret_cast<const x8 *>(p.v.at(b, mine - first, h) + 8 * (piece % CH)) : x8{};
+    return h < head1 && mine >= from && mine < to ? read_once<x8>(p.v.at(b, mine - first, h) + 8 * (piece % CH)) : x8{};
   };
   x8 next = value(head0 + lane);
 #pragma unroll 1
@@ -134,7 +134,7 @@ struct PagedAttendParams {
   Turn turn;
   uint32_t *tickets;        // kPagedParts zero words
   float *partial;           // [places][16][D] sums, then [places][16][2] references and totals
-  int rounds;               // of 256 workgroups, besides those of sequences and heads: what the grid has
+  int rounds;               // of workgroups that fit on the chip, besides those of sequences and heads: what the grid has
   int batch, group, tiles;  // group: query heads of a KV head; tiles of up to 16 of them
   float scale;              // score scale * log2(e)
 };
@@ -143,7 +143,7 @@ constexpr int kUnit = 2 * kChunk;     // slots of a wave's step
 // Parts that the whole work is split into at the most, besides those that sequences and heads are by themselves, and places
 // for the sums of parts.
 constexpr int kPagedParts = 1024, kPagedPlaces = 2 * kPagedParts + 2;
-constexpr int kPagedLeast = 16;       // units of a part at the least: two a wave
+constexpr int kPagedWhole = 16 * kUnit;   // slots of a sequence up to which it is never split
 constexpr float kPagedLowest = -3.402823466e38f;
 // Probabilities are taken relative to a reference 2^kPagedLift below a row's running maximum when it was set, and it is
 // set anew where a score exceeds it by kPagedLift + kPagedSlack (units of log2): fp16 then has the probabilities in
@@ -194,13 +194,17 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   uint32_t all = lane < p.batch ? units_of(at0) : 0;
   for (int i = lane + 64; i < p.batch; i += 64) all += units_of(p.position[i]);
   all = lanes_sum(all);
-  // Units of a part at the most.  A CU holds one workgroup, and takes `kStart` units' time to start it; the memory takes 1.4 times
-  // a CU's time for a 256th of the work.  So rounds of 256 workgroups, as few as cost the least (half a part of a sequence
-  // and head lies idle in the mean), and parts no smaller than they must be to fit in them.  (Parts are never more than
-  // sequences times heads and 256 rounds: each sequence has less than one part over what its share of the work is.)
-  uint32_t most = kPagedLeast;
+  // Units of a part at the most.  As many workgroups of W waves as fit on the chip are a round, which takes `kStart` units' time
+  // to start; the memory takes 1.4 times a CU's time for its share of the work.  So as few rounds as cost the least (half a part
+  // of a sequence and head lies idle in the mean), and parts no smaller than they must be to fit in them.  (Parts are never
+  // more than sequences times heads and the rounds': each sequence has less than one part over what its share of the work is.)
+  // Short sequences are not split, for joining parts takes 4 us (one of 500 slots, 3 heads of 64: 6.6 us whole, 8.0 split; of 1200
+  // 9.6 and 8.1; two of 803, one head of 128: 11.7 and 9.3).  Where they are, parts may be small: 8 units, one for each wave.
+  constexpr int kRound = 256 * 8 / W;
+  constexpr uint32_t kWhole = (D == 64 ? 2 : 1) * kPagedWhole / kUnit, kLeast = 8;
+  uint32_t most = kWhole;
   if (p.batch > 64) {
-    most = max((uint32_t)(((uint64_t)all * heads + 256 * p.rounds - 1) / (256 * p.rounds)), most);
+    most = max((uint32_t)(((uint64_t)all * heads + kRound * p.rounds - 1) / (kRound * p.rounds)), most);
   } else {
     const uint32_t n = lane < p.batch ? units_of(at0) : 0;
     if (__any(n > most)) {
@@ -210,19 +214,19 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
       float least = INFINITY, size = 0.0f;
       uint32_t room = 0;
       for (int k = 1; k <= p.rounds; ++k) {
-        const float m = fminf(longest, work * __builtin_amdgcn_rcpf(fmaxf(256.0f * k - 0.5f * pairs, 1.0f)));
-        const float cost = fmaxf(work * (1.4f / 256), k * (fmaxf(m, (float)kPagedLeast) + kStart));
-        if (256 * k >= pairs && cost < 0.95f * least) {
+        const float m = fminf(longest, work * __builtin_amdgcn_rcpf(fmaxf((float)kRound * k - 0.5f * pairs, 1.0f)));
+        const float cost = fmaxf(work * (1.4f / 256), k * (8 / W) * (fmaxf(m, (float)kLeast) + kStart));
+        if (kRound * k >= pairs && cost < 0.95f * least) {
           least = cost;
           size = m;
-          room = 256 * k;
+          room = kRound * k;
         }
       }
       if (room == 0) {                    // more sequences and heads than that
         room = ~0u;
-        size = work / (256.0f * p.rounds);
+        size = work / (float)(kRound * p.rounds);
       }
-      most = max((uint32_t)size + 1, most);
+      most = max((uint32_t)size + 1, kLeast);
       for (int i = 0; i < 4 && lanes_sum((n + most - 1) / most) * heads > room; ++i) most += most / 8 + 1;
     }
   }
@@ -294,13 +298,13 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
 #pragma unroll
     for (int t = 0; t < C; ++t)
 #pragma unroll
-      for (int u = 0; u < U; ++u) kn[t][u] = *reinterpret_cast<const u4 *>(kc[t] + kd + (u & 1) * 4 * D + u / 2 * 64);
+      for (int u = 0; u < U; ++u) kn[t][u] = read_once<u4>(kc[t] + kd + (u & 1) * 4 * D + u / 2 * 64);
   };
   auto fetch_values = [&]() {
 #pragma unroll
     for (int t = 0; t < C; ++t)
 #pragma unroll
-      for (int d = 0; d < DT / 2; ++d) vn[t][d] = *reinterpret_cast<const u4 *>(vc[t] + vd + d * 32 * kChunk);
+      for (int d = 0; d < DT / 2; ++d) vn[t][d] = read_once<u4>(vc[t] + vd + d * 32 * kChunk);
   };
   if (unit < (int)to) {
     find(unit, 0);

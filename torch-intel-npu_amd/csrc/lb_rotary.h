@@ -18,8 +18,8 @@ struct RotaryParams {
 };
 
 // A thread holds V pairs of a row, their sines and cosines, and goes through every `lanes`-th head of the row's queries
-// and keys: the sines are computed once for those heads.  Memory bounds it.
-template <class T, int V>
+// and keys: the sines are computed once for those heads.  Memory bounds it.  ONCE: the rows are more than the caches hold.
+template <class T, int V, bool ONCE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams<T> p) {
   typedef T Piece __attribute__((ext_vector_type(V)));
   const int turned = p.turn.dims / (2 * V), pieces = turned + p.copies;
@@ -48,8 +48,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams<T> p) {
     const int side = h >= p.heads[0], hs = side ? h - p.heads[0] : h;
     const T *in = (side ? p.x[1] : p.x[0]).at(b, i, hs) + first;
     T *out = (side ? p.out[1] : p.out[0]).at(b, i, hs) + first;
-    Piece lo = *reinterpret_cast<const Piece *>(in), hi = {};
-    if (both) hi = *reinterpret_cast<const Piece *>(in + step);
+    Piece lo = ONCE ? read_once<Piece>(in) : *reinterpret_cast<const Piece *>(in), hi = {};
+    if (both) hi = ONCE ? read_once<Piece>(in + step) : *reinterpret_cast<const Piece *>(in + step);
     if (turns) {
       if (!p.turn.neighbours || V == 1) {
 #pragma unroll

@@ -20,6 +20,10 @@ template <> struct Of16<bf16> {
   static __device__ __forceinline__ f4 mma(x8 a, x8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 
+// A load of what nobody reads again soon: it leaves the caches to others.
+template <class V>
+__device__ __forceinline__ V read_once(const void *p) { return __builtin_nontemporal_load(static_cast<const V *>(p)); }
+
 // Rows of contiguous values, strides in elements.
 template <class T>
 struct Rows {

@@ -11,7 +11,6 @@ using namespace lb::abi;
 
 namespace {
 
-constexpr int kWaves = 8;   // of a workgroup of paged_attend_kernel
 static_assert(kPagedParts * 4 <= LB_ZEROED_WORKSPACE_BYTES, "tickets are the workspace's zeroed bytes");
 
 template <class T>
@@ -62,7 +61,7 @@ void with_kind(const lb_paged_cache &c, F &&f) {
 }
 
 struct AttendPlan {
-  int tiles, rounds;
+  int tiles, waves, rounds;
   int64_t grid;
   size_t bytes;
 };
@@ -71,12 +70,16 @@ AttendPlan attend_plan(const lb_paged_attention_args *a) {
   AttendPlan plan{};
   const lb_paged_cache &c = a->cache;
   plan.tiles = (int)((a->heads / c.kv_heads + 15) / 16);
-  const int64_t heads = c.kv_heads * plan.tiles, pairs = heads * a->batch, units = (a->table.longest * c.page + kUnit - 1) / kUnit;
-  // A workgroup per sequence and head, and where sequences can be long enough the rounds of 256 that they can be split into: few
-  // sequences are split evenly in one, more of them need more to end together.
-  const bool split = units > kPagedLeast;
-  plan.rounds = pairs <= 128 ? 1 : kPagedParts / 256;
-  plan.grid = pairs + (split ? 256 * plan.rounds : 0);
+  const int64_t heads = c.kv_heads * plan.tiles, pairs = heads * a->batch;
+  // Eight waves a workgroup; where heads of 128, whose registers leave room for one on a CU, are more than CUs, two of four
+  // (54 sequences of up to 22 slots, 8 heads: 11.3 -> 7.9 us; 40 of up to 2001 39.6 -> 38.0; 33 of up to 8192 98.5 -> 98.7.
+  // 128 of up to 800, 3 heads of 64: 13.8 with eight, 15.3 with four).
+  plan.waves = c.head_dim == 128 && pairs > 256 ? 4 : 8;
+  // A workgroup per sequence and head, and where sequences can be long enough the rounds of 256 or 512 that they can be split into:
+  // few sequences are split evenly in one, more of them need more to end together.
+  const bool split = a->table.longest * c.page > kPagedWhole;
+  plan.rounds = pairs <= 128 ? 1 : kPagedParts / (256 * 8 / plan.waves);
+  plan.grid = pairs + (split ? plan.rounds * (256 * 8 / plan.waves) : 0);
   plan.grid = (plan.grid + heads - 1) / heads * heads;   // whole tickets
   plan.bytes = split ? LB_ZEROED_WORKSPACE_BYTES + (size_t)kPagedPlaces * 16 * (c.head_dim + 2) * sizeof(float) : 0;
   return plan;
@@ -190,9 +193,16 @@ lb_status lb_paged_attention(const lb_paged_attention_args *a, void *stream) {
     p.group = (int)(a->heads / c.kv_heads);
     p.tiles = plan.tiles;
     p.scale = a->scale * 1.44269504088896340736f;
-    const dim3 grid((unsigned)plan.grid), block(64 * kWaves);
-    if (p.turn.frequencies) hipLaunchKernelGGL((paged_attend_kernel<T, dim(), kWaves, true>), grid, block, 0, static_cast<hipStream_t>(stream), p);
-    else hipLaunchKernelGGL((paged_attend_kernel<T, dim(), kWaves, false>), grid, block, 0, static_cast<hipStream_t>(stream), p);
+    auto go = [&](auto waves) {
+      constexpr int W = decltype(waves)::value;
+      const dim3 grid((unsigned)plan.grid), block(64 * W);
+      if (p.turn.frequencies) hipLaunchKernelGGL((paged_attend_kernel<T, dim(), W, true>), grid, block, 0, static_cast<hipStream_t>(stream), p);
+      else hipLaunchKernelGGL((paged_attend_kernel<T, dim(), W, false>), grid, block, 0, static_cast<hipStream_t>(stream), p);
+    };
+    if constexpr (dim() == 128) {
+      if (plan.waves == 4) return go(std::integral_constant<int, 4>{});
+    }
+    go(std::integral_constant<int, 8>{});
   });
   return launch_status(what);
 }
