@@ -47,7 +47,8 @@ __device__ __forceinline__ void each_adapter(int id, int share, int shares, F &&
   }
 }
 
-// z of 16 MT rows and 16 RT ranks over one slice of K: waves take every eighth 64 of it and meet in LDS.
+// z of 16 MT rows and 16 RT ranks over one slice of K: waves take every eighth 64 of it and meet in LDS.  The rows' memory bounds it
+// (4001 rows of 4096, rank 32: 15 us), or with few rows the chain of index, factors and sums (4.8 us for 64 rows of 64 adapters).
 template <class T, int RT, int MT>
 __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -281,7 +282,8 @@ __device__ __forceinline__ void gather(const AdaptersParams<T> &p, int first, bo
 }
 
 // out = y + s z B^T.  A wave takes 16 rows and `span` outputs; the waves of a workgroup have `stack` tiles of rows and 4 / stack
-// spans.
+// spans.  (64 rows of 64 adapters, 4096 outputs, rank 16: 6.5 us, of which the launch and the loads of index, z and factors one after
+// the other are most.)
 template <class T, int RC>
 __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
@@ -313,7 +315,8 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
 // out = y + s z B^T of 64 rows and `span` outputs, 128 at a time, for many rows (p.wide).  y is read and out written in rows of
 // 256 bytes, 1 KB a wave at once, since a transfer whose lanes have 16 rows costs the address unit twice that of whole lines;
 // the products come to the lanes of those rows through LDS.  z is added up and split once a workgroup, and kept in LDS; the
-// factors of 32 outputs, which a wave holds, serve all rows of the tile.
+// factors of 32 outputs, which a wave holds, serve all rows of the tile.  Memory bounds it: 4001 rows of 14336 outputs, rank 32, 229 MB
+// of y and out, take 53 us (4.3 TB/s).  (out is stored past the caches: 5360 rows of 4096, both launches, 44.3 -> 41.0 us.)
 template <class T, int RC>
 __global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p)
         const float sum = (float)y[i][e] + (e < 4 ? lo[e] : hi[e - 4]);
         v[e] = whose >= 0 ? (T)sum : whose == -1 ? y[i][e] : (T)__builtin_nanf("");
       }
-      *reinterpret_cast<x8 *>(p.out + (size_t)(first + row) * p.ldo + n) = v;
+      __builtin_nontemporal_store(v, reinterpret_cast<x8 *>(p.out + (size_t)(first + row) * p.ldo + n));
     }
     __syncthreads();                      // (mem is read)
   }
@@ -428,7 +431,8 @@ __global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p)
 
 // Both products of 16 rows in one launch, for few rows: a workgroup of W waves computes z of an adapter of the tile itself (its
 // waves take every W-th 64 of K and meet in LDS) and `span` outputs, 64 a wave at a time, whose factors and y are requested
-// before z is there.  Every span's workgroup reads the whole of A again, from the caches.
+// before z is there.  Every span's workgroup reads the whole of A again, from the caches.  5 rows of 576 by 576, rank 8: 4.3 us, hardly
+// more than an empty launch takes.
 template <class T, int RT>
 __global__ __launch_bounds__(64 * kRowsWaves) void adapters_rows_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;

@@ -38,7 +38,9 @@ struct PagedAppendParams {
 // A workgroup takes one chunk of 16 slots that new rows fall into, for `heads` KV heads of a sequence.  Values are read in rows and
 // turned in LDS into the 16 bytes that 8 slots of a dim are, so that both sides move whole lines; the chunk's sines and cosines are
 // computed behind their loads, once for all heads, into LDS; then keys, 8 dims of a row a thread.  (One loop body for every
-// key: straight-line code of four rows took a short call as long to fetch as to run.)
+// key: straight-line code of four rows took a short call as long to fetch as to run.)  Memory bounds it where rows are many: prompts
+// of 4100, 3476, 2526 and 951 rows of 8 heads of 128, bf16, 90 MB in and out, take 23.7 us (3.8 TB/s).  500 rows of 3 heads
+// of 64 take 5.5: the launch, and the positions, the table and the rows one after the other.
 template <class T, int D>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -167,6 +169,11 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
 // One new token a sequence.  A workgroup takes a part of a sequence's slots for a KV head (and up to 16 of its query heads),
 // its W waves every W-th unit of slots each with a reference and total of their own, joined in LDS; parts are joined by
 // the workgroup that counts last.  Which part it takes is found from the positions, on the device.
+//
+// Memory bounds it where the slots are many, 16-bit keys and values read once: one sequence of 130999 slots, 8 heads of 128, takes
+// 86.3 us (6.2 TB/s), 64 of up to 8193 178 us (6.1).  The products take K (as rows of 16 slots) and V (as rows of 16 dims) straight from
+// their pages, and P comes out of one as the operand of the other, so LDS holds only what waves exchange.  Few slots cost the
+// chain of loads (positions, table, keys and values: 5.7 us for 150), and parts another 4 us (sums out, count, sums in).
 //
 // TURNED: queries are turned by their position (and the new key).  A turned query enters the product as the sum of two numbers of
 // the type, so that its rounding (2^-9 of bf16, which large scores would pass on whole) is not added to the held keys'.
