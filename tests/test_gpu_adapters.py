@@ -6,6 +6,9 @@ numbers are exact, each addition rounds; additions of parts and of slices among 
 2^-17 of the row's largest |z| bounds both.  The second sum has 2 rank products, off by 2 rank 2^-24 of their magnitudes, and the
 scale's product and the sum with y are rounded to 32 bits.  Then the output's own half step.
 """
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -174,3 +177,20 @@ def test_capture_and_streams(device):
         other = lb.adapters_add(y, x, adapters, index, out=torch.zeros_like(y))
     side.synchronize()
     assert torch.equal(other, want)
+
+
+def test_copies_and_pickles(device):
+    """They have factors of their own, and calls over them read those."""
+    announce('adapters copies')
+    x, y, adapters = make(device, 'fp16', 3, 64, 64, 8, 2, seed=8)
+    index = torch.tensor([1, -1, 0], device=device)
+    want = lb.adapters_add(y, x, adapters, index, out=torch.zeros_like(y))
+    for again in (copy.deepcopy, lambda a: pickle.loads(pickle.dumps(a))):
+        twin = again(adapters)
+        assert twin.down.data_ptr() != adapters.down.data_ptr()
+        assert torch.equal(lb.adapters_add(y, x, twin, index, out=torch.zeros_like(y)), want)
+        twin.up.zero_()
+        assert torch.equal(lb.adapters_add(y, x, twin, index, out=torch.zeros_like(y)), y)
+    assert torch.equal(lb.adapters_add(y, x, adapters, index, out=torch.zeros_like(y)), want)
+    with pytest.raises(AttributeError):
+        adapters.up = adapters.up.clone()

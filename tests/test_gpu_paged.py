@@ -13,6 +13,9 @@ Attention: with p the probabilities, A = sum p |v|, R the largest sum |q k| scal
   - the output's own half step.
 All are counted at their worst and added.
 """
+import copy
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -375,6 +378,40 @@ def test_streams(device):
                 outs.append(lb.paged_attention(q, cache, table, position))
     torch.cuda.synchronize()
     assert all(torch.equal(out, want) for out in outs)
+
+
+def test_copies_and_pickles(device):
+    """They have buffers of their own, and calls over them read those."""
+    announce('paged copies')
+    cache, table = filled(device, 'bf16', 5, 2, 32, 64), ints([[4, 1, 3]], device).int()
+    rotary = lb.Rotary(lb.rotary_frequencies(64, device=device), pairs='neighbours', scale=1.5)
+    q, position = rand(device, 'bf16', 1, 6, 64), ints([80], device)
+    want = lb.paged_attention(q, cache, table, position, rotary=rotary)
+    for again in (copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))):
+        twin, turns = again(cache), again(rotary)
+        assert twin.keys.data_ptr() != cache.keys.data_ptr() and torch.equal(twin.keys, cache.keys) and torch.equal(twin.values, cache.values)
+        assert torch.equal(lb.paged_attention(q, twin, table, position, rotary=turns), want)
+        twin.keys.zero_()
+        assert not torch.equal(lb.paged_attention(q, twin, table, position, rotary=turns), want)
+    assert torch.equal(lb.paged_attention(q, cache, table, position, rotary=rotary), want)
+    with pytest.raises(AttributeError):
+        cache.keys = cache.keys.clone()
+    with pytest.raises(AttributeError):
+        rotary.scale = 2.0
+
+
+def test_read(device):
+    announce('paged read')
+    cache = filled(device, 'fp16', 3, 2, 16, 64)
+    keys, values = cache.read([2, 0], 20)
+    assert torch.equal(keys[:, :16], cache.keys[2]) and torch.equal(keys[:, 16:], cache.keys[0][:, :4])
+    assert torch.equal(values[:, 16:], cache.values[0, :, 0].transpose(1, 2)[:, :4])
+    again = cache.read(ints([2, 0, -1], device).int(), 20)       # (a row of a table, with what stands behind the sequence's pages)
+    assert torch.equal(again[0], keys) and torch.equal(again[1], values)
+    assert cache.read([], 0)[0].shape == (2, 0, 64)
+    for pages, length in (([2, 3], 20), ([-1], 1), ([0], 17), ([0], -1)):
+        with pytest.raises(ValueError):
+            cache.read(pages, length)
 
 
 def test_far_pages(device):

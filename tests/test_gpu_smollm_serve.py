@@ -173,6 +173,20 @@ def test_refusals(device):
     assert sorted(decoder._free) == [0, 1, 2, 3]
 
 
+def test_prompts_that_are_none(device):
+    """Tokens outside the vocabulary, two rows and numbers that are not whole are refused before anything is enqueued."""
+    announce('smollm serve prompts')
+    stack, io, _, _ = make(device, 'w8a16', capacity=32)
+    decoder = SmolBatchDecoder(stack, io, batch=1, slots=32, page=16, graph=False)
+    for ids in ([-1], [io.vocab_size], [[1], [2]], [1.5], torch.tensor([1], dtype=torch.int32), torch.tensor([[[1]]])):
+        with pytest.raises(ValueError, match='tokens'):
+            decoder.admit(ids, steps=1)
+    assert sorted(decoder._free) == [0, 1]
+    place = decoder.admit(torch.tensor([[1, io.vocab_size - 1]], device=device), steps=1)
+    decoder.step()
+    decoder.release(place)
+
+
 def test_operators_together(device):
     """Rotary, append, attention and adapters in the order in which a layer uses them, against each other's definitions: a prompt
     appended, then tokens one at a time, equal a token's attention over all of its rows turned by lb_rotary."""

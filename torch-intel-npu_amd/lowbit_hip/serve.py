@@ -259,7 +259,8 @@ def rotary(q, position, rotary, *, k=None, out=None, out_k=None, back=False):
     their positions, and with k [batch, seq, k_heads, head_dim] its rows too, in one launch.  position: int64 [batch] (row i
     of sequence b lies at position[b] + i) or [batch, seq] (each row's own), on the device.  Into out and out_k, which may be
     q and k themselves (both or neither); new tensors where they are not given.  back: by the negative angle, still times the
-    scale, which is the transpose: of an output's gradient it makes the input's.  Returns out, or (out, out_k)."""
+    scale, which is the transpose: of an output's gradient it makes the input's (autograd does not record
+    the call).  Returns out, or (out, out_k)."""
     if out is None and isinstance(q, torch.Tensor):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out_k is None and isinstance(k, torch.Tensor):
@@ -338,10 +339,13 @@ class PagedKVCache:
     def read(self, pages, length):
         """Keys and values [kv_heads, length, head_dim] of a sequence with these pages (int64 or int32 numbers, as a list or a
         tensor), in the order of its slots."""
-        pages = torch.as_tensor(pages, device=self.device).reshape(-1).long()
+        pages = torch.as_tensor(pages).reshape(-1).long()
         length = _whole(length, 'length', 0, pages.numel() * self.page)
-        keys = self.keys[pages].transpose(0, 1).reshape(self.kv_heads, -1, self.head_dim)
-        values = self.values[pages].transpose(-1, -2).transpose(0, 1).reshape(self.kv_heads, -1, self.head_dim)
+        pages = pages[:-(-length // self.page)].to(self.device)     # (what stands behind them may be no page)
+        if length and not bool(((pages >= 0) & (pages < self.pages)).all()):
+            raise ValueError(f'pages must be 0 to {self.pages - 1}')
+        keys = self.keys[pages].transpose(0, 1).reshape(self.kv_heads, pages.numel() * self.page, self.head_dim)
+        values = self.values[pages].transpose(-1, -2).transpose(0, 1).reshape(self.kv_heads, pages.numel() * self.page, self.head_dim)
         return keys[:, :length].contiguous(), values[:, :length].contiguous()
 
     def nbytes(self):

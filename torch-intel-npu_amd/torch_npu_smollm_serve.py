@@ -152,7 +152,12 @@ class SmolBatchDecoder:
         """Prefills a request (ids: its prompt's int64 tokens, one row) that may take up to `steps` steps, with an adapter's number
         or -1, into a free place.  Its first token is then tokens[place].  Returns the place.  ValueError where no place
         is free or the pages left are too few (a request gets all of its pages here)."""
-        ids = torch.as_tensor(ids, dtype=torch.int64, device=self.device).reshape(1, -1)
+        ids = torch.as_tensor(ids)
+        if ids.numel() == 0 or ids.dtype != torch.int64 or ids.ndim > 2 or (ids.ndim == 2 and ids.shape[0] != 1):
+            raise ValueError('ids must be one row of int64 tokens')
+        if int(ids.min()) < 0 or int(ids.max()) >= self.io.vocab_size:
+            raise ValueError(f'tokens must be 0 to {self.io.vocab_size - 1}')
+        ids = ids.to(self.device).reshape(1, -1)
         s = ids.shape[1]
         if type(steps) is not int or steps < 0 or s < 1 or s + steps > self.slots or s > self.stack.layers[0].capacity:
             raise ValueError(f'a request takes 1 to {self.stack.layers[0].capacity} prompt tokens and {self.slots} slots in all')
