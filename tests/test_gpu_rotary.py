@@ -52,6 +52,12 @@ CASES = [
     ('fp16', 1, 2, 1, 1, 1024, 1024, 'half'),
     ('bf16', 1, 700, 15, 5, 64, 64, 'half'),
     ('fp16', 64, 1, 24, 1, 64, 64, 'half'),
+    ('fp16', 3, 4001, 1, 0, 64, 64, 'half'),
+    ('bf16', 3, 4001, 2, 1, 64, 24, 'neighbours'),
+    ('bf16', 1, 3, 70, 10, 128, 128, 'half'),
+    ('fp32', 2, 2, 3, 2, 1024, 1024, 'half'),
+    ('fp32', 1, 3, 2, 1, 1023, 1022, 'neighbours'),
+    ('fp16', 1, 2, 5, 2, 1020, 1016, 'half'),
 ]
 
 

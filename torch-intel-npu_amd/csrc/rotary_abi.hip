@@ -34,15 +34,16 @@ void launch(const lb_rotary_args *a, bool in_place, hipStream_t s) {
   p.back = a->back != 0;
   p.copies = in_place ? 0 : (int)((a->head_dim - p.turn.dims + 2 * V - 1) / (2 * V));
   const int64_t rows = a->batch * a->seq, pieces = p.turn.dims / (2 * V) + p.copies, all = a->heads + a->k_heads;
-  // Heads side by side until there are threads enough for the chip; past that a thread's sines serve several heads (8192 rows of
-  // 40 heads of 128, bf16: 2^17, 2^18, 2^19, 2^20, 2^22 threads at the most 41.6, 39.1, 36.1, 35.5, 41.6 us).
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(all, (1 << 20) / (rows * pieces))), turns = (all + most - 1) / most;
+  // A row's heads side by side in a wave, as many as it has lanes for, and where a lane would have more than two of them, more waves (8192
+  // rows of 40 heads of 128, bf16: 1, 2, 3, 5 waves a row 33.4, 31.7, 30.5, 36.4 us; 2048 rows 10.0, 9.5, 9.4, 10.0).
+  const int64_t lanes = std::min<int64_t>(all, std::max<int64_t>(1, 64 / pieces)), turns = (all + lanes - 1) / lanes;
   p.lanes = (int)((all + turns - 1) / turns);
-  // Rows of 64 MB and more are hardly in the caches, and read past them (8192 rows of 40 heads of 128, bf16, 84 MB: 35.0 -> 31.3 us;
-  // but 5 x 1111 of 16 of 64, fp32, 23 MB: 10.9 -> 13.5).
-  const bool once = rows * all * a->head_dim * (int64_t)sizeof(T) >= 64 << 20;
-  const int64_t threads = rows * pieces * p.lanes;
-  const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+  p.shares = (int)std::min<int64_t>((turns + 1) / 2, std::max<int64_t>(1, (1 << 20) / rows));
+  p.rows = (int)std::max<int64_t>(1, std::min<int64_t>(64 / (pieces * p.lanes), rows / 4096));
+  // Rows of 48 MB and more are hardly in the caches, and read past them (rows of 40 heads of 128, bf16, in turn over three inputs: 6000
+  // rows 27.2 -> 24.2 us, 4500 20.1 either way, 3000 12.2 -> 15.0).
+  const bool once = rows * all * a->head_dim * (int64_t)sizeof(T) >= 48 << 20;
+  const dim3 grid((unsigned)((rows + 4 * p.rows - 1) / (4 * p.rows) * p.shares)), block(256);
   if (once) hipLaunchKernelGGL((rotary_kernel<T, V, true>), grid, block, 0, s, p);
   else hipLaunchKernelGGL((rotary_kernel<T, V, false>), grid, block, 0, s, p);
 }
