@@ -2,7 +2,8 @@
 
 Tolerance: z = x A^T is a sum of K fp32 products, off by K 2^-24 of the sum of their magnitudes at the most (products of 16-bit
 numbers are exact, each addition rounds; additions of parts and of slices among them).  It enters the second product as two
-16-bit numbers: what is left of bf16 is 2^-18 of each z (2^-9 twice), of fp16 2^-22 and the subnormals' 2^-25 of the row's largest;
+16-bit numbers: what is left of bf16 is 2^-17 of each z (half a step, 2^-8 of it, and what lies
+below that has half a step of 2^-9 of it), of fp16 2^-22 and the subnormals' 2^-25 of the row's largest;
 2^-17 of the row's largest |z| bounds both.  The second sum has 2 rank products, off by 2 rank 2^-24 of their magnitudes, and the
 scale's product and the sum with y are rounded to 32 bits.  Then the output's own half step.
 """

@@ -3,12 +3,13 @@
 Append: values are copied; a turned key has the tolerance of the rotation (2^-20 of its pair's magnitudes, and its own half step).
 
 Attention: with p the probabilities, A = sum p |v|, R the largest sum |q k| scale of a score and n slots, the kernel differs by
-  - the rounding of each probability to the type, half a step of it, in the sum with V and in the total (twice A eps / 2), and of
-    fp16 ones below 2^-14, half of 2^-24 relative to a largest one of 2^10 or more (n 2^-35 max|v|, twice);
+  - the rounding of each probability to fp16, half a step of it, in the sum with V and in the total (twice A eps / 2), and of those
+    below 2^-14, half of 2^-24 relative to a largest one of 2^10 or more (n 2^-35 max|v|, twice); to two numbers of bf16, half a
+    step of the second, which is half a step of the first and less: 2^-17 A (in the sum alone);
   - the score in fp32: D exact products' sums and the scaling (factors of 1 +- (D + 4) 2^-24 R), the reference's subtraction (a score
     is at most R log2(e) in units of log2, its half step 2^-24 of that) and the exponential (2^-22): each on p, in the sum and total;
   - of a turned q (and k): the rotation's 2^-20 (as test_gpu_rotary derives; twice for |a| + |b| against a value of the pair, in
-    the sum over dims at most that), and what is left of q as two numbers of the type, 2^-18 (bf16): 2^-17 R in all;
+    the sum over dims at most that), and what is left of q as two numbers of the type, 2^-17 (bf16, as above): 2^-17 + 2^-19 R in all;
   - sums of n / 32 steps and of 256 parts in fp32, each a rounding of A: (n / 32 + 300) 2^-24 A, and the total's, twice;
   - the output's own half step.
 All are counted at their worst and added.
@@ -85,9 +86,9 @@ def check(out, q, cache, table, position, scale, type, turned=False):
         k, v = so.held(keys, values, table[b, :-(-n // cache.page)].tolist(), n)
         want, mean, size = so.attention(q[b] if turned else host(q[b]), k, v, scale)
         R = size[:, None]
-        score = ((dim + 8) * 2.0 ** -24 + (2.0 ** -17 if turned else 0)) * R + 2.0 ** -22
+        score = ((dim + 8) * 2.0 ** -24 + (2.0 ** -17 + 2.0 ** -19 if turned else 0)) * R + 2.0 ** -22
         tiny = 2 * n * 2.0 ** -35 * np.abs(v).max() if type == 'fp16' else 0.0
-        near = (eps + 2 * np.expm1(score) + 2 * (n / 32 + 300) * 2.0 ** -24) * mean + tiny
+        near = ((eps if type == 'fp16' else 2.0 ** -17) + 2 * np.expm1(score) + 2 * (n / 32 + 300) * 2.0 ** -24) * mean + tiny
         bound = near + eps / 2 * (np.abs(want) + near) + 2.0 ** -25 * (type == 'fp16')
         got = host(out[b]).astype(np.float64)
         worst = float(np.max(np.abs(got - want) / bound))
