@@ -476,7 +476,7 @@ typedef struct lb_rotation {
 typedef struct lb_rotary_args {
   uint32_t struct_size;      /* sizeof(lb_rotary_args) */
   uint32_t type;             /* lb_type */
-  int64_t batch, seq;        /* rows per sequence */
+  int64_t batch, seq;        /* rows per sequence; batch * seq up to 2^25 */
   int64_t head_dim;          /* 2 .. LB_ROTARY_MAX_DIMS */
   int64_t heads, k_heads;    /* k_heads 0: no keys */
   lb_rows q, out;            /* [batch, seq, heads]; out may be q itself (the same address and strides) */
@@ -526,7 +526,7 @@ typedef struct lb_paged_append_args {
   lb_paged_cache cache;
   lb_page_table table;
   int64_t batch;               /* 1 .. 65535 */
-  int64_t seq;                 /* rows of k and v per sequence */
+  int64_t seq;                 /* rows of k and v per sequence, 1 .. 2^25 */
   lb_rows k, v;                /* [batch, seq, kv_heads] rows of the cache's type, whole 16-byte pieces */
   const int64_t *position;     /* device [batch]: the slot of a sequence's first row */
   const int64_t *rows;         /* device [batch], 0..seq, or NULL: how many of its rows are appended (a padded batch) */
@@ -586,7 +586,7 @@ typedef struct lb_adapters_args {
   int64_t count;               /* adapters */
   const void *down;            /* A [count, rank, K], 16-byte aligned */
   const void *up;              /* B [count, N, rank], 16-byte aligned */
-  const float *scales;         /* [count], or NULL: 1 */
+  const float *scales;         /* [count], below 2^64 in size, or NULL: 1 */
   const int64_t *index;        /* device [M] */
   const void *x;               /* [M, ldx], 16-byte aligned, ldx a multiple of 8 */
   int64_t ldx;

@@ -237,6 +237,9 @@ APPENDS = [
     ('bf16', 5, 128, 128, 2, 40, [120, 16], [33, 40], 40, 'half'),
     ('fp16', 9, 64, 1024, 1, 90, [7], [90], 6, 'half'),
     ('fp16', 2, 128, 16, 2, 17, [14, 31], None, 100, 'neighbours'),
+    ('fp16', 3, 64, 16, 20, 400, [7 * b % 40 for b in range(20)], [400 - 19 * b for b in range(20)], 64, 'half'),
+    ('bf16', 11, 128, 32, 6, 600, [0, 5, 16, 31, 600, 2], [600, 599, 600, 1, 0, 593], 128, 'half'),
+    ('fp16', 8, 128, 64, 8, 600, [3 * b for b in range(8)], None, 64, 'neighbours'),
 ]
 
 

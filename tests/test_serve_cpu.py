@@ -75,7 +75,7 @@ BAD_ROTATION = [
     (dict(rotation__frequencies=0x900004), 'frequencies'),
 ]
 BAD_ROTARY = BAD_ROTATION + [
-    (dict(struct_size=8), 'struct_size'), (dict(type=3), 'type'), (dict(batch=0), 'rows'), (dict(seq=2 ** 28), 'rows'),
+    (dict(struct_size=8), 'struct_size'), (dict(type=3), 'type'), (dict(batch=0), 'rows'), (dict(seq=2 ** 28), 'rows'), (dict(batch=8, seq=2 ** 22 + 1), 'rows'),
     (dict(head_dim=1), 'head_dim'), (dict(head_dim=1025), 'head_dim'), (dict(heads=0), 'heads'), (dict(k_heads=-1), 'heads'),
     (dict(rotation__frequencies=0), 'frequencies'), (dict(position=0), 'position'), (dict(position=0x800004), 'position'),
     (dict(q__data=0), 'q must'), (dict(q__data=0x100001), 'q must'), (dict(k__data=0), 'k must'),

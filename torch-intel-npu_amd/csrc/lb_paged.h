@@ -39,12 +39,12 @@ struct PagedAppendParams {
 // turned in LDS into the 16 bytes that 8 slots of a dim are, so that both sides move whole lines; the chunk's sines and cosines are
 // computed behind their loads, once for all heads, into LDS; then keys, 8 dims of a row a thread.  (One loop body for every
 // key: straight-line code of four rows took a short call as long to fetch as to run.)  Memory bounds it where rows are many: prompts
-// of 4100, 3476, 2526 and 951 rows of 8 heads of 128, bf16, 90 MB in and out, take 23.7 us (3.8 TB/s).  500 rows of 3 heads
+// of 4100, 3476, 2526 and 951 rows of 8 heads of 128, bf16, 90 MB in and out, take 20.5 us (4.4 TB/s).  500 rows of 3 heads
 // of 64 take 5.5: the launch, and the positions, the table and the rows one after the other.
-template <class T, int D>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> p) {
+template <class T, int D, int NT>
+__global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams<T> p) {
   typedef typename Of16<T>::x8 x8;
-  constexpr int CH = D / 8, LANES = 256 / (kChunk * CH), PITCH = D + 8;   // pieces of a row; heads at once
+  constexpr int CH = D / 8, LANES = NT / (kChunk * CH), PITCH = D + 8;   // pieces of a row; heads at once
   __shared__ float2 turns[kChunk][D / 2];
   __shared__ __align__(16) T tile[LANES][kChunk][PITCH];
   const int tid = threadIdx.x, b = blockIdx.y, head0 = blockIdx.z * p.heads, head1 = min(head0 + p.heads, p.c.kv_heads);
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> 
   };
   x8 next = value(head0 + lane);
 #pragma unroll 1
-  for (int i = tid; i < kChunk * (D / 2); i += 256)
+  for (int i = tid; i < kChunk * (D / 2); i += NT)
     if (i % (D / 2) < half) turns[i / (D / 2)][i % (D / 2)] = turn_of(p.turn, i % (D / 2), (double)(base + i / (D / 2)));
   for (int h0 = head0; h0 < head1; h0 += LANES) {
     *reinterpret_cast<x8 *>(&tile[lane][piece / CH][8 * (piece % CH)]) = next;
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendParams<T> 
   // Keys.
   const bool pieces = p.turn.neighbours || half % 8 == 0;     // a pair's second dims are a piece too
   const int items = (head1 - head0) * (kChunk * CH);
-  for (int i = tid; i < items; i += 256) {
+  for (int i = tid; i < items; i += NT) {
     const int dim = 8 * (i % CH), slot = base + i / CH % kChunk, h = head0 + i / (CH * kChunk);
     if (slot < from || slot >= to) continue;
     const T *const row = p.k.at(b, slot - first, h);

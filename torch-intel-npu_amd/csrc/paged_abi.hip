@@ -109,7 +109,7 @@ lb_status lb_paged_append(const lb_paged_append_args *a, void *stream) {
   const lb_paged_cache &c = a->cache;
   Range cache[2], reads[6];
   if (const lb_status st = check_cache(what, c, a->table, a->batch, cache, reads[0]); st != LB_OK) return st;
-  if (a->seq < 1 || a->seq > kMaxSeq) return fail(LB_INVALID_ARGUMENT, "%s: seq 1 to 2^28 required", what);
+  if (a->seq < 1 || a->seq > kMaxSeq) return fail(LB_INVALID_ARGUMENT, "%s: seq 1 to 2^25 required", what);
   if (const lb_status st = check_strided(what, "k", a->k, a->batch, a->seq, c.kv_heads, c.head_dim, 2, true, false, reads[1]); st != LB_OK) return st;
   if (const lb_status st = check_strided(what, "v", a->v, a->batch, a->seq, c.kv_heads, c.head_dim, 2, true, false, reads[2]); st != LB_OK) return st;
   if (const lb_status st = check_array(what, "position", a->position, (size_t)a->batch * 8, 8, true, reads[3]); st != LB_OK) return st;
@@ -118,9 +118,16 @@ lb_status lb_paged_append(const lb_paged_append_args *a, void *stream) {
   if (const lb_status st = check_apart(what, cache, 2, reads, 6); st != LB_OK) return st;
   // Chunks that seq consecutive slots can fall into, wherever the first lies.
   const int64_t chunks = std::min((a->seq + 2 * kChunk - 2) / kChunk, a->table.longest * c.page / kChunk);
-  // Heads of a workgroup: they share its sines and cosines, but with more than four the loads of the first wait behind one another
-  // (four prompts of up to 4100 rows, 8 heads of 128: 1, 2, 4, 8 heads 27.0, 24.9, 25.9, 30.3 us).
-  const int64_t heads = std::max<int64_t>(1, std::min<int64_t>({c.kv_heads, 4, chunks * a->batch * c.kv_heads / 4096}));
+  // Heads of a workgroup: they share its sines and cosines, so as many as leave two workgroups a CU (8 heads of 128: prompts of 4100,
+  // 3476, 2526 and 951 rows, 2, 4, 8 heads 23.1, 22.3, 20.5 us; one of 4096 rows 10.2, 9.4, 10.0).  Threads: up to 1024, of which three
+  // of four have something to do (the first of these with 8 heads in 256, 512, 1024: 26.8, 24.3, 20.5; 4 x 8000 rows of 5 heads of 64
+  // in 256, 512: 17.9, 19.6; 8 x 2000 of 3: 9.3, 8.3).
+  const int64_t heads = std::max<int64_t>(1, std::min<int64_t>(c.kv_heads, chunks * a->batch * c.kv_heads / 512));
+  int threads = 1024;
+  for (; threads > 256; threads /= 2) {
+    const int64_t beside = threads / (kChunk * (int64_t)c.head_dim / 8);   // heads at once
+    if ((heads + beside - 1) / beside * beside * 3 <= heads * 4) break;
+  }
   with_kind(c, [&](auto type, auto dim) {
     typedef decltype(type) T;
     PagedAppendParams<T> p{};
@@ -132,7 +139,12 @@ lb_status lb_paged_append(const lb_paged_append_args *a, void *stream) {
     p.turn = turn_params(a->rotation);
     p.seq = (int)a->seq;
     p.heads = (int)heads;
-    hipLaunchKernelGGL((paged_append_kernel<T, dim()>), dim3((unsigned)chunks, (unsigned)a->batch, (unsigned)((c.kv_heads + heads - 1) / heads)), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+    const dim3 grid((unsigned)chunks, (unsigned)a->batch, (unsigned)((c.kv_heads + heads - 1) / heads));
+    auto go = [&](auto nt) {
+      hipLaunchKernelGGL((paged_append_kernel<T, dim(), decltype(nt)::value>), grid, dim3(threads), 0, static_cast<hipStream_t>(stream), p);
+    };
+    threads == 1024 ? go(std::integral_constant<int, 1024>{}) : threads == 512 ? go(std::integral_constant<int, 512>{})
+                                                                              : go(std::integral_constant<int, 256>{});
   });
   return launch_status(what);
 }

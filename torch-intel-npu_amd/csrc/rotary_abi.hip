@@ -59,7 +59,7 @@ extern "C" lb_status lb_rotary(const lb_rotary_args *a, void *stream) {
   if (a->head_dim < 2 || a->head_dim > LB_ROTARY_MAX_DIMS || a->heads < 1 || a->heads > 65535 || a->k_heads < 0 || a->k_heads > 65535)
     return fail(LB_INVALID_ARGUMENT, "%s: head_dim 2 to %d, heads 1 to 65535 and k_heads 0 to 65535 required", what, LB_ROTARY_MAX_DIMS);
   if (a->batch < 1 || a->seq < 1 || a->batch > kMaxSeq || a->seq > kMaxSeq / a->batch)
-    return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^28 rows required", what);
+    return fail(LB_INVALID_ARGUMENT, "%s: 1 to 2^25 rows required", what);
   const size_t size = a->type == LB_TYPE_FP32 ? 4 : 2;
   Range reads[4], writes[2];
   if (const lb_status st = check_strided(what, "q", a->q, a->batch, a->seq, a->heads, a->head_dim, size, false, false, reads[0]); st != LB_OK) return st;
@@ -102,8 +102,6 @@ extern "C" lb_status lb_rotary(const lb_rotary_args *a, void *stream) {
            (!a->k_heads || (in_pieces(a->k, a->batch, a->seq, a->k_heads, V, size) && in_pieces(a->out_k, a->batch, a->seq, a->k_heads, V, size)));
   };
   const int V = size == 2 && fits(8) ? 8 : fits(4) ? 4 : 1;
-  if (a->batch * a->seq * (a->head_dim / (2 * V) + 2) > (int64_t)1 << 31)
-    return fail(LB_UNSUPPORTED, "%s: more than 2^31 pieces of rows", what);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->type == LB_TYPE_FP32) {
     V == 4 ? launch<float, 4>(a, in_place, s) : launch<float, 1>(a, in_place, s);

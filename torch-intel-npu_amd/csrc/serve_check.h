@@ -10,7 +10,7 @@
 namespace lb {
 namespace abi {
 
-constexpr int64_t kMaxStride = (int64_t)1 << 40, kMaxSeq = (int64_t)1 << 28;
+constexpr int64_t kMaxStride = (int64_t)1 << 40, kMaxSeq = (int64_t)1 << 25;   // (launches of up to 2^31 threads)
 constexpr size_t kMaxBytes = (size_t)1 << 60;   // (no buffer is larger; sums of a few stay in 64 bits)
 
 // Rows [batch, seq, heads] of dim values of `size` bytes; written ones may not share memory with one another.  pieces: they
