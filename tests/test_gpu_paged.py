@@ -115,6 +115,8 @@ CASES = [
     ('bf16', 16, 16, 64, 32, [2100] + [1 + b % 40 for b in range(69)]),
     ('bf16', 4, 1, 64, 32, [1 + (b % 7) * 400 * (b % 31 == 0) + b % 50 for b in range(200)]),
     ('fp16', 16, 8, 128, 32, [1 + (b * 7919) % 1500 for b in range(36)]),
+    ('bf16', 24, 1, 64, 64, [26001, 9]),
+    ('fp16', 16, 1, 128, 64, [20000]),
     ('bf16', 8, 8, 128, 16, [3000] + [1 + b % 40 for b in range(80)]),
     ('bf16', 12, 12, 128, 64, [513, 512, 1] + [1 + b % 30 for b in range(21)]),
 ]

@@ -206,7 +206,10 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   // of a sequence and head lies idle in the mean), and parts no smaller than they must be to fit in them.  (Parts are never
   // more than sequences times heads and the rounds': each sequence has less than one part over what its share of the work is.)
   // Short sequences are not split, for joining parts takes 4 us (one of 500 slots, 3 heads of 64: 6.6 us whole, 8.0 split; of 1200
-  // 9.6 and 8.1; two of 803, one head of 128: 11.7 and 9.3).  Where they are, parts may be small: 8 units, one for each wave.
+  // 9.6 and 8.1; two of 803, one head of 128: 11.7 and 9.3).  Where they are, parts may be small: 8 units, one for each wave.  But the
+  // workgroup that joins n parts reads n sums of as many rows as it has query heads, a CU by itself, while each part takes 1 / n of the
+  // slots, read at that rate too: the two are even where a part has sqrt(units x query heads / 32) units (16 heads of 128 over one KV
+  // head, a sequence of 60001 slots: 39.7 -> 25.3 us; 24 of 64, two of up to 26499: 15.0 -> 13.5).
   constexpr int kRound = 256 * 8 / W;
   constexpr uint32_t kWhole = (D == 64 ? 2 : 1) * kPagedWhole / kUnit, kLeast = 8;
   uint32_t most = kWhole;
@@ -233,7 +236,8 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
         room = ~0u;
         size = work / (float)(kRound * p.rounds);
       }
-      most = max((uint32_t)size + 1, kLeast);
+      const uint32_t even = __builtin_amdgcn_sqrtf(longest * min(p.group, 16) * (1.0f / 32));
+      most = max(max((uint32_t)size + 1, kLeast), even);
       for (int i = 0; i < 4 && lanes_sum((n + most - 1) / most) * heads > room; ++i) most += most / 8 + 1;
     }
   }
