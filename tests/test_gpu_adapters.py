@@ -67,6 +67,11 @@ CASES = [
     ('fp16', 2300, 72, 264, 64, 70),
     ('bf16', 2048, 40, 264, 128, 4),
     ('fp16', 9, 64, 4168, 104, 3),
+    ('fp16', 94, 1544, 2056, 128, 21),
+    ('bf16', 64, 4104, 1032, 8, 64),
+    ('fp16', 200, 264, 1032, 32, 3),
+    ('bf16', 130, 520, 2048, 24, 1),
+    ('fp16', 128, 40, 72, 8, 2),
 ]
 
 

@@ -21,13 +21,18 @@ struct AdaptersPlan {
 
 AdaptersPlan adapters_plan(const lb_adapters_args *a) {
   AdaptersPlan plan{};
-  const int64_t most = std::min<int64_t>(a->count, 16), tiles16 = (a->M + 15) / 16;
-  plan.fused = a->M <= 128 && a->rank <= 64 && a->K * a->rank <= 1 << 15;
+  const int64_t tiles16 = (a->M + 15) / 16;
+  plan.tiles = (a->M + 63) / 64;
+  // What a tile of 64 rows comes to at the most, up to 16 rows of one adapter each.
+  const int64_t full = std::min<int64_t>(tiles16, 4), units = std::min<int64_t>({a->M, 64, a->count + full});
+  // One launch where every workgroup has little of A to go through, and there are few (fp16, one launch and two: 576x576, rank 64 of 8 rows
+  // 7.1, 8.2 us; 576x1536, rank 64 of 2 10.4, 8.3; 4096x4096, rank 8 of 20 rows of 20 adapters 7.5, 8.6, rank 16 of 1 8.1, 8.3;
+  // 960x2560, rank 8 of 30 rows of 40 6.4, 8.6, of 96 of 64 11.4, 9.2; 14336x4096, rank 8 of 64 of 64 68, 13).
+  plan.span = 256;
+  const int64_t all = std::min<int64_t>(a->M, a->count * plan.tiles + tiles16);
+  plan.fused = a->M <= 128 && a->rank <= 64 && a->K * a->rank <= 3 << 14 && all * ((a->N + plan.span - 1) / plan.span) <= 320;
   if (plan.fused) {
-    plan.tiles = tiles16;
-    plan.span = 256;
-    plan.shares = (int)most;
-    plan.bytes = 0;
+    plan.shares = (int)units;
     return plan;
   }
   // Tiles of 64 rows and 64 ranks where x is large, so that it is read once (4096x4096 rank 128 of 3000 rows: 16, 32, 64 ranks a
@@ -35,18 +40,18 @@ AdaptersPlan adapters_plan(const lb_adapters_args *a) {
   // of 40 rows 13.2, 14.3, 16.2 us; rank 64 of 827 rows 25.7, 22.9, 24.0).  Parts of K, of 1024 at the least, until there is a
   // workgroup a CU (4096x14336 rank 32 of one row: 4, 8, 14 parts 13.5, 10.8, 10.3 us).
   plan.rows = a->M * a->K < 3 << 21 ? 1 : 4;
-  plan.tiles = (a->M + 16 * plan.rows - 1) / (16 * plan.rows);
   const int64_t rank16 = (a->rank + 15) / 16;
   plan.ranks = rank16 <= 1 ? 1 : plan.rows == 1 ? (a->M <= 256 ? 1 : 2) : rank16 <= 2 ? 2 : 4;
   plan.groups = (int)((rank16 + plan.ranks - 1) / plan.ranks);
-  const int64_t alone = plan.tiles * plan.groups;
+  const int64_t alone = (plan.rows == 1 ? tiles16 : plan.tiles) * plan.groups;
   plan.slices = (int)std::max<int64_t>(1, std::min<int64_t>({256 / alone, (a->K + 1023) / 1024, 16}));
-  plan.shares = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(a->count, 16 * plan.rows), 512 / (alone * plan.slices)));
+  plan.shares = (int)(plan.rows == 1 ? std::min<int64_t>(units, std::max<int64_t>(full, 512 / (plan.tiles * plan.groups * plan.slices)))
+                                     : std::max<int64_t>(1, std::min<int64_t>({a->count, 64, 512 / (alone * plan.slices)})));
   plan.tile = a->M >= 256;    // (4096x4096 rank 32: 500 rows 13.5 -> 12.0 us, 763 rows of 14336x4096 24.5 -> 18.7)
   plan.stack = tiles16 >= 4 ? 4 : tiles16 >= 2 ? 2 : 1;
-  plan.shares_up = (int)(a->M < 1024 ? most : 1);
+  plan.shares_up = (int)(a->M < 1024 ? (units + plan.stack - 1) / plan.stack : 1);
   plan.span = plan.wide_span = 512;
-  while (plan.span > (a->rank > 32 ? 64 : 128) && tiles16 * plan.shares_up * ((a->N + plan.span - 1) / plan.span) < 2048) plan.span /= 2;
+  while (plan.span > (a->rank > 32 ? 64 : 128) && plan.tiles * plan.shares_up * plan.stack * ((a->N + plan.span - 1) / plan.span) < 2048) plan.span /= 2;
   while (plan.wide_span > 128 && (a->M + 63) / 64 * ((a->N + plan.wide_span - 1) / plan.wide_span) < 512) plan.wide_span /= 2;
   plan.bytes = ((size_t)plan.slices * a->M * a->rank * 4 + 255) / 256 * 256;
   return plan;
@@ -105,9 +110,9 @@ void launch(const lb_adapters_args *a, const AdaptersPlan &plan, hipStream_t s) 
     a->rank <= 16 ? go(One{}) : a->rank <= 32 ? go(Two{}) : go(Four{});
     return;
   }
-  const int64_t wide = plan.span * (4 / plan.stack), rows = 16 * plan.stack;   // of a workgroup of adapters_up_kernel
+  const int64_t wide = plan.span * (4 / plan.stack);   // outputs of a workgroup of adapters_up_kernel
   const dim3 down((unsigned)(plan.tiles * plan.slices * plan.groups), (unsigned)plan.shares);
-  const dim3 up((unsigned)((a->M + rows - 1) / rows * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up + 1);
+  const dim3 up((unsigned)(plan.tiles * ((a->N + wide - 1) / wide)), (unsigned)plan.shares_up + 1);
   const dim3 tile((unsigned)((a->M + 63) / 64 * ((a->N + plan.wide_span - 1) / plan.wide_span)));
   auto first = [&](auto rt) {
     constexpr int RT = decltype(rt)::value;

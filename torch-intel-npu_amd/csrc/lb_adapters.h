@@ -1,10 +1,11 @@
 // gfx950 kernels of lb_adapters (include/lowbit_decode_hip.h): out = y + s (x A^T) B^T, the factors A [rank, K] and
 // B [N, rank] those of each row's own adapter.
 //
-// Two launches: z = x A^T in fp32 (adapters_down_kernel), then y + s z B^T (adapters_up_kernel).  Both take tiles of rows
-// as the columns of 16x16x32 products, whose rows are ranks and outputs, so that a lane holds one row throughout and rows
-// of other adapters in the tile cost nothing but their share of an instruction: a tile goes once through the factors
-// of each adapter that it holds, whatever their order.
+// z = x A^T in fp32 (adapters_down_kernel), then y + s z B^T (adapters_up_kernel, or of many rows adapters_tile_kernel), or both in one
+// launch where that is little (adapters_rows_kernel).  Rows are the columns of 16x16x32 products, whose rows are ranks and
+// outputs, so that a lane holds one row throughout.  Of few rows, the columns are up to 16 of one adapter, wherever they lie among 64
+// (94 rows of 21 adapters in no order, 14336 by 4096, rank 128: 43.6 us, against 66.2 with columns of 16 rows side by side); of many,
+// 64 rows side by side, each adapter's in turn.
 #pragma once
 #include "lb_serve.h"
 
@@ -22,7 +23,7 @@ struct AdaptersParams {
   long long ldx, ldy, ldo;
   int M, N, K, rank, count;
   int slices, groups;       // parts of K, added in the second launch; groups of ranks
-  int shares, shares_up;    // workgroups that share a tile's adapters, in each launch
+  int shares, shares_up;    // workgroups that share a tile of rows, in each launch
   int span, stack;          // adapters_up_kernel: outputs of a wave, tiles of a workgroup (adapters_rows_kernel: outputs of one)
   int wide;                 // rows of y and out are whole 16-byte pieces
 };
@@ -47,8 +48,32 @@ __device__ __forceinline__ void each_adapter(int id, int share, int shares, F &&
   }
 }
 
+// Calls f(adapter, row, rows) for this share of what a tile of 64 rows holds, up to 16 rows of one adapter at a time: `row` that of the lane's
+// column (lane % 16, where that is below `rows`).  So an adapter's factors are read once for its rows, wherever in the tile they are.
+// (Every lane finds the rows of its adapter at once, by the bits of its number, so that a share has its part without going through those
+// before it: adapter by adapter took 4 us of a tile of 64.)
+template <class F>
+__device__ __forceinline__ void each_sixteen(int id, int lane, int count, int share, int shares, F &&f) {
+  uint64_t same = __ballot(id >= 0);
+  for (int bits = count - 1, bit = 0; bits >> bit; ++bit) {
+    const uint64_t set = __ballot(id >> bit & 1);
+    same &= id >> bit & 1 ? set : ~set;
+  }
+  const int before = __popcll(same & ((1ull << lane) - 1));      // rows of the lane's adapter before its own
+  const uint64_t firsts = __ballot(id >= 0 && before % 16 == 0);
+  const int index = __builtin_amdgcn_mbcnt_hi((uint32_t)(firsts >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)firsts, 0));
+  for (int n = share; n < (int)__popcll(firsts); n += shares) {
+    const int at = __builtin_ctzll(__ballot((firsts >> lane & 1) && index == n));
+    const int a = __builtin_amdgcn_readlane(id, at), column = before - __builtin_amdgcn_readlane(before, at);
+    const bool mine = id == a && column >= 0 && column < 16;
+    const int row = __builtin_amdgcn_ds_permute(4 * (mine ? column : 63), lane);   // (nobody asks lane 63)
+    f(a, __shfl(row, lane & 15), (int)__popcll(__ballot(mine)));
+  }
+}
+
 // z of 16 MT rows and 16 RT ranks over one slice of K: waves take every eighth 64 of it and meet in LDS.  The rows' memory bounds it
 // (4001 rows of 4096, rank 32: 15 us), or with few rows the chain of index, factors and sums (4.8 us for 64 rows of 64 adapters).
+// (MT 1: up to 16 rows of one adapter in 64; MT 4: 64 rows of any, each adapter's in turn.)
 template <class T, int RT, int MT>
 __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -56,10 +81,11 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
   __shared__ f4 met[W][TILES][64];
   const int lane = threadIdx.x & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slice = blockIdx.x % p.slices, rest = blockIdx.x / p.slices, rank0 = rest % p.groups * (16 * RT), first = rest / p.groups * (16 * MT);
-  const int id = adapter_of(p, first, lane, 16 * MT);
+  const int slice = blockIdx.x % p.slices, rest = blockIdx.x / p.slices, rank0 = rest % p.groups * (16 * RT), first = rest / p.groups * 64;
+  const int id = adapter_of(p, first, lane, 64);
   const int all = (p.K + 63) / 64, size = (all + p.slices - 1) / p.slices, from = slice * size, to = min(all, from + size);
-  each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
+  // Rows of an adapter's columns 16 t + c, behind `first`, and whether they are its own.
+  auto part = [&](int a, auto row_of, auto lives) {
     f4 acc[RT][MT] = {};
     const T *const down = p.down + (size_t)a * p.rank * p.K;
     const int row = j % 8, at = 32 * (j / 8) + 8 * g;       // (see rows_from_lines)
@@ -71,8 +97,8 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
       for (int r = 0; r < RT; ++r) dr[r][b] = down + (size_t)min(rank0 + 16 * r + 8 * b + row, p.rank - 1) * p.K + at;
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
-        live[t][b] = mine >> (16 * t + 8 * b + row) & 1;
-        xr[t][b] = p.x + (size_t)min(first + 16 * t + 8 * b + row, p.M - 1) * p.ldx + at;
+        live[t][b] = lives(t, 8 * b + row);
+        xr[t][b] = p.x + (size_t)min(first + row_of(t, 8 * b + row), p.M - 1) * p.ldx + at;
       }
     }
     const u4 none = {0, 0, 0, 0};
@@ -114,22 +140,30 @@ __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p)
       f4 sum = met[0][i][lane];
 #pragma unroll
       for (int w = 1; w < W; ++w) sum += met[w][i][lane];
-      const int rank = rank0 + i / MT * 16 + 4 * g, row = i % MT * 16 + j;
-      if (rank < p.rank && (mine >> row & 1))
-        *reinterpret_cast<f4 *>(p.z + ((size_t)slice * p.M + first + row) * p.rank + rank) = sum;
+      const int rank = rank0 + i / MT * 16 + 4 * g, at_row = row_of(i % MT, j);
+      if (rank < p.rank && lives(i % MT, j)) *reinterpret_cast<f4 *>(p.z + ((size_t)slice * p.M + first + at_row) * p.rank + rank) = sum;
     }
-  });
+  };
+  if constexpr (MT == 1)
+    each_sixteen(id, lane, p.count, blockIdx.y, p.shares, [&](int a, int at_row, int rows) {
+      part(a, [&](int, int c) { return __shfl(at_row, c); }, [&](int, int c) { return c < rows; });
+    });
+  else
+    each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
+      part(a, [&](int t, int c) { return 16 * t + c; }, [&](int t, int c) { return (bool)(mine >> (16 * t + c) & 1); });
+    });
 }
 
-// Rows of 16 without an adapter, and those whose adapter there is not: y's values or NaNs, outputs from .. to - 1, by the lanes of a
-// wave, 8 outputs a lane at once.
+// Rows row0 .. row0 + 15 of a tile without an adapter, and those whose adapter there is not: y's values or NaNs, outputs from .. to
+// - 1, by the lanes of a wave, 8 outputs a lane at once.
 template <class T>
-__device__ __forceinline__ void rows_without(const AdaptersParams<T> &p, int id, int first, int lane, int from, int to) {
+__device__ __forceinline__ void rows_without(const AdaptersParams<T> &p, int id, int first, int row0, int lane, int from, int to) {
   typedef typename Of16<T>::x8 x8;
-  if (!__ballot(lane < 16 && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y))) return;
+  if (!__ballot(lane >= row0 && lane < row0 + 16 && first + lane < p.M && id < 0 && (id == -2 || p.out != p.y))) return;
   const int pieces = (to - from + 7) / 8;
+  const int ids = __shfl(id, row0 + (lane & 15));      // (of lanes that take part to the end)
   for (int i = lane; i < 16 * pieces; i += 64) {
-    const int row = i / pieces, n = from + 8 * (i - row * pieces), whose = __shfl(id, row);
+    const int row = row0 + i / pieces, n = from + 8 * (i % pieces), whose = __shfl(ids, row - row0);
     if (first + row >= p.M || whose >= 0 || (whose == -1 && p.out == p.y)) continue;
     const T *const y = p.y + (size_t)(first + row) * p.ldy + n;
     T *const out = p.out + (size_t)(first + row) * p.ldo + n;
@@ -258,9 +292,9 @@ struct Writer {
   }
 };
 
-// z of row j of 16 from `first` on, its slices added in their order.
+// z of a row, its slices added in their order.
 template <class T, int RC>
-__device__ __forceinline__ void gather(const AdaptersParams<T> &p, int first, bool live, int j, int g, float (&z)[RC][8]) {
+__device__ __forceinline__ void gather(const AdaptersParams<T> &p, int row, bool live, int g, float (&z)[RC][8]) {
   // Parts in flight: the registers of four of rank 128 leave room for one wave a SIMD (64 rows of 60 adapters, 4096 outputs: 31.0 us
   // against 27.1).
   constexpr int SLICES = RC == 4 ? 2 : 4;
@@ -271,7 +305,7 @@ __device__ __forceinline__ void gather(const AdaptersParams<T> &p, int first, bo
 #pragma unroll
       for (int c = 0; c < RC; ++c)
         if (live && s0 + s < p.slices && 32 * c + 8 * g < p.rank) {
-          const float *const at = p.z + ((size_t)(s0 + s) * p.M + first + j) * p.rank + 32 * c + 8 * g;
+          const float *const at = p.z + ((size_t)(s0 + s) * p.M + row) * p.rank + 32 * c + 8 * g;
           part[s][c][0] = *reinterpret_cast<const f4 *>(at);
           part[s][c][1] = *reinterpret_cast<const f4 *>(at + 4);
         }
@@ -284,8 +318,8 @@ __device__ __forceinline__ void gather(const AdaptersParams<T> &p, int first, bo
   }
 }
 
-// out = y + s z B^T.  A wave takes 16 rows and `span` outputs; the waves of a workgroup have `stack` tiles of rows and 4 / stack
-// spans.  (64 rows of 64 adapters, 4096 outputs, rank 16: 6.5 us, of which the launch and the loads of index, z and factors one after
+// out = y + s z B^T.  A wave takes up to 16 rows of one adapter in 64, and `span` outputs; the waves of a workgroup have `stack` of those and
+// 4 / stack spans.  (64 rows of 64 adapters, 4096 outputs, rank 16: 5.4 us, of which the launch and the loads of index, z and factors one after
 // the other are most.)
 template <class T, int RC>
 __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
@@ -293,22 +327,23 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int beside = 4 / p.stack, spans = (p.N + p.span * beside - 1) / (p.span * beside);
   const int from = (blockIdx.x % spans * beside + wave / p.stack) * p.span, to = min(p.N, from + p.span);
-  const int first = (blockIdx.x / spans * p.stack + wave % p.stack) * 16;
+  const int first = blockIdx.x / spans * 64;
   if (from >= to) return;
-  const int id = adapter_of(p, first, lane, 16);
+  const int id = adapter_of(p, first, lane, 64);
   if (blockIdx.y == p.shares_up) {        // (workgroups of their own, so that no product waits for it)
-    rows_without(p, id, first, lane, from, to);
+    for (int i = wave % p.stack; i < 4; i += p.stack) rows_without(p, id, first, 16 * i, lane, from, to);
     return;
   }
-  each_adapter(id, blockIdx.y, p.shares_up, [&](int a, uint64_t mine) {
-    const bool live = mine >> j & 1;
+  each_sixteen(id, lane, p.count, blockIdx.y * p.stack + wave % p.stack, p.shares_up * p.stack, [&](int a, int at_row, int rows) {
+    const bool live = j < rows;
+    const int row = first + at_row;
     const T *const up = p.up + (size_t)a * p.N * p.rank;
-    const T *const y = p.y + (size_t)(first + j) * p.ldy;
-    T *const out = p.out + (size_t)(first + j) * p.ldo;
+    const T *const y = p.y + (size_t)row * p.ldy;
+    T *const out = p.out + (size_t)row * p.ldo;
     Writer<T, RC> writer;
     writer.begin(p, up, y, from, to, live, j, g);
     float scale = p.scales ? p.scales[a] : 1.0f, z[RC][8] = {};
-    gather<T, RC>(p, first, live, j, g, z);
+    gather<T, RC>(p, row, live, g, z);
     Halves<T, RC> halves;
     halves.split(z, scale);
     writer.run(p, up, y, out, halves, scale, from, to, 64, live, j, g);
@@ -437,7 +472,7 @@ __global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p)
   }
 }
 
-// Both products of 16 rows in one launch, for few rows: a workgroup of W waves computes z of an adapter of the tile itself (its
+// Both products in one launch, for few rows: a workgroup of W waves computes z of up to 16 rows of one adapter in 64 itself (its
 // waves take every W-th 64 of K and meet in LDS) and `span` outputs, 64 a wave at a time, whose factors and y are requested
 // before z is there.  Every span's workgroup reads the whole of A again, from the caches.  5 rows of 576 by 576, rank 8: 4.3 us, hardly
 // more than an empty launch takes.
@@ -450,23 +485,25 @@ __global__ __launch_bounds__(64 * kRowsWaves) void adapters_rows_kernel(Adapters
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int spans = (p.N + p.span - 1) / p.span;
-  const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * 16;
-  const int id = adapter_of(p, first, lane, 16), all = (p.K + 63) / 64;
+  const int from = blockIdx.x % spans * p.span, to = min(p.N, from + p.span), first = blockIdx.x / spans * 64;
+  const int id = adapter_of(p, first, lane, 64), all = (p.K + 63) / 64;
   if (blockIdx.y == p.shares) {           // (workgroups of their own, so that no product waits for it)
-    for (int n0 = from + 64 * wave; n0 < to; n0 += 64 * W) rows_without(p, id, first, lane, n0, min(to, n0 + 64));
+    for (int i = 0; i < 64; i += 16)
+      for (int n0 = from + 64 * wave; n0 < to; n0 += 64 * W) rows_without(p, id, first, i, lane, n0, min(to, n0 + 64));
     return;
   }
-  each_adapter(id, blockIdx.y, p.shares, [&](int a, uint64_t mine) {
-    const bool live = mine >> j & 1;
+  each_sixteen(id, lane, p.count, blockIdx.y, p.shares, [&](int a, int at_row, int rows) {
+    const bool live = j < rows;
+    const int row = first + at_row;
     const T *const up = p.up + (size_t)a * p.N * p.rank;
-    const T *const y = p.y + (size_t)(first + j) * p.ldy;
-    T *const out = p.out + (size_t)(first + j) * p.ldo;
+    const T *const y = p.y + (size_t)row * p.ldy;
+    T *const out = p.out + (size_t)row * p.ldo;
     Writer<T, RC> writer;
     const int mine0 = from + 64 * wave;
     if (mine0 < to) writer.begin(p, up, y, mine0, to, live, j, g);
     float scale = p.scales ? p.scales[a] : 1.0f;
     f4 acc[RT] = {};
-    const T *const down = p.down + (size_t)a * p.rank * p.K + 8 * g, *const x = p.x + (size_t)(first + j) * p.ldx + 8 * g;
+    const T *const down = p.down + (size_t)a * p.rank * p.K + 8 * g, *const x = p.x + (size_t)row * p.ldx + 8 * g;
     for (int piece = wave; piece < all; piece += W * AHEAD) {
       x8 d[AHEAD][2][RT], xv[AHEAD][2];
 #pragma unroll
