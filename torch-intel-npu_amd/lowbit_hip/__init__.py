@@ -1210,9 +1210,9 @@ def _kv_run(fn, args, device, what, stream=None):
     index = device.index
     if index is not None and index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            status = fn(args, ctypes.c_void_p(_raw_stream(device) if stream is None else stream))
+            status = fn(args, _raw_stream(device) if stream is None else stream)
     else:
-        status = fn(args, ctypes.c_void_p(_raw_stream(device) if stream is None else stream))
+        status = fn(args, _raw_stream(device) if stream is None else stream)
     if status != OK:
         _check(status, what)
 

@@ -223,8 +223,12 @@ def _head_rows(t, name, shape, dtype, device):
         raise ValueError(f'{name} must be {dtype} [batch, seq, heads, head_dim] = {list(shape)}')
     if t.device != device:
         raise ValueError(f'{name} must be on {device} with q (found {t.device})')
+    return _heads(t, name)
+
+
+def _heads(t, name):
     b, i, h, d = t.stride()
-    if d != 1 and shape[3] > 1:
+    if d != 1 and t.shape[3] > 1:
         raise ValueError(f'the heads of {name} must be contiguous')
     return t.data_ptr(), b, i, h
 
@@ -238,7 +242,7 @@ def _rotary_args(q, position, rotary, out, k, out_k, back):
     batch, seq, heads, dim = shape
     if (k is None) != (out_k is None):
         raise ValueError('k and out_k go together')
-    q, out = _head_rows(q, 'q', shape, dtype, device), _head_rows(out, 'out', shape, dtype, device)
+    q, out = _heads(q, 'q'), _head_rows(out, 'out', shape, dtype, device)
     if k is None:
         k_heads, k, out_k = 0, _NO_ROWS, _NO_ROWS
     else:
@@ -360,24 +364,26 @@ def _paged_cache(cache):
 
 
 def _page_table(t, batch, device):
-    if (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.ndim != 2 or t.shape[0] != batch or t.shape[1] < 1
-            or (t.stride(1) != 1 and t.shape[1] > 1)):
-        raise ValueError(f'table must be int32 [batch, pages] = [{batch}, pages] with contiguous rows')
-    if t.device != device:
-        raise ValueError(f'table must be on {device} with the cache (found {t.device})')
-    return t.data_ptr(), t.stride(0), t.shape[1]
+    if isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.ndim == 2:
+        (rows, longest), (stride, step) = t.shape, t.stride()
+        if rows == batch and longest >= 1 and (step == 1 or longest == 1):
+            if t.device != device:
+                raise ValueError(f'table must be on {device} with the cache (found {t.device})')
+            return t.data_ptr(), stride, longest
+    raise ValueError(f'table must be int32 [batch, pages] = [{batch}, pages] with contiguous rows')
 
 
 def _append_args(cache, k, v, table, position, rows, rotary, keep, copy):
     cache = _paged_cache(cache)
     if not isinstance(k, torch.Tensor) or k.ndim != 4 or k.numel() == 0:
         raise ValueError('k must be [batch, seq, kv_heads, head_dim]')
-    batch, seq = k.shape[:2]
-    shape, device = (batch, seq, cache.kv_heads, cache.head_dim), cache.device
-    k, v = (_rows(t, name, shape, cache.dtype, device, keep, copy) for t, name in ((k, 'k'), (v, 'v')))
+    batch, seq, _, _ = k.shape
+    device, dtype, dim = cache.device, cache.dtype, cache.head_dim
+    shape, counts = (batch, seq, cache.kv_heads, dim), (batch,)
     return PagedAppendArgs.from_buffer_copy(cache._heads[PagedAppendArgs] + _APPEND.pack(
-        *_page_table(table, batch, device), batch, seq, *k, *v, _counts(position, 'position', (batch,), device),
-        0 if rows is None else _counts(rows, 'rows', (batch,), device)) + _rotation(rotary, device, cache.head_dim))
+        *_page_table(table, batch, device), batch, seq, *_rows(k, 'k', shape, dtype, device, keep, copy),
+        *_rows(v, 'v', shape, dtype, device, keep, copy), _counts(position, 'position', counts, device),
+        0 if rows is None else _counts(rows, 'rows', counts, device)) + _rotation(rotary, device, dim))
 
 
 def paged_append(cache, k, v, table, position, *, rows=None, rotary=None):
