@@ -72,7 +72,7 @@ __device__ __forceinline__ void each_sixteen(int id, int lane, int count, int sh
 }
 
 // z of 16 MT rows and 16 RT ranks over one slice of K: waves take every eighth 64 of it and meet in LDS.  The rows' memory bounds it
-// (4001 rows of 4096, rank 32: 15 us), or with few rows the chain of index, factors and sums (4.8 us for 64 rows of 64 adapters).
+// (4001 rows of 4096, rank 32: 13.4 us), or with few rows the chain of index, factors and sums (5.0 us for 64 rows of 64 adapters).
 // (MT 1: up to 16 rows of one adapter in 64; MT 4: 64 rows of any, each adapter's in turn.)
 template <class T, int RT, int MT>
 __global__ __launch_bounds__(512) void adapters_down_kernel(AdaptersParams<T> p) {
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(AdaptersParams<T> p) {
 // 256 bytes, 1 KB a wave at once, since a transfer whose lanes have 16 rows costs the address unit twice that of whole lines;
 // the products come to the lanes of those rows through LDS.  z is added up and split once a workgroup, and kept in LDS; the
 // factors of 32 outputs, which a wave holds, serve all rows of the tile.  Memory bounds it: 4001 rows of 14336 outputs, rank 32, 229 MB
-// of y and out, take 53 us (4.3 TB/s).  (out is stored past the caches: 5360 rows of 4096, both launches, 44.3 -> 41.0 us.)
+// of y and out, take 52 us (4.4 TB/s).  (out is stored past the caches: 5360 rows of 4096, both launches, 44.3 -> 41.0 us.)
 template <class T, int RC>
 __global__ __launch_bounds__(256) void adapters_tile_kernel(AdaptersParams<T> p) {
   typedef typename Of16<T>::x8 x8;
