@@ -564,8 +564,8 @@ lb_status lb_paged_attention_workspace_bytes(const lb_paged_attention_args *args
 
 /*
  * Grouped-query attention of one new token a sequence: the token at slot p attends over slots 0 .. p.  Scores, softmax and
- * sums in fp32, the probabilities rounded to the type for the product with the values, out rounded once.  The slots are
- * split over the chip by what the sequences hold, found on the device, and the parts joined in a fixed order.  What lies
+ * sums in fp32, the probabilities rounded to fp16 or taken as two numbers of bf16 for the product with the values, out rounded
+ * once.  The slots are split over the chip by what the sequences hold, found on the device, and the parts joined in a fixed order.  What lies
  * behind slot p in its page is not looked at, whatever it is.  A position past the table (or below -1), or an entry of
  * the table below a sequence's length that is not a page, gives NaN in the sequence's out.
  */
@@ -574,7 +574,7 @@ lb_status lb_paged_attention(const lb_paged_attention_args *args, void *stream);
 /*
  * Low-rank adapters of many requests beside a projection that they share: out[m] = y[m] + s_a (x[m] A_a^T) B_a^T for row m
  * with adapter a = index[m], out[m] = y[m] where a is -1, and NaN where it is no adapter.  Rows are taken in any order of
- * adapters; those of one adapter are fastest side by side.
+ * adapters; of more than 64 rows, those of one adapter are fastest side by side.
  */
 #define LB_ADAPTERS_MAX_RANK 128
 
