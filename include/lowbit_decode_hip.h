@@ -549,7 +549,7 @@ typedef struct lb_paged_attention_args {
   lb_rows q, out;              /* [batch, 1, heads] rows of the cache's type, whole 16-byte pieces (row_stride is not read) */
   const int64_t *position;     /* device [batch]: the slot of a sequence's new token; -1: it has none, and out is 0 */
   lb_rows k, v;                /* data NULL: the token's row is in its page already; else [batch, 1, kv_heads], appended */
-  lb_rotation rotation;        /* of q (and k) by position, rounded to the type (frequencies NULL: taken as they are) */
+  lb_rotation rotation;        /* of q (and k, then rounded to the type) by position (frequencies NULL: taken as they are) */
   float scale;                 /* score scale, finite (usually 1 / sqrt(head_dim)) */
   uint32_t reserved2;
   void *workspace;             /* lb_paged_attention_workspace_bytes, 256-byte aligned.  Its first LB_ZEROED_WORKSPACE_BYTES
