@@ -36,12 +36,14 @@ AdaptersPlan adapters_plan(const lb_adapters_args *a) {
     return plan;
   }
   // Tiles of 64 rows and 64 ranks where x is large, so that it is read once (4096x4096 rank 128 of 3000 rows: 16, 32, 64 ranks a
-  // workgroup 68.4, 51.7, 47.0 us); elsewhere of 16 rows, and of 16 ranks where those are few, for more workgroups (rank 128
+  // workgroup 68.4, 51.7, 47.0 us); sooner where there are more groups of ranks that each read it (64 rows and 16: rank 128, 270 rows of
+  // 14336 28.7, 37.8 us, 150 rows 30.5, 23.4; rank 64, 400 rows 23.9, 27.1, 300 rows 22.4, 20.7; rank 32, 2000 rows of 4096 20.2, 23.6,
+  // 300 of 14336 17.5, 14.8); elsewhere of 16 rows, and of 16 ranks where those are few, for more workgroups (rank 128
   // of 40 rows 13.2, 14.3, 16.2 us; rank 64 of 827 rows 25.7, 22.9, 24.0).  Parts of K, of 1024 at the least, while there are
   // fewer than 224 workgroups (4096x14336 rank 32 of one row: 4, 8, 14 parts 10.7, 9.8, 9.8 us), but no more than the second launch
   // adds up quickly, four at once: each of its workgroups reads them all (4096x14336, rank 64 of 1500 rows, 8 parts 30.7, 9 37.0;
   // rank 32 of 3000, 4 parts 41.3, 5 54.2; 4096x4096, rank 32 of 5360, 2 parts 37.3, 3 42.4; rank 128 of 30 rows, 4 parts 18.2, 14 22.3).
-  plan.rows = a->M * a->K < 3 << 21 ? 1 : 4;
+  plan.rows = a->M * a->K < (a->rank <= 32 ? 7 : a->rank <= 64 ? 5 : 3) << 20 ? 1 : 4;
   const int64_t rank16 = (a->rank + 15) / 16;
   plan.ranks = rank16 <= 1 ? 1 : plan.rows == 1 ? (a->M <= 256 ? 1 : 2) : rank16 <= 2 ? 2 : 4;
   plan.groups = (int)((rank16 + plan.ranks - 1) / plan.ranks);
