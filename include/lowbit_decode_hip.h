@@ -564,7 +564,7 @@ lb_status lb_paged_attention_workspace_bytes(const lb_paged_attention_args *args
 
 /*
  * Grouped-query attention of one new token a sequence: the token at slot p attends over slots 0 .. p.  Scores, softmax and
- * sums in fp32, the probabilities rounded to fp16 or taken as two numbers of bf16 for the product with the values, out rounded
+ * sums in fp32, the probabilities taken as two numbers of the type for the product with the values, out rounded
  * once.  The slots are split over the chip by what the sequences hold, found on the device, and the parts joined in a fixed order.  What lies
  * behind slot p in its page is not looked at, whatever it is.  A position past the table (or below -1), or an entry of
  * the table below a sequence's length that is not a page, gives NaN in the sequence's out.

@@ -1,0 +1,51 @@
+"""lb_paged_attention where the bits of its probabilities and the range of its numbers show, against its definition in 64 bits
+(the bounds of test_gpu_paged, but for what is said here)."""
+import numpy as np
+import pytest
+import torch
+
+import lowbit_hip as lb
+from conftest import announce
+from oracle import serve_oracle as so
+from test_gpu_paged import TYPES, filled, host, ints, rand, table_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('type', ['fp16', 'bf16'])
+@pytest.mark.parametrize('heads,kv,dim', [(4, 2, 64), (8, 8, 128)])
+def test_probabilities_keep_their_bits(device, type, heads, kv, dim):
+    """Sums over 31 slots that cancel: what is rounded of a probability is then large beside the output.
+
+    The last slot's value is set against the sum of the others, so that of A = sum p |v| hardly anything is left and the output's own
+    half step is small.  A probability enters as two numbers of its type: what is left of it is half a step of the second (a quarter
+    of the square of the type's step: 2^-22 of it in fp16, 2^-17 in bf16 as test_gpu_paged counts it), and of fp16 half of
+    2^-24 relative to a largest one of 2^10 (31 2^-35 of max|v|).  The score: (D + 8) 2^-24 R and the exponential's 2^-22, in the sum
+    and in the total.  One unit of slots in one wave: 32 additions of the products, 8 of the waves, the same of the total,
+    and a quotient: 96 2^-24.  Rounded to one fp16 number, each p is off by up to 2^-12 of A by itself."""
+    announce('paged bits', type, heads, kv, dim)
+    n, page, eps = 31, 16, torch.finfo(TYPES[type]).eps
+    cache = filled(device, type, 3, kv, page, dim, seed=21, loud=False)
+    cache.keys.mul_(0.0625)
+    table = ints([[2, 0]], device).int()
+    q = rand(device, type, 1, heads, dim, seed=22)
+    scale, group = dim ** -0.5, heads // kv
+    keys, values = host(cache.keys), host(cache.values)
+    k, v = so.held(keys, values, [2, 0], n)
+    for h in range(kv):                     # against the sum that the group's first query sees
+        s = k[h] @ host(q)[0, h * group].astype(np.float64) * scale
+        p = np.exp(s - s.max())
+        values[0, h, 0, :, (n - 1) % 16] = -(p[:-1] @ v[h, :-1]) / p[-1]
+    cache.values.copy_(torch.from_numpy(values))
+    values = host(cache.values)
+    k, v = so.held(keys, values, [2, 0], n)
+    want, mean, size = so.attention(host(q[0]), k, v, scale)
+    out = host(lb.paged_attention(q, cache, table, ints([n - 1], device))[0]).astype(np.float64)
+    score = (dim + 8) * 2.0 ** -24 * size[:, None] + 2.0 ** -22
+    left, tiny = (2.0 ** -22, n * 2.0 ** -35 * np.abs(v).max()) if type == 'fp16' else (2.0 ** -17, 0.0)
+    near = (left + 2 * np.expm1(score) + 2 * 96 * 2.0 ** -24) * mean + 2 * tiny
+    bound = near + eps / 2 * (np.abs(want) + near) + 2.0 ** -25 * (type == 'fp16')
+    first = np.arange(kv) * group
+    worst = float(np.max((np.abs(out - want) / bound)))
+    assert float(np.median(np.abs(want[first]) / mean[first])) < eps      # (they do cancel)
+    assert worst <= 1, worst

@@ -454,11 +454,10 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[d] *= shrink;
     }
-    // A probability's rounding to bf16, 2^-8 of it, would be as large as the output's own: what it takes away is a second operand (one
-    // sequence of 130999 slots, 8 heads of 128: 86.0 -> 86.4 us, 32 of up to 1984, 3 of 64: 11.3 -> 11.45).  fp16's is 2^-11, and
-    // there the total is the sum of the rounded ones.
-    constexpr bool SPLIT = __is_same(T, bf16);
-    x8 x[C / 2], rest[SPLIT ? C / 2 : 1];
+    // A probability enters the product as the sum of two numbers of the type, for its rounding to one (2^-8 of it in bf16, 2^-11 in fp16)
+    // is as large as the output's own, and larger where values cancel (one sequence of 130999 slots, 8 heads of 128, bf16: 86.0 -> 86.4
+    // us; 32 of up to 1984, 3 of 64, fp16: 11.3 -> 11.5; 64 of up to 8192, 8 of 128, fp16: 178.4 -> 178.3).
+    x8 x[C / 2], rest[C / 2];
 #pragma unroll
     for (int t = 0; t < C; ++t)
 #pragma unroll
@@ -466,15 +465,15 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
         const float prob = __builtin_amdgcn_exp2f(s[t][e] - ref);
         const T high = (T)prob;
         x[t / 2][t % 2 * 4 + e] = high;
-        if constexpr (SPLIT) rest[t / 2][t % 2 * 4 + e] = (T)(prob - (float)high);
-        total += SPLIT ? prob : (float)high;
+        rest[t / 2][t % 2 * 4 + e] = (T)(prob - (float)high);
+        total += prob;
       }
 #pragma unroll
     for (int t = 0; t < C; t += 2)
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         acc[d] = Of16<T>::mma(vf[t / 2][d], x[t / 2], acc[d]);
-        if constexpr (SPLIT) acc[d] = Of16<T>::mma(vf[t / 2][d], rest[t / 2], acc[d]);
+        acc[d] = Of16<T>::mma(vf[t / 2][d], rest[t / 2], acc[d]);
       }
     if (next < (int)to) fetch_values();
   }
