@@ -49,3 +49,32 @@ def test_probabilities_keep_their_bits(device, type, heads, kv, dim):
     worst = float(np.max((np.abs(out - want) / bound)))
     assert float(np.median(np.abs(want[first]) / mean[first])) < eps      # (they do cancel)
     assert worst <= 1, worst
+
+
+@pytest.mark.parametrize('type', ['fp16', 'bf16'])
+@pytest.mark.parametrize('sign', [1, -1])
+def test_scores_of_any_size(device, type, sign):
+    """Equal scores of 2^5 to 2^34 in units of log2, on either side of zero: the values' mean, however coarse the scores' own steps
+    are (16 of those units from 2^27 on).  Then one slot a step above the others: past 2^32, where a step is 512, its value alone.
+
+    All probabilities are equal, so that they cancel exactly from the quotient but for their sums: 2^-16 covers 8 additions a lane of
+    each, the joins' and the quotient's, and bf16's second number (2^-17); then the output's half step."""
+    announce('paged scores of any size', type, sign)
+    n, page, dim = 200, 32, 64
+    cache = filled(device, type, 7, 1, page, dim, seed=31)
+    table = ints([list(range(7))], device).int()
+    _, v = so.held(host(cache.keys), host(cache.values), range(7), n)
+    mean, size = v[0].mean(0), np.abs(v[0]).mean(0)
+    q = torch.zeros((1, 2, dim), dtype=TYPES[type], device=device)
+    q[0, :, 3] = 2.0 ** 11
+    half = torch.finfo(TYPES[type]).eps / 2
+    cache.keys.zero_()
+    for e in range(-17, 13):
+        for part in (1.0, 1.25, 1.375):
+            cache.keys[..., 3] = sign * 2.0 ** 11 * part
+            out = host(lb.paged_attention(q, cache, table, ints([n - 1], device), scale=2.0 ** e))[0].astype(np.float64)
+            worst = float(np.max(np.abs(out - mean) / ((half + 2.0 ** -16) * size + 2.0 ** -25)))
+            assert worst <= 1, (e, part, worst)
+    cache.keys[2, 0, 9, 3] *= 1.0 + sign * torch.finfo(TYPES[type]).eps * 2     # slot 73: the largest by a 512th or more
+    out = lb.paged_attention(q, cache, table, ints([n - 1], device), scale=2.0 ** 12)
+    assert torch.equal(out[0, 0], cache.values[2, 0, 0, :, 9]) and torch.equal(out[0, 1], out[0, 0])

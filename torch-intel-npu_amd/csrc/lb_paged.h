@@ -447,7 +447,9 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][e]);
     if (__any(top - ref > kPagedLift + kPagedSlack)) {
-      const float raised = fmaxf(ref, kv_max_across(top) - kPagedLift);
+      // (Where a score's own step is 16, from 2^27 on, the difference rounds to one past what fp16 has room for.)
+      const float largest = kv_max_across(top), below = largest - kPagedLift;
+      const float raised = fmaxf(ref, largest - below > kPagedLift + kPagedSlack ? largest : below);
       const float shrink = __builtin_amdgcn_exp2f(ref - raised);
       ref = raised;
       total *= shrink;
