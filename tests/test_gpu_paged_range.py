@@ -7,7 +7,7 @@ import torch
 import lowbit_hip as lb
 from conftest import announce
 from oracle import serve_oracle as so
-from test_gpu_paged import TYPES, filled, host, ints, rand, table_of
+from test_gpu_paged import check, TYPES, filled, host, ints, rand, table_of
 
 pytestmark = pytest.mark.gpu
 
@@ -78,3 +78,23 @@ def test_scores_of_any_size(device, type, sign):
     cache.keys[2, 0, 9, 3] *= 1.0 + sign * torch.finfo(TYPES[type]).eps * 2     # slot 73: the largest by a 512th or more
     out = lb.paged_attention(q, cache, table, ints([n - 1], device), scale=2.0 ** 12)
     assert torch.equal(out[0, 0], cache.values[2, 0, 0, :, 9]) and torch.equal(out[0, 1], out[0, 0])
+
+
+@pytest.mark.parametrize('heads,kv,dim,lengths', [(4, 2, 64, [300, 5, 3000]), (6, 2, 128, [40, 1200]), (2, 2, 64, [70] * 66)])
+@pytest.mark.parametrize('size', [2.0 ** 124, 2.0 ** -100])
+def test_values_of_any_size(device, heads, kv, dim, lengths, size):
+    """bf16 values near the type's largest and smallest: no sum on the way passes 32 bits' range where the output does not."""
+    announce('paged values of any size', heads, kv, dim, size)
+    page = 64
+    pages = sum(-(-n // page) for n in lengths) + 1
+    cache = filled(device, 'bf16', pages, kv, page, dim, seed=41)
+    cache.values.mul_(size)
+    table, position = table_of(device, lengths, page, pages), [n - 1 for n in lengths]
+    q = rand(device, 'bf16', len(lengths), heads, dim, seed=42)
+    out = lb.paged_attention(q, cache, table, ints(position, device))
+    check(out, q, cache, table.cpu(), position, dim ** -0.5, 'bf16')
+    if size > 1:
+        top = torch.finfo(torch.bfloat16).max
+        cache.values.fill_(top)
+        out = lb.paged_attention(q, cache, table, ints(position, device))
+        assert bool((out == top).all())

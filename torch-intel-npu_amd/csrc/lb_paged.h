@@ -147,10 +147,13 @@ constexpr int kUnit = 2 * kChunk;     // slots of a wave's step
 constexpr int kPagedParts = 1024, kPagedPlaces = 2 * kPagedParts + 2;
 constexpr int kPagedWhole = 16 * kUnit;   // slots of a sequence up to which it is never split
 constexpr float kPagedLowest = -3.402823466e38f;
-// Probabilities are taken relative to a reference 2^kPagedLift below a row's running maximum when it was set, and it is
-// set anew where a score exceeds it by kPagedLift + kPagedSlack (units of log2): fp16 then has the probabilities in
-// [2^-24, 2^14], of which the smallest are 2^-34 of the largest.
-constexpr float kPagedLift = 10.0f, kPagedSlack = 4.0f;
+// Probabilities are taken relative to a reference kPagedLift below a row's running maximum when it was set, and it is set anew where
+// a score exceeds it by kPagedLift + kPagedSlack (units of log2).  fp16 then has the probabilities in [2^-24, 2^14], of which the
+// smallest are 2^-34 of the largest.  bf16 has exponents enough, and takes them up to 2^-20: the values of 2^20 slots, whatever their
+// size, stay in the range of a sum.
+template <class T> constexpr float kPagedLift = 10.0f;
+template <> inline constexpr float kPagedLift<bf16> = -24.0f;
+constexpr float kPagedSlack = 4.0f;
 
 // Sum over the wave's lanes.
 __device__ __forceinline__ uint32_t lanes_sum(uint32_t x) { return __builtin_amdgcn_readlane(kv_scan(x), 63); }
@@ -446,10 +449,10 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
     for (int t = 0; t < C; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) top = fmaxf(top, s[t][e]);
-    if (__any(top - ref > kPagedLift + kPagedSlack)) {
+    if (__any(top - ref > kPagedLift<T> + kPagedSlack)) {
       // (Where a score's own step is 16, from 2^27 on, the difference rounds to one past what fp16 has room for.)
-      const float largest = kv_max_across(top), below = largest - kPagedLift;
-      const float raised = fmaxf(ref, largest - below > kPagedLift + kPagedSlack ? largest : below);
+      const float largest = kv_max_across(top), below = largest - kPagedLift<T>;
+      const float raised = fmaxf(ref, largest - below > kPagedLift<T> + kPagedSlack ? largest : below);
       const float shrink = __builtin_amdgcn_exp2f(ref - raised);
       ref = raised;
       total *= shrink;
