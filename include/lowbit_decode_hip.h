@@ -492,6 +492,7 @@ typedef struct lb_rotary_args {
  * formed and reduced in 64 bits, so positions of any size (up to 2^53, below zero too) are as exact as the frequencies.
  * Replaces the RoPE gather of the reference's graphs (torch_npu_smollm.py:262-303), whose tables and products are fp16,
  * for any position, type, pairing, part of the head and scaling.  Fastest where rows are whole 16-byte pieces.
+ * q, k, out and out_k may be slices of one tensor, as long as no row that is written is one of another (but for q and k in place).
  */
 lb_status lb_rotary(const lb_rotary_args *args, void *stream);
 

@@ -70,31 +70,25 @@ extern "C" lb_status lb_rotary(const lb_rotary_args *a, void *stream) {
   }
   if (const lb_status st = check_array(what, "position", a->position, (size_t)(a->per_row ? a->batch * a->seq : a->batch) * 8, 8, true, reads[2]); st != LB_OK) return st;
   if (const lb_status st = check_rotation(what, a->rotation, a->head_dim, true, reads[3]); st != LB_OK) return st;
-  // In place: out is q's rows and out_k k's, which may lie between one another (slices of one projection's rows).
+  // In place: out is q's rows and out_k k's.  What is written and read may else be slices of one tensor that lie between one another.
   const bool q_same = same_rows(a->q, a->out, a->batch, a->seq, a->heads);
   const bool k_same = !a->k_heads || same_rows(a->k, a->out_k, a->batch, a->seq, a->k_heads);
   const bool in_place = q_same && k_same;
+  if (!in_place && q_same != k_same && a->k_heads) return fail(LB_INVALID_ARGUMENT, "%s: q and k are turned in place both or neither", what);
+  if (const lb_status st = check_apart(what, writes, 1, reads + 2, 2); st != LB_OK) return st;
+  if (const lb_status st = check_apart(what, writes + 1, 1, reads + 2, 2); st != LB_OK) return st;
+  auto apart = [&](const lb_rows &x, int64_t x_heads, const lb_rows &y, int64_t y_heads) {
+    return rows_apart(x, x_heads, y, y_heads, a->batch, a->seq, a->head_dim, size);
+  };
   if (in_place) {
-    if (a->k_heads) {                     // interleaved slices of one tensor share its range, but not its rows
-      if (overlaps(writes[0], writes[1])) {
-        const uintptr_t apart = writes[0].lo < writes[1].lo ? writes[1].lo - writes[0].lo : writes[0].lo - writes[1].lo;
-        const lb_rows &lower = writes[0].lo < writes[1].lo ? a->q : a->k, &upper = writes[0].lo < writes[1].lo ? a->k : a->q;
-        const int64_t nl = writes[0].lo < writes[1].lo ? a->heads : a->k_heads, nu = writes[0].lo < writes[1].lo ? a->k_heads : a->heads;
-        const int64_t wl = (nl == 1 ? 0 : (nl - 1) * lower.head_stride) + a->head_dim, wu = (nu == 1 ? 0 : (nu - 1) * upper.head_stride) + a->head_dim;
-        const int64_t pitch = a->seq > 1 ? lower.row_stride : lower.batch_stride;
-        const bool pitched = (a->seq == 1 || lower.row_stride == upper.row_stride) && (a->batch == 1 || lower.batch_stride == upper.batch_stride) &&
-                             (a->batch == 1 || a->seq == 1 || lower.batch_stride % lower.row_stride == 0);
-        if (!pitched || apart < (size_t)wl * size || apart + (size_t)wu * size > (size_t)pitch * size)
-          return fail(LB_INVALID_ARGUMENT, "%s: rows of q and k overlap", what);
-      }
-    }
-    const Range others[2] = {reads[2], reads[3]};
-    for (const Range &w : writes)
-      if (const lb_status st = check_apart(what, &w, 1, others, 2); st != LB_OK) return st;
+    if (a->k_heads && !apart(a->q, a->heads, a->k, a->k_heads)) return fail(LB_INVALID_ARGUMENT, "%s: rows of q and k overlap", what);
   } else {
-    if (q_same != k_same && a->k_heads)
-      return fail(LB_INVALID_ARGUMENT, "%s: q and k are turned in place both or neither", what);
-    if (const lb_status st = check_apart(what, writes, 2, reads, 4); st != LB_OK) return st;
+    const struct { const char *name; const lb_rows &rows; int64_t heads; } out[2] = {{"out", a->out, a->heads}, {"out_k", a->out_k, a->k_heads}},
+                                                                          in[2] = {{"q", a->q, a->heads}, {"k", a->k, a->k_heads}};
+    for (int i = 0; i < (a->k_heads ? 2 : 1); ++i)
+      for (int j = 0; j < (a->k_heads ? 2 : 1); ++j)
+        if (!apart(out[i].rows, out[i].heads, in[j].rows, in[j].heads)) return fail(LB_INVALID_ARGUMENT, "%s: %s overlaps %s", what, out[i].name, in[j].name);
+    if (a->k_heads && !apart(a->out, a->heads, a->out_k, a->k_heads)) return fail(LB_INVALID_ARGUMENT, "%s: out_k overlaps out", what);
   }
   auto fits = [&](int V) {
     return a->rotation.dims % (2 * V) == 0 && a->head_dim % V == 0 && in_pieces(a->q, a->batch, a->seq, a->heads, V, size) &&

@@ -41,6 +41,43 @@ inline lb_status check_strided(const char *what, const char *name, const lb_rows
   return range.hi < range.lo ? fail(LB_INVALID_ARGUMENT, "%s: %s does not fit the address space", what, name) : LB_OK;
 }
 
+// Whether two sets of checked rows, of the same batch, seq and dim, share no memory: slices of one tensor lie between one another, but
+// its outer axes (any of batch, seq and heads, which both step through alike) hold them apart in blocks of `upper` behind `lower`.
+inline bool rows_apart(const lb_rows &a, int64_t a_heads, const lb_rows &b, int64_t b_heads, int64_t batch, int64_t seq, int64_t dim, size_t size) {
+  const bool swap = reinterpret_cast<uintptr_t>(b.data) < reinterpret_cast<uintptr_t>(a.data);
+  const lb_rows &lower = swap ? b : a, &upper = swap ? a : b;
+  const size_t bytes = reinterpret_cast<uintptr_t>(upper.data) - reinterpret_cast<uintptr_t>(lower.data);
+  struct Axis { int64_t low, up, low_stride, up_stride; };
+  const Axis axes[3] = {{batch, batch, lower.batch_stride, upper.batch_stride}, {seq, seq, lower.row_stride, upper.row_stride},
+                        {swap ? b_heads : a_heads, swap ? a_heads : b_heads, lower.head_stride, upper.head_stride}};
+  for (int outer = 0; outer < 8; ++outer) {
+    struct { int64_t size, stride; } steps[3];
+    int n = 0;
+    int64_t low = dim, up = dim;         // extents of a block's rows
+    bool alike = true;
+    for (int i = 0; i < 3; ++i) {
+      const Axis &x = axes[i];
+      if (outer >> i & 1) {
+        alike = alike && (x.low == 1 || x.up == 1 || x.low_stride == x.up_stride);
+        if (std::max(x.low, x.up) > 1) steps[n++] = {std::max(x.low, x.up), x.low > 1 ? x.low_stride : x.up_stride};
+      } else {
+        low += x.low == 1 ? 0 : (x.low - 1) * x.low_stride;
+        up += x.up == 1 ? 0 : (x.up - 1) * x.up_stride;
+      }
+    }
+    if (!alike || bytes < (size_t)low * size) continue;
+    std::sort(steps, steps + n, [](const auto &s, const auto &t) { return s.stride < t.stride; });
+    unsigned __int128 extent = bytes + (unsigned __int128)up * size;
+    bool apart = true;
+    for (int i = 0; i < n; ++i) {
+      apart = apart && (unsigned __int128)steps[i].stride * size >= extent;
+      extent += (unsigned __int128)(steps[i].size - 1) * steps[i].stride * size;
+    }
+    if (apart) return true;
+  }
+  return false;
+}
+
 inline lb_status check_array(const char *what, const char *name, const void *p, size_t bytes, size_t align, bool needed, Range &range) {
   range = Range{};
   if (!p && !needed) return LB_OK;

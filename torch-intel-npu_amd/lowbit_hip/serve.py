@@ -262,7 +262,7 @@ def rotary(q, position, rotary, *, k=None, out=None, out_k=None, back=False):
     """lb_rotary: the rows of q [batch, seq, heads, head_dim] (fp16, bf16 or fp32, any strides of contiguous heads) turned by
     their positions, and with k [batch, seq, k_heads, head_dim] its rows too, in one launch.  position: int64 [batch] (row i
     of sequence b lies at position[b] + i) or [batch, seq] (each row's own), on the device.  Into out and out_k, which may be
-    q and k themselves (both or neither); new tensors where they are not given.  back: by the negative angle, still times the
+    q and k themselves (both or neither) or slices of one tensor; new tensors where they are not given.  back: by the negative angle, still times the
     scale, which is the transpose: of an output's gradient it makes the input's (autograd does not record
     the call).  Returns out, or (out, out_k)."""
     if out is None and isinstance(q, torch.Tensor):
