@@ -52,12 +52,14 @@ struct Turn {
 };
 
 // scale cos and scale sin of pair i at a position.  The angle is formed in 64 bits and reduced to a part of a turn there
-// (at position 2^20 a product in 32 bits is off by 0.06); the sine and cosine are 32 bits' own, right to an ulp or two.
+// (at position 2^20 a product in 32 bits is off by 0.06); the sine and cosine are 32 bits' own, right to an ulp or two, and
+// what the part of a turn loses in 32 bits turns them on by itself (so that a small sine is as exact as a large one).
 __device__ __forceinline__ float2 turn_of(const Turn &t, int i, double position) {
-  const double turns = position * t.frequencies[i] * 0.15915494309189533577;
+  const double turns = position * t.frequencies[i] * 0.15915494309189533577, part = 2.0 * (turns - __builtin_rint(turns));
+  const float half_turns = (float)part, rest = 3.14159265358979323846f * (float)(part - (double)half_turns);
   float s, c;
-  sincospif(2.0f * (float)(turns - __builtin_rint(turns)), &s, &c);
-  return make_float2(t.scale * c, t.scale * s);
+  sincospif(half_turns, &s, &c);
+  return make_float2(t.scale * (c - s * rest), t.scale * (s + c * rest));
 }
 
 // First dim of pair i, and how far from it the second one lies.
