@@ -125,6 +125,12 @@ def _rows(t, name, shape, dtype, device, keep, copy):
     return at, b, i, h
 
 
+def _inference(what, *tensors):
+    """No gradient is recorded, so none may be asked for."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f'{what} is inference-only; use no_grad/inference_mode')
+
+
 def _counts(t, name, shape, device):
     if not isinstance(t, torch.Tensor) or t.dtype != torch.int64 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f'{name} must be a contiguous int64 tensor {list(shape)}')
@@ -380,10 +386,12 @@ def _append_args(cache, k, v, table, position, rows, rotary, keep, copy):
     batch, seq, _, _ = k.shape
     device, dtype, dim = cache.device, cache.dtype, cache.head_dim
     shape, counts = (batch, seq, cache.kv_heads, dim), (batch,)
-    return PagedAppendArgs.from_buffer_copy(cache._heads[PagedAppendArgs] + _APPEND.pack(
+    a = PagedAppendArgs.from_buffer_copy(cache._heads[PagedAppendArgs] + _APPEND.pack(
         *_page_table(table, batch, device), batch, seq, *_rows(k, 'k', shape, dtype, device, keep, copy),
         *_rows(v, 'v', shape, dtype, device, keep, copy), _counts(position, 'position', counts, device),
         0 if rows is None else _counts(rows, 'rows', counts, device)) + _rotation(rotary, device, dim))
+    _inference('paged_append', k, v)
+    return a
 
 
 def paged_append(cache, k, v, table, position, *, rows=None, rotary=None):
@@ -391,7 +399,7 @@ def paged_append(cache, k, v, table, position, *, rows=None, rotary=None):
     position[b] .. of each sequence, in the pages that the table gives them.  table: int32 [batch, pages], position and rows:
     int64 [batch], on the device.  With a Rotary the keys are turned by their slots first.  A sequence whose rows do not lie in
     the table's slots is left alone, as are rows whose entry is not a page.  k and v may have any strides (a copy is made where
-    rows are not 16-byte pieces)."""
+    rows are not 16-byte pieces).  Inference only: rows that ask for a gradient are refused."""
     keep = []
     a = _append_args(cache, k, v, table, position, rows, rotary, keep, True)
     _kv_run(library().lb_paged_append, a, cache.device, 'lb_paged_append')
@@ -437,6 +445,7 @@ def _attention_args(q, cache, table, position, out, k, v, rotary, scale, keep, c
         *(_NO_ROWS if k is None else rows(k, 'k', cache.kv_heads, copy)),
         *(_NO_ROWS if v is None else rows(v, 'v', cache.kv_heads, copy)))
         + _rotation(rotary, device, dim) + _ATTENTION_TAIL.pack(scale, 0, 0, 0))
+    _inference('paged_attention', q, k, v, out)
     need = cache._needs.get((batch, heads, longest))
     if need is None:
         need = _needed(library().lb_paged_attention_workspace_bytes, 'lb_paged_attention_workspace_bytes', a)
@@ -452,7 +461,8 @@ def paged_attention(q, cache, table, position, *, k=None, v=None, rotary=None, s
     already, or get here where k and v [batch, kv_heads, head_dim] are given.  position -1: no token, its out is 0; a position
     that does not lie in the table, or a page that there is not, gives NaN.  With a Rotary q (and k) are turned by the position
     first.  table: int32 [batch, pages], position: int64 [batch], on the device; scale: default head_dim ** -0.5.  Any strides of
-    q, k and v (a copy is made where rows are not 16-byte pieces)."""
+    q, k and v (a copy is made where rows are not 16-byte pieces).  Inference only: tensors that ask for a gradient are
+    refused."""
     if out is None and isinstance(q, torch.Tensor):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     keep = []
@@ -584,6 +594,7 @@ def _adapters_args(y, x, adapters, index, out, keep, copy):
         ldx = x.stride(0)
     a = AdaptersArgs.from_buffer_copy(_ADAPTERS.pack(_ADAPTERS.size, TYPES[dtype], M, N, K, adapters.rank, adapters.count, *adapters._at, at,
                                                      x.data_ptr(), ldx, *places[:2], *places[-2:], 0, 0))
+    _inference('adapters_add', x, y, out, adapters.down, adapters.up, adapters.scales)
     need = adapters._needs.get(M)
     if need is None:
         need = _needed(library().lb_adapters_workspace_bytes, 'lb_adapters_workspace_bytes', a)
@@ -596,7 +607,8 @@ def _adapters_args(y, x, adapters, index, out, keep, copy):
 def adapters_add(y, x, adapters, index, *, out=None):
     """lb_adapters: adds to the rows of y [M, N], a projection of x [M, K], what the adapter of each adds to it:
     y[m] + scales[a] (x[m] . down[a]^T) . up[a]^T with a = index[m] (int64 on the device; -1: none, the row stays; any other
-    number that is no adapter: NaN).  In place, or into out."""
+    number that is no adapter: NaN).  In place, or into out.  Inference only: tensors and factors that ask for a gradient are
+    refused."""
     out = y if out is None else out
     keep = []
     a, need = _adapters_args(y, x, adapters, index, out, keep, True)
