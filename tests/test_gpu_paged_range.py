@@ -98,3 +98,21 @@ def test_values_of_any_size(device, heads, kv, dim, lengths, size):
         cache.values.fill_(top)
         out = lb.paged_attention(q, cache, table, ints(position, device))
         assert bool((out == top).all())
+
+
+@pytest.mark.parametrize('dim,whole', [(64, 1024), (128, 512)])
+@pytest.mark.parametrize('batch', [3, 70])
+def test_about_the_longest_that_is_not_split(device, dim, whole, batch):
+    """Tables of as many slots as are never split, which take no workspace, and of a page more."""
+    announce('paged whole', dim, batch)
+    page = 16
+    for slots in (whole, whole + page):
+        lengths = [slots, slots - 15, 1] + [1 + (b * 7919) % slots for b in range(batch - 3)]
+        pages = sum(-(-n // page) for n in lengths) + 1
+        cache, table = filled(device, 'fp16', pages, 2, page, dim, seed=51), table_of(device, lengths, page, pages)
+        assert table.shape[1] * page == slots
+        q, position = rand(device, 'fp16', batch, 6, dim, seed=52), [n - 1 for n in lengths]
+        call = lb.PreparedPagedAttention(q, cache, table, ints(position, device), torch.zeros_like(q))
+        assert (call.scratch is None) == (slots == whole)
+        call.run()
+        check(call.out, q, cache, table.cpu(), position, dim ** -0.5, 'fp16')

@@ -145,7 +145,8 @@ constexpr int kUnit = 2 * kChunk;     // slots of a wave's step
 // Parts that the whole work is split into at the most, besides those that sequences and heads are by themselves, and places
 // for the sums of parts.
 constexpr int kPagedParts = 1024, kPagedPlaces = 2 * kPagedParts + 2;
-constexpr int kPagedWhole = 16 * kUnit;   // slots of a sequence up to which it is never split
+// Slots of a sequence up to which it is never split (the host leaves out what only splitting needs).
+constexpr int paged_whole(int dim) { return (dim == 64 ? 32 : 16) * kUnit; }
 constexpr float kPagedLowest = -3.402823466e38f;
 // Probabilities are taken relative to a reference kPagedLift below a row's running maximum when it was set, and it is set anew where
 // a score exceeds it by kPagedLift + kPagedSlack (units of log2).  fp16 then has the probabilities in [2^-24, 2^14], of which the
@@ -195,9 +196,9 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 
-  // Units of a sequence: those of its slots, none where there is no token, one where it lies outside (to write NaNs).
+  // Units of a sequence: those of its slots, one where there is no token or it lies outside (to write zeros or NaNs).
   const int64_t slots = p.c.slots();
-  auto units_of = [&](int64_t at) -> uint32_t { return at < 0 ? 1 : at >= slots ? 1 : (uint32_t)(at / UNIT) + 1; };
+  auto units_of = [&](int64_t at) -> uint32_t { return at < 0 || at >= slots ? 1 : (uint32_t)(at / UNIT) + 1; };
   const uint32_t heads = p.c.kv_heads * p.tiles, hh = blockIdx.x % heads, ticket = blockIdx.x / heads;
   const int h = hh / p.tiles, tile = hh % p.tiles;
   const int64_t at0 = lane < p.batch ? p.position[lane] : 0;
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
   // slots, read at that rate too: the two are even where a part has sqrt(units x query heads / 32) units (16 heads of 128 over one KV
   // head, a sequence of 60001 slots: 39.7 -> 25.3 us; 24 of 64, two of up to 26499: 15.0 -> 13.5).
   constexpr int kRound = 256 * 8 / W;
-  constexpr uint32_t kWhole = (D == 64 ? 2 : 1) * kPagedWhole / kUnit, kLeast = 8;
+  constexpr uint32_t kWhole = paged_whole(D) / kUnit, kLeast = 8;
   uint32_t most = kWhole;
   if (p.batch > 64) {
     most = max((uint32_t)(((uint64_t)all * heads + kRound * p.rounds - 1) / (kRound * p.rounds)), most);

@@ -77,7 +77,7 @@ AttendPlan attend_plan(const lb_paged_attention_args *a) {
   plan.waves = c.head_dim == 128 && pairs > 256 ? 4 : 8;
   // A workgroup per sequence and head, and where sequences can be long enough the rounds of 256 or 512 that they can be split into:
   // few sequences are split evenly in one, more of them need more to end together.
-  const bool split = a->table.longest * c.page > kPagedWhole;
+  const bool split = a->table.longest * c.page > paged_whole((int)c.head_dim);
   plan.rounds = pairs <= 128 ? 1 : kPagedParts / (256 * 8 / plan.waves);
   plan.grid = pairs + (split ? plan.rounds * (256 * 8 / plan.waves) : 0);
   plan.grid = (plan.grid + heads - 1) / heads * heads;   // whole tickets
