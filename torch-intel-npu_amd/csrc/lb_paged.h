@@ -462,16 +462,17 @@ __global__ __launch_bounds__(64 * W) void paged_attend_kernel(PagedAttendParams<
     }
     // A probability enters the product as the sum of two numbers of the type, for its rounding to one (2^-8 of it in bf16, 2^-11 in fp16)
     // is as large as the output's own, and larger where values cancel (one sequence of 130999 slots, 8 heads of 128, bf16: 86.0 -> 86.4
-    // us; 32 of up to 1984, 3 of 64, fp16: 11.3 -> 11.5; 64 of up to 8192, 8 of 128, fp16: 178.4 -> 178.3).
+    // us; 32 of up to 1984, 3 of 64, fp16: 11.35 -> 11.45; 4 of 1000: 10.8 -> 11.1; 64 of up to 8192, 8 of 128: 177.1 -> 178.2).  fp16's first
+    // number is cut off rather than rounded, which leaves the second as exact and needs no conversion back (4 of 1000: 11.2 -> 11.1).
     x8 x[C / 2], rest[C / 2];
 #pragma unroll
     for (int t = 0; t < C; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float prob = __builtin_amdgcn_exp2f(s[t][e] - ref);
-        const T high = (T)prob;
-        x[t / 2][t % 2 * 4 + e] = high;
-        rest[t / 2][t % 2 * 4 + e] = (T)(prob - (float)high);
+        const float high = __is_same(T, f16) ? __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, prob) & 0xFFFFE000u) : (float)(T)prob;
+        x[t / 2][t % 2 * 4 + e] = (T)high;
+        rest[t / 2][t % 2 * 4 + e] = (T)(prob - high);
         total += prob;
       }
 #pragma unroll
