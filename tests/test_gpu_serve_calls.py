@@ -118,3 +118,21 @@ def test_replays_beside_eager_calls(device):
             eager.append(lb.paged_attention(q, cache, table, position))
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all(torch.equal(e, want) for e in eager)
+
+
+def test_workspaces_that_are_none(device):
+    """Too short, of another type, of bytes that do not lie side by side (an expanded byte is one), or at any address: refused when the call
+    is prepared."""
+    announce('serve workspaces')
+    cache, table = filled(device, 'fp16', 70, 2, 16, 128, seed=70), table_of(device, [1000], 16, 70)
+    q, position = rand(device, 'fp16', 1, 4, 128), ints([999], device)
+    prepare = lambda workspace: lb.PreparedPagedAttention(q, cache, table, position, torch.zeros_like(q), workspace=workspace)
+    need = prepare(None).scratch.numel()
+    zeros = lambda n, dtype=torch.uint8: torch.zeros(n, dtype=dtype, device=device)
+    for bad in (zeros(need - 1), zeros(need, torch.int8), zeros(1).expand(need), zeros(2 * need)[::2], zeros(need + 16)[16:], torch.zeros(need, dtype=torch.uint8),
+                need):
+        with pytest.raises(ValueError, match='workspace must'):
+            prepare(bad)
+    call = prepare(zeros(need + 256)[256:])
+    call.run()
+    check(call.out, q, cache, table.cpu(), [999], 128 ** -0.5, 'fp16')

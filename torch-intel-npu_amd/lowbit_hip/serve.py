@@ -485,8 +485,9 @@ class PreparedPagedAttention(_PreparedKV):
         if need:
             if workspace is None:
                 workspace = _kv_new_workspace(need, cache.device)
-            elif workspace.device != cache.device or workspace.dtype != torch.uint8 or workspace.numel() < need:
-                raise ValueError(f'the workspace must have {need} bytes on {cache.device}')
+            elif (not isinstance(workspace, torch.Tensor) or workspace.device != cache.device or workspace.dtype != torch.uint8
+                  or workspace.numel() < need or not workspace.is_contiguous() or workspace.data_ptr() % 256):
+                raise ValueError(f'the workspace must be {need} contiguous bytes (uint8) at a 256-byte address on {cache.device}')
             keep.append(workspace)
             a.workspace, a.workspace_bytes = workspace.data_ptr(), need
         self._bind('lb_paged_attention', 'lb_paged_attention', a, cache.device, keep)
