@@ -168,18 +168,14 @@ class SmolBatchDecoder:
         place, need = self._held.index(None), -(-(s + steps) // self.page)
         if need > len(self._free):
             raise ValueError(f'{need} pages are needed and {len(self._free)} are free')
-        taken = [self._free.pop() for _ in range(need)]
+        taken = self._free[:-need - 1:-1]               # (theirs only once the prompt is in them, whatever ends it)
         row = torch.tensor([taken], dtype=torch.int32, device=self.device)
-        try:
-            h = self._prompt(self.io.embed_tokens(ids), adapter, row)
-            token = self.io.logits(h)[0, 0].argmax()
-        except Exception:
-            self._free += taken
-            raise
+        token = self.io.logits(self._prompt(self.io.embed_tokens(ids), adapter, row))[0, 0].argmax()
+        del self._free[-need:]
+        self._held[place] = [taken, steps]
         self.table[place, :need] = row[0]
         self.table[place, need:] = -1
         self.position[place], self.index[place], self.tokens[place] = s, adapter, token
-        self._held[place] = [taken, steps]
         return place
 
     @torch.no_grad()
