@@ -39,8 +39,8 @@ struct PagedAppendParams {
 // turned in LDS into the 16 bytes that 8 slots of a dim are, so that both sides move whole lines; the chunk's sines and cosines are
 // computed behind their loads, once for all heads, into LDS; then keys, 8 dims of a row a thread.  (One loop body for every
 // key: straight-line code of four rows took a short call as long to fetch as to run.)  Memory bounds it where rows are many: prompts
-// of 4100, 3476, 2526 and 951 rows of 8 heads of 128, bf16, 90 MB in and out, take 20.5 us (4.4 TB/s).  500 rows of 3 heads
-// of 64 take 5.5: the launch, and the positions, the table and the rows one after the other.
+// of 4100, 3476, 2526 and 951 rows of 8 heads of 128, bf16, 90 MB in and out, take 20.9 us (4.3 TB/s).  500 rows of 3 heads
+// of 64 take 4.3: the launch, and the positions, the table and the rows one after the other.
 template <class T, int D, int NT>
 __global__ __launch_bounds__(NT) void paged_append_kernel(PagedAppendParams<T> p) {
   typedef typename Of16<T>::x8 x8;
@@ -175,9 +175,16 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
 // the workgroup that counts last.  Which part it takes is found from the positions, on the device.
 //
 // Memory bounds it where the slots are many, 16-bit keys and values read once: one sequence of 130999 slots, 8 heads of 128, takes
-// 86.3 us (6.2 TB/s), 64 of up to 8193 178 us (6.1).  The products take K (as rows of 16 slots) and V (as rows of 16 dims) straight from
+// 86.5 us (6.2 TB/s), 64 of up to 8193 178 us (6.1).  The products take K (as rows of 16 slots) and V (as rows of 16 dims) straight from
 // their pages, and P comes out of one as the operand of the other, so LDS holds only what waves exchange.  Few slots cost the
-// chain of loads (positions, table, keys and values: 5.7 us for 150), and parts another 4 us (sums out, count, sums in).
+// chain of loads (positions, table, keys and values: 5.8 us for 150), and parts another 4 us (sums out, count, sums in).
+//
+// Batches of more than 64 keep a simpler plan, parts of a 1024th of the work but never of sequences that are short, and every workgroup
+// goes through the positions up to its own: as the square of the batch where sequences are short (3 heads of 64, up to 60 slots: 64, 256,
+// 1024 and 4096 sequences 5.2, 11.0, 55.7, 534 us), hardly where they are long (8 heads of 128, up to 2000 slots: 64, 128 and 256
+// sequences 53.0, 95.6, 173 us; 64 and 65 with one of 60001 slots, 16 query heads over one of 128, 25.3, 27.0).  Of more than 16 query
+// heads a KV head, each tile of 16 reads the slots anew, side by side, the second time mostly from the caches (131000 slots, one
+// head of 64: 16 and 24 query heads 20.6, 22.1 us).
 //
 // TURNED: queries are turned by their position (and the new key).  A turned query enters the product as the sum of two numbers of
 // the type, so that its rounding (2^-8 of bf16, which large scores would pass on whole) is not added to the held keys'.

@@ -25,6 +25,9 @@ class SmolBatchDecoder:
     adapters: None, or one dict per layer of projection weight names to lowbit_hip.Adapters (fp16, all of one count): a
     request takes one of their numbers, or none.  graph=False runs every step eagerly.
 
+    A prompt without an adapter runs through the layers as they are, keys turned by their fp16 tables; one with an adapter has its keys turned
+    by lb_rotary, as every step has.
+
     admit() prefills a request into a free place, step() gives every request its next token, release() frees a place.
     tokens holds the last token of each place (int64 on the device, -1 where there is no request), logits the last step's.
     """
